@@ -1,0 +1,308 @@
+"""Timed cases of the entity-prediction operators: the scaled embedding lookup with its gradient by sorted ids, the
+distillation loss against a teacher's top logits, and the microscaled 4-bit table (quantisation and product).
+
+Each case describes one call of a knowledge-graph embedding model that predicts an entity out of all entities of the
+graph: ``embed`` looks up query rows (and returns the table's gradient), ``distill`` is the loss over the entity logits,
+``quantize`` packs a table into 4 bits and reads it back, ``linear`` multiplies rows with a packed table.
+
+``run`` computes the plain form in elementary torch operations (``own = False``) or makes the framework's calls
+(``own = True``) on what ``prepare`` made; ``exact`` computes the same outputs in 64 bits.
+"""
+import math
+
+import torch
+
+own = False
+
+_TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+_BYTES = {"fp32": 4, "bf16": 2, "fp16": 2}
+_BLOCK = 32                                       # values that share one scale in the 4-bit table
+
+
+def listed():
+    return [
+        # the rows of one batch of queries (batch_size 128) out of the full graph's entity table, at inference: latency
+        {"name": "embed_batch", "op": "embed", "rows": 130000, "dim": 256, "ids": 128, "dtype": "fp32", "train": False},
+        # a training batch over the synthetic graph's 5000 entities with 768-wide features, odd count, padded ids
+        {"name": "embed_step", "op": "embed", "rows": 5000, "dim": 768, "ids": 1021, "dtype": "fp32", "train": True},
+        # the endpoints of a large batch of edges: a million lookups with the hubs of a biomedical graph
+        {"name": "embed_edges", "op": "embed", "rows": 130000, "dim": 256, "ids": 1000003, "dtype": "bf16", "train": True},
+        # a small step: 16 queries over the synthetic graph's entities, the teacher's ten best
+        {"name": "distill_small", "op": "distill", "rows": 16, "vocab": 5000, "k": 10, "dtype": "fp32", "train": True},
+        # validation loss of an odd number of queries over a part of the entities (one node type), half precision
+        {"name": "distill_valid", "op": "distill", "rows": 1021, "vocab": 32771, "k": 32, "dtype": "fp16", "train": False},
+        # one batch (128) over all entities with fp32 logits, as the decoder's product writes them
+        {"name": "distill_batch", "op": "distill", "rows": 128, "vocab": 130000, "k": 64, "dtype": "fp32", "train": True},
+        # the largest step: 4096 queries over all entities in bf16
+        {"name": "distill_large", "op": "distill", "rows": 4096, "vocab": 130000, "k": 100, "dtype": "bf16", "train": True},
+        # a batch of odd-shaped fp32 activations packed and read back
+        {"name": "quantize_batch", "op": "quantize", "rows": 1021, "cols": 770, "dtype": "fp32"},
+        # the full graph's 768-wide feature table, once per set of weights
+        {"name": "quantize_table", "op": "quantize", "rows": 130000, "cols": 768, "dtype": "bf16"},
+        # serving: one query against every entity
+        {"name": "linear_query", "op": "linear", "rows": 1, "cols": 256, "outs": 130000, "dtype": "bf16", "out": "fp32",
+         "bias": False},
+        # evaluation: an odd batch of queries against every entity, the logits written in bf16
+        {"name": "linear_entities", "op": "linear", "rows": 1021, "cols": 256, "outs": 130000, "dtype": "bf16",
+         "out": "bf16", "bias": False},
+        # a large square projection, bound by the matrix units
+        {"name": "linear_large", "op": "linear", "rows": 8192, "cols": 8192, "outs": 8192, "dtype": "bf16", "out": "bf16",
+         "bias": True},
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A whole number between lo and hi, spread over its logarithm."""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["embed", "embed", "distill", "distill", "quantize", "linear", "linear"])
+    dtype = rng.choice(["fp32", "bf16", "fp16"])
+    while True:
+        if op == "embed":
+            case = {"op": op, "rows": _spread(rng, 32, 130000), "dim": _spread(rng, 8, 1024), "ids": _spread(rng, 1, 1000003),
+                    "dtype": dtype, "train": rng.random() < 0.7}
+            if rng.random() < 0.5:
+                case["dim"] = max(8, case["dim"] // 64 * 64)
+            top = listed()[2]
+        elif op == "distill":
+            case = {"op": op, "rows": _spread(rng, 1, 4096), "vocab": _spread(rng, 33, 200000), "dtype": dtype,
+                    "k": _spread(rng, 1, 128), "train": rng.random() < 0.7}
+            case["k"] = min(case["k"], case["vocab"] // 2)
+            top = listed()[6]
+        elif op == "quantize":
+            case = {"op": op, "rows": _spread(rng, 1, 130000), "cols": _spread(rng, 8, 2048), "dtype": dtype}
+            top = listed()[8]
+        else:
+            case = {"op": op, "rows": _spread(rng, 1, 8192), "cols": _spread(rng, 24, 8192), "outs": _spread(rng, 16, 130000),
+                    "dtype": dtype, "out": rng.choice(["fp32", "bf16"]), "bias": rng.random() < 0.5}
+            top = listed()[11]
+        mine, most = work(case), work(top)
+        # (an output-bound product may move as many bytes as the largest distillation step)
+        bytes_most = max(most["bytes"], work(listed()[6])["bytes"] // 4) if op == "linear" else most["bytes"]
+        if mine["bytes"] <= bytes_most and mine["flops"] <= most["flops"]:
+            return case
+
+
+def work(case):
+    e = _BYTES[case["dtype"]]
+    if case["op"] == "embed":
+        n, d, v = case["ids"], case["dim"], case["rows"]
+        moved = 8 * n + min(n, v) * d * e + n * d * e            # ids, the rows looked up, the result
+        if case["train"]:
+            moved += n * d * e + v * d * e                       # the result's gradient, the table's gradient
+        return {"bytes": moved, "flops": n * d * (2 if case["train"] else 1)}
+    if case["op"] == "distill":
+        r, v, k = case["rows"], case["vocab"], case["k"]
+        moved = r * v * e + r * k * 12 + 4
+        if case["train"]:
+            moved += r * v * e
+        return {"bytes": moved, "flops": r * v * (7 if case["train"] else 4)}
+    packed = 0.5 + 1.0 / _BLOCK
+    if case["op"] == "quantize":
+        n = case["rows"] * case["cols"]
+        return {"bytes": int(n * (e + packed) + n * (packed + e)), "flops": 4 * n}
+    m, k, n = case["rows"], case["cols"], case["outs"]
+    moved = m * k * e + n * k * packed + m * n * _BYTES[case["out"]] + (4 * n if case["bias"] else 0)
+    return {"bytes": int(moved), "flops": 2 * m * n * k}
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(int(seed))
+    dtype = _TYPES[case["dtype"]]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=gen, device="cuda", dtype=torch.float32)
+
+    def uniform(*shape):
+        return torch.rand(*shape, generator=gen, device="cuda", dtype=torch.float32)
+
+    def whole(lo, hi, *shape):
+        return torch.randint(lo, hi, shape, generator=gen, device="cuda")
+
+    if case["op"] == "embed":
+        v, d, n = case["rows"], case["dim"], case["ids"]
+        # degrees of a biomedical graph: a few hubs take a percent of the lookups each
+        ids = (uniform(n).double().pow(3) * v).long().clamp_(max=v - 1)
+        step = next(s for s in (7919, 7907, 7901) if math.gcd(s, v) == 1)
+        ids = (ids * step + 13) % v
+        ids = torch.where(whole(0, 50, n) == 0, torch.full_like(ids, v - 1), ids)      # padded places
+        state = {"weight": (normal(v, d) * 0.05).to(dtype), "ids": ids, "scale": math.sqrt(d), "pad": v - 1}
+        if case["train"]:
+            state["grad"] = normal(n, d).to(dtype)
+    elif case["op"] == "distill":
+        r, v, k = case["rows"], case["vocab"], case["k"]
+        logits = normal(r, v).mul_(2.0)
+        known = whole(0, v, r, max(1, v // 1000))                 # known answers, filtered out of the student's logits
+        logits.scatter_(1, known, float("-inf"))
+        start = whole(0, v, r, 1)
+        ids = (start + torch.cumsum(whole(1, v // k + 1, r, k), 1)) % v            # k different entities per row
+        rank = torch.arange(k, device="cuda", dtype=torch.float32)
+        teacher = 8.0 - 2.0 * torch.log1p(rank) - 0.1 * uniform(r, k)
+        logits.scatter_(1, ids, 0.5 * teacher + normal(r, k))
+        row = torch.arange(r, device="cuda")[:, None]
+        place = torch.arange(k, device="cuda")[None, :]
+        left_out = (row % 17 == 5) | ((row % 7 == 3) & (place >= k - k // 3))      # queries with no or few answers
+        state = {"logits": logits.to(dtype), "teacher_ids": torch.where(left_out, torch.full_like(ids, -1), ids),
+                 "teacher_logits": teacher, "temperature": 2.0}
+    elif case["op"] == "quantize":
+        x = normal(case["rows"], case["cols"])
+        state = {"x": (x * torch.exp(1.5 * normal(case["rows"], 1))).to(dtype)}
+    else:
+        m, k, n = case["rows"], case["cols"], case["outs"]
+        x, w = normal(m, k).to(dtype), (normal(n, k) / math.sqrt(k)).to(dtype)
+        state = {"x": x, "bias": normal(n) if case["bias"] else None, "out": _TYPES[case["out"]]}
+        if own:
+            from biomedkg_amd import ops
+            state["table"] = ops.mx4_quantize(w)                  # a served table is packed once
+        else:
+            state["table"] = _packed_values(w)
+    state["op"], state["train"] = case["op"], case.get("train", False)
+    return state
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+def _packed_values(x):
+    """The values that the 4-bit table holds for ``x`` (fp32): blocks of 32 along the row share a power of two, the
+    largest not above the block's largest magnitude divided by 4; values are rounded to the nearest of
+    0, .5, 1, 1.5, 2, 3, 4, 6 (ties to the even code)."""
+    rows, cols = x.shape
+    blocks = (cols + _BLOCK - 1) // _BLOCK
+    f = torch.zeros(rows, blocks * _BLOCK, dtype=torch.float32, device=x.device)
+    f[:, :cols] = x
+    f = f.view(rows, blocks, _BLOCK)
+    largest = f.abs().amax(2, keepdim=True)
+    _, e = torch.frexp(largest)
+    e = (torch.where(largest > 0, e - 1, torch.full_like(e, -200)) - 2).clamp(-127, 127)
+    y = torch.ldexp(torch.ldexp(f, -(e // 2)), -(e - e // 2))
+    a = y.abs()
+    step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
+    a = (torch.round(a / step) * step).clamp(max=6.0)
+    q = torch.ldexp(torch.ldexp(torch.copysign(a, y), e // 2), e - e // 2)
+    q = torch.where(torch.isfinite(largest), q, torch.full_like(q, float("nan")))
+    return q.view(rows, -1)[:, :cols]
+
+
+def _plain(s):
+    if s["op"] == "embed":
+        w, ids = s["weight"], s["ids"]
+        out = (w[ids].float() * s["scale"]).to(w.dtype)
+        if not s["train"]:
+            return out
+        g = s["grad"].float() * (ids != s["pad"])[:, None]
+        dw = torch.zeros(w.shape, dtype=torch.float32, device=w.device).index_add_(0, ids, g) * s["scale"]
+        return out, dw.to(w.dtype)
+    if s["op"] == "distill":
+        t, ids = s["temperature"], s["teacher_ids"]
+        z = s["logits"].float() / t
+        lse = torch.logsumexp(z, 1, keepdim=True)
+        real = ids >= 0
+        tv = torch.where(real, s["teacher_logits"].float() / t, float("-inf"))
+        used = real.any(1, keepdim=True)
+        top = torch.where(used, tv.amax(1, keepdim=True), 0.0)
+        mass = torch.exp(tv - top)
+        total = torch.where(used, mass.sum(1, keepdim=True), 1.0)
+        q = mass / total
+        at = torch.gather(z, 1, ids.clamp(min=0))
+        terms = torch.where(q > 0, q * ((tv - top - torch.log(total)) - (at - lse)), 0.0)
+        rows = ids.size(0)
+        loss = terms.sum() * (t * t) / rows
+        if not s["train"]:
+            return loss
+        d = torch.exp(z - lse) * used
+        d.scatter_add_(1, ids.clamp(min=0), -q)
+        return loss, (d * (t / rows)).to(s["logits"].dtype)
+    if s["op"] == "quantize":
+        return _packed_values(s["x"]).to(s["x"].dtype)
+    y = _packed_values(s["x"]) @ s["table"].t()
+    return (y if s["bias"] is None else y + s["bias"]).to(s["out"])
+
+
+def run(state):
+    if not own:
+        return _plain(state)
+    from biomedkg_amd import ops
+    s = state
+    if s["op"] == "embed":
+        if not s["train"]:
+            return ops.embedding(s["weight"], s["ids"], scale=s["scale"], padding_idx=s["pad"])
+        w = s["weight"].detach().requires_grad_()
+        out = ops.embedding(w, s["ids"], scale=s["scale"], padding_idx=s["pad"])
+        out.backward(s["grad"])
+        return out.detach(), w.grad
+    if s["op"] == "distill":
+        if not s["train"]:
+            return ops.topk_distill_loss(s["logits"], s["teacher_ids"], s["teacher_logits"], s["temperature"])
+        x = s["logits"].detach().requires_grad_()
+        loss = ops.topk_distill_loss(x, s["teacher_ids"], s["teacher_logits"], s["temperature"])
+        loss.backward()
+        return loss.detach(), x.grad
+    if s["op"] == "quantize":
+        return ops.mx4_dequantize(ops.mx4_quantize(s["x"]), s["x"].dtype)
+    return ops.mx4_linear(s["x"], s["table"], bias=s["bias"], out_dtype=s["out"])
+
+
+# ------------------------------------------------------------------------------------------------ 64-bit values
+def _nearest(x):
+    """What the 4-bit table holds for ``x``, in 64 bits: the block's exponent from a logarithm that is put right by
+    comparison, every value moved to the nearer of its two neighbours in the list."""
+    rows, cols = x.shape
+    out = torch.empty(rows, cols, dtype=torch.float64, device=x.device)
+    grid = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64, device=x.device)
+    for c in range(0, cols, _BLOCK):
+        b = x[:, c:c + _BLOCK].double()
+        m = b.abs().max(1, keepdim=True).values
+        e = torch.floor(torch.log2(m.clamp(min=1e-300)))
+        e = e + (torch.pow(2.0, e + 1) <= m).double() - (torch.pow(2.0, e) > m).double()
+        s = torch.pow(2.0, (e - 2).clamp(-127, 127))
+        a = (b.abs() / s).clamp(max=6.0)
+        hi = torch.searchsorted(grid, a.contiguous()).clamp(1, 7)
+        below, above = a - grid[hi - 1], grid[hi] - a
+        up = (above < below) | ((above == below) & (hi % 2 == 0))
+        out[:, c:c + _BLOCK] = torch.where(up, grid[hi], grid[hi - 1]) * torch.sign(b) * s
+    return out
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "embed":
+        w, ids = s["weight"], s["ids"]
+        out = w.double()[ids] * s["scale"]
+        if not case["train"]:
+            return out
+        g = s["grad"].double()
+        keep = ids != s["pad"]
+        dw = torch.zeros(w.shape, dtype=torch.float64, device=w.device)
+        dw.index_add_(0, ids[keep], g[keep])
+        return out, dw * s["scale"]
+    if case["op"] == "distill":
+        t, rows = s["temperature"], case["rows"]
+        loss = 0.0
+        grad = torch.zeros(rows, case["vocab"], dtype=torch.float64, device="cuda") if case["train"] else None
+        for lo in range(0, rows, 256):
+            z = s["logits"][lo:lo + 256].double() / t
+            ids, tv = s["teacher_ids"][lo:lo + 256], s["teacher_logits"][lo:lo + 256].double() / t
+            real = ids >= 0
+            full = real.any(1)
+            z, ids, tv, real = z[full], ids[full], tv[full], real[full]
+            log_p = torch.log_softmax(z, 1)
+            log_q = torch.log_softmax(tv.masked_fill(~real, float("-inf")), 1)
+            q = log_q.exp()
+            gap = log_q - log_p.gather(1, ids.clamp(min=0))
+            loss = loss + (q * gap.masked_fill(~real, 0.0)).sum() * t * t / rows
+            if grad is not None:
+                d = log_p.exp()
+                d.scatter_add_(1, ids.clamp(min=0), -q)
+                grad[lo:lo + 256][full] = d * t / rows
+        return loss if grad is None else (loss, grad)
+    if case["op"] == "quantize":
+        return _nearest(s["x"])
+    gen = torch.Generator(device="cuda").manual_seed(int(seed))
+    m, k, n = case["rows"], case["cols"], case["outs"]
+    dtype = _TYPES[case["dtype"]]
+    x = torch.randn(m, k, generator=gen, device="cuda").to(dtype)
+    w = (torch.randn(n, k, generator=gen, device="cuda") / math.sqrt(k)).to(dtype)
+    y = _nearest(x) @ _nearest(w).t()
+    return y if s["bias"] is None else y + s["bias"].double()
