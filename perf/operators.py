@@ -29,7 +29,7 @@ def listed():
         {"name": "embed_edges", "op": "embed", "rows": 130000, "dim": 256, "ids": 1000003, "dtype": "bf16", "train": True},
         # a small step: 16 queries over the synthetic graph's entities, the teacher's ten best
         {"name": "distill_small", "op": "distill", "rows": 16, "vocab": 5000, "k": 10, "dtype": "fp32", "train": True},
-        # validation loss of an odd number of queries over a part of the entities (one node type), half precision
+        # validation: the loss of each of an odd number of queries over a part of the entities (one node type), fp16
         {"name": "distill_valid", "op": "distill", "rows": 1021, "vocab": 32771, "k": 32, "dtype": "fp16", "train": False},
         # one batch (128) over all entities with fp32 logits, as the decoder's product writes them
         {"name": "distill_batch", "op": "distill", "rows": 128, "vocab": 130000, "k": 64, "dtype": "fp32", "train": True},
@@ -95,7 +95,7 @@ def work(case):
         return {"bytes": moved, "flops": n * d * (2 if case["train"] else 1)}
     if case["op"] == "distill":
         r, v, k = case["rows"], case["vocab"], case["k"]
-        moved = r * v * e + r * k * 12 + 4
+        moved = r * v * e + r * k * 12 + 4 * r
         if case["train"]:
             moved += r * v * e
         return {"bytes": moved, "flops": r * v * (7 if case["train"] else 4)}
@@ -164,6 +164,11 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------------------------------------ plain forms
+def _power(e):
+    """2^e in fp32 for whole numbers in [-126, 127], exactly (a library's power may be off in the last place)."""
+    return ((e + 127).to(torch.int32) << 23).view(torch.float32)
+
+
 def _packed_values(x):
     """The values that the 4-bit table holds for ``x`` (fp32): blocks of 32 along the row share a power of two, the
     largest not above the block's largest magnitude divided by 4; values are rounded to the nearest of
@@ -176,11 +181,12 @@ def _packed_values(x):
     largest = f.abs().amax(2, keepdim=True)
     _, e = torch.frexp(largest)
     e = (torch.where(largest > 0, e - 1, torch.full_like(e, -200)) - 2).clamp(-127, 127)
-    y = torch.ldexp(torch.ldexp(f, -(e // 2)), -(e - e // 2))
+    half, rest = e // 2, e - e // 2                       # (2^127 has no reciprocal in the normal range: two factors)
+    y = f * _power(-half) * _power(-rest)
     a = y.abs()
     step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
     a = (torch.round(a / step) * step).clamp(max=6.0)
-    q = torch.ldexp(torch.ldexp(torch.copysign(a, y), e // 2), e - e // 2)
+    q = torch.copysign(a, y) * _power(half) * _power(rest)
     q = torch.where(torch.isfinite(largest), q, torch.full_like(q, float("nan")))
     return q.view(rows, -1)[:, :cols]
 
@@ -208,9 +214,9 @@ def _plain(s):
         at = torch.gather(z, 1, ids.clamp(min=0))
         terms = torch.where(q > 0, q * ((tv - top - torch.log(total)) - (at - lse)), 0.0)
         rows = ids.size(0)
-        loss = terms.sum() * (t * t) / rows
         if not s["train"]:
-            return loss
+            return terms.sum(1) * (t * t)
+        loss = terms.sum() * (t * t) / rows
         d = torch.exp(z - lse) * used
         d.scatter_add_(1, ids.clamp(min=0), -q)
         return loss, (d * (t / rows)).to(s["logits"].dtype)
@@ -234,7 +240,8 @@ def run(state):
         return out.detach(), w.grad
     if s["op"] == "distill":
         if not s["train"]:
-            return ops.topk_distill_loss(s["logits"], s["teacher_ids"], s["teacher_logits"], s["temperature"])
+            return ops.topk_distill_loss(s["logits"], s["teacher_ids"], s["teacher_logits"], s["temperature"],
+                                         reduction="none")
         x = s["logits"].detach().requires_grad_()
         loss = ops.topk_distill_loss(x, s["teacher_ids"], s["teacher_logits"], s["temperature"])
         loss.backward()
@@ -245,6 +252,11 @@ def run(state):
 
 
 # ------------------------------------------------------------------------------------------------ 64-bit values
+def _power64(e):
+    """2^e in 64 bits for whole numbers of the normal range, from its bits."""
+    return ((e.clamp(-1000, 1000).long() + 1023) << 52).view(torch.float64)
+
+
 def _nearest(x):
     """What the 4-bit table holds for ``x``, in 64 bits: the block's exponent from a logarithm that is put right by
     comparison, every value moved to the nearer of its two neighbours in the list."""
@@ -255,8 +267,8 @@ def _nearest(x):
         b = x[:, c:c + _BLOCK].double()
         m = b.abs().max(1, keepdim=True).values
         e = torch.floor(torch.log2(m.clamp(min=1e-300)))
-        e = e + (torch.pow(2.0, e + 1) <= m).double() - (torch.pow(2.0, e) > m).double()
-        s = torch.pow(2.0, (e - 2).clamp(-127, 127))
+        e = e + (_power64(e + 1) <= m).double() - (_power64(e) > m).double()
+        s = _power64((e - 2).clamp(-127, 127))
         a = (b.abs() / s).clamp(max=6.0)
         hi = torch.searchsorted(grid, a.contiguous()).clamp(1, 7)
         below, above = a - grid[hi - 1], grid[hi] - a
@@ -279,7 +291,7 @@ def exact(case, seed):
         return out, dw * s["scale"]
     if case["op"] == "distill":
         t, rows = s["temperature"], case["rows"]
-        loss = 0.0
+        losses = torch.zeros(rows, dtype=torch.float64, device="cuda")
         grad = torch.zeros(rows, case["vocab"], dtype=torch.float64, device="cuda") if case["train"] else None
         for lo in range(0, rows, 256):
             z = s["logits"][lo:lo + 256].double() / t
@@ -291,12 +303,12 @@ def exact(case, seed):
             log_q = torch.log_softmax(tv.masked_fill(~real, float("-inf")), 1)
             q = log_q.exp()
             gap = log_q - log_p.gather(1, ids.clamp(min=0))
-            loss = loss + (q * gap.masked_fill(~real, 0.0)).sum() * t * t / rows
+            losses[lo:lo + 256][full] = (q * gap.masked_fill(~real, 0.0)).sum(1) * t * t
             if grad is not None:
                 d = log_p.exp()
                 d.scatter_add_(1, ids.clamp(min=0), -q)
                 grad[lo:lo + 256][full] = d * t / rows
-        return loss if grad is None else (loss, grad)
+        return losses if grad is None else (losses.sum() / rows, grad)
     if case["op"] == "quantize":
         return _nearest(s["x"])
     gen = torch.Generator(device="cuda").manual_seed(int(seed))
