@@ -12,7 +12,9 @@ JOBS=${JOBS:-4}
 HIPCC=${HIPCC:-hipcc}
 OBJ=${OBJ_DIR:-obj}
 OUT=${OUT_SO:-libbiomedkg_hip.so}
-FLAGS="${EXTRA_FLAGS} --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Wno-unused-result -Wno-unused-value"
+# (packed fp32 arithmetic off: some forms of v_pk_{add,mul,fma}_f32, which -O3 makes out of ordinary float code, have given wrong
+# results on this hardware now and then; hipcc's host pass warns that it does not know the feature, which is harmless)
+FLAGS="${EXTRA_FLAGS} --offload-arch=gfx950 -O3 -fPIC -std=c++17 -Wno-unused-result -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops"
 mkdir -p "$OBJ"
 
 needs_build() {  # $1 source, $2 object
