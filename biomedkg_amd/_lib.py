@@ -161,6 +161,16 @@ SIGNATURES = {
     "bkg_ggd_bce_f32": (I32, [P, I64, P, I64, I64, P, P, P, P]),
     "bkg_ggd_bce_bwd_f32": (I32, [P, I64, P, I64, I64, P, P, P, I64, P, I64, P]),
     "bkg_redaf_fused_xw": (I32, [I64, I64, I64, P, I32, I64, P, I64, P, P, P, F32, U64, U32, P, I64, P]),
+    # embed.hip, distill.hip, mx4.hip
+    "bkg_embed_rows": (I32, [P, I32, I64, I64, I64, P, I32, I64, F32, P, I64, P]),
+    "bkg_embed_grad_workspace_bytes": (I64, [I64, I64]),
+    "bkg_embed_grad": (I32, [P, I32, I64, I64, P, I32, I64, I64, I64, F32, P, P, I64, P]),
+    "bkg_distill_workspace_floats": (I64, [I64, I64, I32]),
+    "bkg_distill_forward": (I32, [P, I32, I64, I64, I64, P, I32, I64, P, I32, I64, I32, F32, F32, P, P, P, P, P]),
+    "bkg_distill_backward": (I32, [P, I32, I64, I64, I64, P, I32, I64, P, I32, I64, I32, F32, P, P, I32, F32, P, I64, P]),
+    "bkg_mx4_quantize": (I32, [P, I32, I64, I64, I64, P, P, P]),
+    "bkg_mx4_dequantize": (I32, [P, P, I64, I64, P, I32, I64, P]),
+    "bkg_mx4_matmul": (I32, [P, P, I64, P, P, I64, I64, P, P, I32, I64, P]),
 }
 
 _lib = None

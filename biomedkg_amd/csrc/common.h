@@ -44,6 +44,13 @@ static inline int check_launch(const char* what) {
     }                                                                                            \
   } while (0)
 
+// Stable ascending sort of an embedding lookup's ids with their positions (graph.hip): key = the id, or n_rows where the id
+// lies outside [0, n_rows) or equals pad (those entries come last).  sorted_keys / perm [n]; scratch: 2 n words + workspace
+// of embed_sort_workspace_bytes(n).
+int64_t embed_sort_workspace_bytes(int64_t n);
+int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, uint32_t* scratch, uint32_t* sorted_keys,
+               uint32_t* perm, void* workspace, int64_t workspace_bytes, hipStream_t s);
+
 static inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Deterministic mode (bkg_set_deterministic_workspace): the split-K weight-gradient products write one [M, N] slab per

@@ -1,0 +1,23 @@
+// The element types a table of rows may have (fp32 / bf16 / fp16) and the widest aligned access its layout allows.
+#pragma once
+#include "common.h"
+
+namespace bkg {
+
+constexpr int BKG_T_F32 = 0, BKG_T_BF16 = 1, BKG_T_F16 = 2;
+static inline int type_bytes(int t) { return t == BKG_T_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(__bf16 v) { return (float)v; }
+__device__ __forceinline__ float widen(_Float16 v) { return (float)v; }
+
+// N consecutive elements as one access (N * sizeof(T) = 2 .. 16 bytes, aligned to their size)
+template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+// log2 of the largest access in bytes (<= 16) that `bytes`, a row of it and its start are all multiples of
+static inline int access_bytes(const void* p, int64_t row_bytes, int64_t ld_bytes) {
+  const uint64_t all = (uint64_t)(uintptr_t)p | (uint64_t)row_bytes | (uint64_t)ld_bytes | 16u;
+  return (int)(all & (~all + 1));
+}
+
+}  // namespace bkg

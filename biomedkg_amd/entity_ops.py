@@ -1,0 +1,281 @@
+"""Operators of entity prediction -- one query scored against EVERY entity of the graph (the reference only scores sampled
+triplets, ``biomedkg/kge_module.py:109-132``): the scaled lookup of table rows with its gradient by sorted ids, the
+distillation loss over the entity logits, and the microscaled 4-bit table a model is served from.  Public names are
+re-exported by :mod:`biomedkg_amd.ops`; like everything there they need HIP tensors and launch on torch's current stream.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _type_of(t, what):
+    code = _TYPE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _rows(t):
+    """``t`` with its columns next to each other (any row stride; expanded rows are copied out)."""
+    return t if (t.stride(1) == 1 or t.size(1) == 1) and (t.stride(0) >= t.size(1) or t.size(0) <= 1) else t.contiguous()
+
+
+def _ids(t, what):
+    if t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: expected int64 or int32, got {t.dtype}")
+
+
+def _same_device(what, first, *others):
+    """All tensors on the current device: the library launches on its current stream."""
+    L.require_cuda(first, *others)
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"{what}: tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()} "
+                         "(use torch.cuda.device)")
+
+
+# ----------------------------------------------------------------------------- embedding
+def _embed_rows(weight, ids, scale):
+    w = _rows(weight)
+    ids = ids if ids.is_contiguous() else ids.contiguous()
+    d = w.size(1)
+    out = torch.empty(ids.shape + (d,), dtype=w.dtype, device=w.device)
+    L.call("bkg_embed_rows", w.data_ptr(), _TYPE[w.dtype], w.stride(0), w.size(0), d, ids.data_ptr(),
+           ids.dtype == torch.int32, ids.numel(), scale, out.data_ptr(), d, L.stream())
+    return out, ids
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, pad):
+        out, ids = _embed_rows(weight, ids, scale)
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.pad, ctx.shape, ctx.dtype = scale, pad, weight.shape, weight.dtype
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        v, d = ctx.shape
+        n = ids.numel()
+        g = _rows(g.reshape(n, d))
+        dw = torch.empty(v, d, dtype=ctx.dtype, device=g.device)
+        ws_bytes = L.lib().bkg_embed_grad_workspace_bytes(n, d)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device)
+        L.call("bkg_embed_grad", g.data_ptr(), _TYPE[ctx.dtype], g.stride(0), d, ids.data_ptr(), ids.dtype == torch.int32, n, v,
+               ctx.pad, ctx.scale, dw.data_ptr(), ws.data_ptr(), ws_bytes, L.stream())
+        return dw, None, None, None
+
+
+def embedding(weight, ids, scale=1.0, padding_idx=None):
+    """``scale * weight[ids]`` -> ``ids.shape + (d,)`` in ``weight``'s type (fp32 / bf16 / fp16, one rounding).
+
+    ``weight [V, d]`` (any row stride), ``ids`` int64 / int32 of any shape.  An id outside ``[0, V)`` reads as a row of zeros
+    and gets no gradient (padded batches); ``padding_idx`` (negative: from the end) reads its row and gets no gradient.
+
+    The gradient is dense ``[V, d]`` in ``weight``'s type: ids sorted (stable), every row summed in fp32 in the order of its
+    positions, rounded once -- bitwise repeatable, no atomics (csrc/embed.hip)."""
+    if weight.dim() != 2:
+        raise ValueError(f"embedding: expected a [V, d] table, got {tuple(weight.shape)}")
+    _type_of(weight, "embedding")
+    _ids(ids, "embedding ids")
+    _same_device("embedding", weight, ids)
+    v, d = weight.shape
+    if v >= 2 ** 31 or ids.numel() >= 2 ** 31 or d > 2 ** 20:
+        raise ValueError("embedding: at most 2^31 - 1 rows and ids, 2^20 columns")
+    scale = float(scale)
+    pad = -1
+    if padding_idx is not None:
+        if not -v <= padding_idx < v:
+            raise ValueError(f"embedding: padding_idx {padding_idx} outside the table's {v} rows")
+        pad = int(padding_idx) % v
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _Embedding.apply(weight, ids, scale, pad)
+    return _embed_rows(weight, ids, scale)[0]
+
+
+# ----------------------------------------------------------------------------- distillation
+def _distill_forward(x, ids, t, temp, sum_scale, want_sum):
+    rows, v = x.shape
+    dev, xt = x.device, _TYPE[x.dtype]
+    ws = torch.empty(L.lib().bkg_distill_workspace_floats(rows, v, xt), dtype=torch.float32, device=dev)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
+    losses = torch.empty(rows, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev) if want_sum else None
+    L.call("bkg_distill_forward", x.data_ptr(), xt, x.stride(0), rows, v, ids.data_ptr(), ids.dtype == torch.int32, ids.stride(0),
+           t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), temp, sum_scale, ws.data_ptr(), stats.data_ptr(),
+           losses.data_ptr(), L.ptr(loss), L.stream())
+    return (loss if want_sum else losses), stats
+
+
+class _TopkDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, ids, t, temp, mean, want_sum):
+        out, stats = _distill_forward(x, ids, t, temp, 1.0 / x.size(0) if mean else 1.0, want_sum)
+        ctx.save_for_backward(x, ids, t, stats)
+        ctx.temp, ctx.coef, ctx.g_step = temp, (temp / x.size(0) if mean else temp), int(not want_sum)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, ids, t, stats = ctx.saved_tensors
+        rows, v = x.shape
+        g = g.to(torch.float32).contiguous()
+        d = torch.empty(rows, v, dtype=x.dtype, device=x.device)
+        L.call("bkg_distill_backward", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, v, ids.data_ptr(),
+               ids.dtype == torch.int32, ids.stride(0), t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), ctx.temp,
+               stats.data_ptr(), g.data_ptr(), ctx.g_step, ctx.coef, d.data_ptr(), v, L.stream())
+        return d, None, None, None, None, None
+
+
+def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, reduction="batchmean"):
+    """Distillation of ``logits [R, V]`` (fp32 / bf16 / fp16) from a teacher's best entries: ``teacher_ids [R, K]`` (int64 /
+    int32) with ``teacher_logits [R, K]`` (constants: no gradient flows into them), ``1 <= K <= 1024``.
+
+    Per row ``T^2 * KL(q || p)`` over the K entries with ``q = softmax(teacher_logits / T)`` over the row's usable entries and
+    ``p = softmax(logits / T)`` over all V columns; the gradient is ``T * (p - q)`` in ``logits``'s type, statistics and sums in
+    fp32 (csrc/distill.hip).  ``K = 1`` is cross entropy.  An entry is not usable if its id lies outside ``[0, V)`` (padding:
+    -1) or its logit is ``-inf``; an id that occurs twice counts twice.  A row without a usable entry, or whose logits are all
+    ``-inf``, is left out: loss 0, gradient 0.  A usable entry whose student logit is ``-inf`` makes the loss ``inf``; NaN stays
+    NaN.
+
+    ``reduction``: ``"batchmean"`` (sum / R), ``"sum"`` -> fp32 scalars, ``"none"`` -> fp32 ``[R]``."""
+    if logits.dim() != 2 or teacher_ids.dim() != 2 or teacher_logits.shape != teacher_ids.shape \
+            or teacher_ids.size(0) != logits.size(0):
+        raise ValueError(f"topk_distill_loss: expected logits [R, V] and teacher ids / logits [R, K], got {tuple(logits.shape)}, "
+                         f"{tuple(teacher_ids.shape)}, {tuple(teacher_logits.shape)}")
+    _type_of(logits, "topk_distill_loss logits")
+    _type_of(teacher_logits, "topk_distill_loss teacher logits")
+    _ids(teacher_ids, "topk_distill_loss teacher ids")
+    _same_device("topk_distill_loss", logits, teacher_ids, teacher_logits)
+    if reduction not in ("batchmean", "sum", "none"):
+        raise ValueError(f"topk_distill_loss: reduction {reduction!r} (batchmean, sum or none)")
+    temp = float(temperature)
+    if not (temp > 0.0 and math.isfinite(temp)):
+        raise ValueError(f"topk_distill_loss: the temperature must be positive and finite, got {temperature}")
+    rows, v = logits.shape
+    k = teacher_ids.size(1)
+    if not 1 <= k <= 1024:
+        raise ValueError(f"topk_distill_loss: between 1 and 1024 teacher entries per row, got {k}")
+    if v == 0 or v >= 2 ** 30 or rows >= 2 ** 24:
+        raise ValueError("topk_distill_loss: between 1 and 2^30 - 1 columns, below 2^24 rows")
+    if teacher_logits.requires_grad:
+        raise ValueError("topk_distill_loss: the teacher's logits are constants (detach them)")
+    if rows == 0:
+        z = logits.float().sum(1)
+        return z if reduction == "none" else z.sum()
+    ids, t = _rows(teacher_ids), _rows(teacher_logits)
+    want_sum = reduction != "none"
+    mean = reduction == "batchmean"
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TopkDistill.apply(_rows(logits), ids, t, temp, mean, want_sum)
+    return _distill_forward(_rows(logits), ids, t, temp, 1.0 / rows if mean else 1.0, want_sum)[0]
+
+
+# ----------------------------------------------------------------------------- microscaled 4-bit tables
+class Mx4Table:
+    """A ``[rows, cols]`` table in microscaled 4 bits (:func:`mx4_quantize`): ``codes`` uint8 ``[rows, P / 2]`` (two columns a
+    byte, the lower one in the low nibble) and ``scales`` uint8 ``[rows, P / 32]`` (the exponent of each 32 columns + 127,
+    255: the block held an infinity or NaN), ``P`` = ``cols`` rounded up to 128.  0.53 bytes a value."""
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes, scales, shape):
+        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
+        rows, cols = self.shape
+        p = (cols + 127) // 128 * 128
+        for t, want, what in ((codes, (rows, p // 2), "codes"), (scales, (rows, p // 32), "scales")):
+            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
+                raise ValueError(f"Mx4Table: {what} must be contiguous uint8 {want} for a table of {self.shape}")
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def __repr__(self):
+        return f"Mx4Table({self.shape[0]} x {self.shape[1]}, {self.nbytes} bytes, {self.device})"
+
+
+def mx4_quantize(x):
+    """``x [rows, cols]`` (fp32 / bf16 / fp16) as an :class:`Mx4Table`: per 32 columns the shared scale is
+    ``2^(floor(log2(max|x|)) - 2)`` (exponent within [-127, 127]), values go to the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 times
+    it, ties to the even code (csrc/mx4.hip).  No gradient."""
+    if x.dim() != 2 or x.size(1) == 0:
+        raise ValueError(f"mx4_quantize: expected [rows, cols] with cols > 0, got {tuple(x.shape)}")
+    _type_of(x, "mx4_quantize")
+    _same_device("mx4_quantize", x)
+    rows, cols = x.shape
+    if cols > 2 ** 24 or rows >= 2 ** 31:
+        raise ValueError("mx4_quantize: at most 2^24 columns and 2^31 - 1 rows")
+    x = _rows(x.detach())
+    p = (cols + 127) // 128 * 128
+    codes = torch.empty(rows, p // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(rows, p // 32, dtype=torch.uint8, device=x.device)
+    L.call("bkg_mx4_quantize", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, codes.data_ptr(), scales.data_ptr(),
+           L.stream())
+    return Mx4Table(codes, scales, (rows, cols))
+
+
+def mx4_dequantize(table, dtype=torch.float32):
+    """The values an :class:`Mx4Table` holds, ``[rows, cols]`` in ``dtype`` (exact in fp32 and bf16; fp16 rounds)."""
+    if not isinstance(table, Mx4Table):
+        raise TypeError("mx4_dequantize: expected an Mx4Table")
+    if dtype not in _TYPE:
+        raise TypeError(f"mx4_dequantize: float32, bfloat16 or float16, got {dtype}")
+    _same_device("mx4_dequantize", table.codes, table.scales)
+    rows, cols = table.shape
+    out = torch.empty(rows, cols, dtype=dtype, device=table.device)
+    L.call("bkg_mx4_dequantize", table.codes.data_ptr(), table.scales.data_ptr(), rows, cols, out.data_ptr(), _TYPE[dtype], cols,
+           L.stream())
+    return out
+
+
+def mx4_linear(x, table, bias=None, out_dtype=None):
+    """``x @ table.T (+ bias)`` with both operands in microscaled 4 bits, products and sums on the matrix cores in fp32, one
+    rounding into ``out_dtype`` (default: ``x``'s type).  ``x [..., cols]`` fp32 / bf16 / fp16 is quantised within the call
+    (or is an :class:`Mx4Table` already: then ``out_dtype`` defaults to fp32), ``table [n, cols]``, ``bias [n]`` fp32.
+
+    For inference: no gradient (an input that requires one is refused while gradients are recorded)."""
+    if not isinstance(table, Mx4Table):
+        raise TypeError("mx4_linear: the table must be an Mx4Table (mx4_quantize)")
+    n, cols = table.shape
+    if isinstance(x, Mx4Table):
+        lead, xq = (x.shape[0],), x
+        if x.shape[1] != cols:
+            raise ValueError(f"mx4_linear: {x.shape[1]} columns against a table of {cols}")
+        out_dtype = out_dtype or torch.float32
+        _same_device("mx4_linear", x.codes, table.codes, bias)
+    else:
+        if x.dim() == 0 or x.size(-1) != cols:
+            raise ValueError(f"mx4_linear: x {tuple(x.shape)} against a table of {cols} columns")
+        _type_of(x, "mx4_linear")
+        _same_device("mx4_linear", x, table.codes, bias)
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+            raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
+        lead = x.shape[:-1]
+        out_dtype = out_dtype or x.dtype
+        xq = mx4_quantize(x.reshape(-1, cols))
+    if out_dtype not in _TYPE:
+        raise TypeError(f"mx4_linear: out_dtype float32, bfloat16 or float16, got {out_dtype}")
+    if bias is not None and (bias.shape != (n,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
+        raise ValueError(f"mx4_linear: bias must be contiguous fp32 [{n}]")
+    m = xq.shape[0]
+    out = torch.empty(m, n, dtype=out_dtype, device=table.device)
+    L.call("bkg_mx4_matmul", xq.codes.data_ptr(), xq.scales.data_ptr(), m, table.codes.data_ptr(), table.scales.data_ptr(), n,
+           cols, L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.stream())
+    return out.view(*lead, n)

@@ -2571,3 +2571,8 @@ def redaf_fusion(x, w_t, b_t, scale, drop: Dropout = None):
                L.ptr(keep[lo * m: hi * m]) if keep is not None else None, p, seed, sid, lo * m, L.ptr(out[lo:hi]),
                out.stride(0), L.stream())
     return out
+
+
+# ----------------------------------------------------------------------------- entity prediction
+from .entity_ops import (Mx4Table, embedding, mx4_dequantize, mx4_linear, mx4_quantize,  # noqa: E402,F401
+                         topk_distill_loss)

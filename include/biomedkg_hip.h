@@ -646,6 +646,36 @@ int bkg_ggd_bce_bwd_f32(const float* pos, int64_t stride_pos, const float* neg, 
                         const int64_t* n_dev, const float* gout, float* dpos, int64_t stride_dpos, float* dneg,
                         int64_t stride_dneg, void* stream);
 
+/* ---- entity prediction: a query scored against every entity (no counterpart in the reference, which scores sampled
+ *      triplets only: biomedkg/kge_module.py:109-132).  Element types: 0 fp32, 1 bf16, 2 fp16; ids int64, or int32 where the
+ *      *_i32 argument is set. */
+/* out[i, :] = scale * w[ids[i], :] (w [n_rows, d], out [n, d], same type); an id outside [0, n_rows) gives a row of zeros */
+int bkg_embed_rows(const void* w, int32_t type, int64_t ldw, int64_t n_rows, int64_t d, const void* ids, int32_t ids_i32,
+                   int64_t n, float scale, void* out, int64_t ldo, void* stream);
+int64_t bkg_embed_grad_workspace_bytes(int64_t n, int64_t d);
+/* dw [n_rows, d] (contiguous, 16-byte aligned; every row is written) = scale * sum of g's rows by id, fp32 sums in position
+ * order; ids outside [0, n_rows) and pad (-1: none) add nothing.  workspace: 256-byte aligned. */
+int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t d, const void* ids, int32_t ids_i32, int64_t n,
+                   int64_t n_rows, int64_t pad, float scale, void* dw, void* workspace, int64_t workspace_bytes, void* stream);
+/* Distillation from a teacher's k best entries per row (csrc/distill.hip has the formulas).  losses [rows] = the rows' losses,
+ * loss (nullable) = sum_scale * their sum; row_stats [rows, 4] is what the backward needs. */
+int64_t bkg_distill_workspace_floats(int64_t rows, int64_t v, int32_t type);
+int bkg_distill_forward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, const void* ids, int32_t ids_i32,
+                        int64_t ld_ids, const void* t, int32_t t_type, int64_t ld_t, int32_t k, float temp, float sum_scale,
+                        float* workspace, float* row_stats, float* losses, float* loss, void* stream);
+/* d [rows, v] = g[row * g_step] * coef * (softmax(x / temp) - q) in x's type (coef: temp, or temp / rows for the mean) */
+int bkg_distill_backward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, const void* ids, int32_t ids_i32,
+                         int64_t ld_ids, const void* t, int32_t t_type, int64_t ld_t, int32_t k, float temp,
+                         const float* row_stats, const float* g, int32_t g_step, float coef, void* d, int64_t ldd, void* stream);
+/* Microscaled 4-bit tables.  codes [rows, P / 2] and scales [rows, P / 32] bytes, P = cols rounded up to 128; two columns a
+ * byte (lower one in the low nibble), a scale byte is the exponent of 32 columns + 127 (255: the block is NaN). */
+int bkg_mx4_quantize(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t cols, void* codes, void* scales, void* stream);
+int bkg_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int32_t type, int64_t ldo,
+                       void* stream);
+/* out [m, n] = A B^T (+ bias [n]) over two packed tables of the same width, fp32 sums, one rounding into `type` */
+int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t m, const void* b_codes, const void* b_scales, int64_t n,
+                   int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
