@@ -3,8 +3,9 @@
 // A row is cut into blocks of 32 values that share a power of two s = 2^E, E = clamp(floor(log2(max |v|)) - 2, -127, 127);
 // a value is held as the nearest of +-{0, .5, 1, 1.5, 2, 3, 4, 6} to v / s (ties to the even code, larger ones to 6): four
 // bits (sign, two exponent bits, one mantissa bit), the lower of two columns in the low nibble.  E + 127 is a byte; 255 marks
-// a block that held an infinity or NaN: all its values read as NaN.  Rows are padded with zeros to a multiple of 128 columns
-// (64 bytes of codes, one dword of scales), so the product has no tail in its inner dimension.
+// a block that held an infinity or NaN: all its values read as NaN.  Rows are padded with zeros to a multiple of 128 columns,
+// and a table lies in PANELS of 128 columns: panel p holds the 64 bytes of codes of every row side by side (and one dword of
+// scales per row), so the product has no tail in its inner dimension and reads neighbouring rows of a panel as one run.
 //
 // Dividing by s only moves the exponent, so quantisation has one rounding and is the same whatever the input's type.
 #include "rowtypes.h"
@@ -13,6 +14,7 @@ namespace bkg {
 
 constexpr int MX_K = 128;                       // columns a row is padded to a multiple of
 
+typedef int mx_i32x4 __attribute__((ext_vector_type(4)));
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
 typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
 
@@ -60,8 +62,9 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__
   if (byte == 255u) q = 0;
   const uint32_t b1 = __shfl_down((int)byte, 4, 64), b2 = __shfl_down((int)byte, 8, 64), b3 = __shfl_down((int)byte, 12, 64);
   if (row < rows) {
-    codes[row * pieces + piece] = q;
-    if ((piece & 15) == 0) scales[row * (pieces >> 4) + (piece >> 4)] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
+    const int64_t at_row = (int64_t)(piece >> 4) * rows + row;                    // (panel, row)
+    codes[at_row * 16 + (piece & 15)] = q;
+    if ((piece & 15) == 0) scales[at_row] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
   }
 }
 
@@ -81,8 +84,9 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
   if (row >= rows) return;
   const int piece = (int)(at - row * pieces), c = piece * 8;
   if (c >= cols) return;
-  const uint32_t q = codes[row * pieces + piece];
-  const int byte = scales[row * (pieces >> 2) + (piece >> 2)], e = byte - 127;
+  const int64_t at_row = (int64_t)(piece >> 4) * rows + row;
+  const uint32_t q = codes[at_row * 16 + (piece & 15)];
+  const int byte = scales[at_row * 4 + ((piece >> 2) & 3)], e = byte - 127;
   T* p = out + row * ldo + c;
   T v[8];
 #pragma unroll
@@ -102,74 +106,211 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
 }
 
 // ---- out[m, n] = sum_k A[m, k] B[n, k] (+ bias[n]).  v_mfma_scale_f32_32x32x64_f8f6f4: lane l holds 32 columns (16 bytes)
-// of row l % 32, block l / 32, and that block's scale byte; the result's column is B's row l % 32.
+// of row l % 32, block l / 32, and that block's scale byte; the result's column is B's row l % 32.  A panel of 128 columns is
+// two such products (h = 0, 1): lane half `half` takes the panel's 16-byte piece 2 h + half and byte 2 h + half of its dword
+// of scales.
 struct Mx4Args {
-  const uint32_t* ca; const uint32_t* sa; int64_t m;
-  const uint32_t* cb; const uint32_t* sb; int64_t n;
-  int steps;                                     // inner dimension / 128
+  const unsigned char* ca; const uint32_t* sa; int64_t m;
+  const unsigned char* cb; const uint32_t* sb; int64_t n;
+  int steps;                                     // panels of 128 columns
+  int m_tiles, n_tiles;
   const float* bias;
   void* out; int64_t ldo;
+  int wide;                                      // the rows of `out` take aligned 16-byte stores
 };
 
-__device__ __forceinline__ mx_i32x8 mx_operand(uint4 v) {
-  return mx_i32x8{(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+__device__ __forceinline__ mx_i32x8 mx_operand(mx_i32x4 v) {
+  return mx_i32x8{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
+}
+template <int H>
+__device__ __forceinline__ mx_f32x16 mx_mfma(mx_i32x4 a, mx_i32x4 b, mx_f32x16 c, uint32_t xa, uint32_t xb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a), mx_operand(b), c, 4, 4, 2 * H, (int)xa, 2 * H, (int)xb);
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void mx4_matmul_kernel(const Mx4Args a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, half = lane >> 5;
-  const int64_t m0 = (int64_t)blockIdx.x * 128 + (wave & 1) * 64, n0 = (int64_t)blockIdx.y * 128 + (wave >> 1) * 64;
-  const int pitch = a.steps * 16;                // dwords of codes per row
-  mx_f32x16 acc[2][2];
+// Tiled product.  Four waves (2 x 2) compute a block of 64 MT x 64 NT outputs, (32 MT) x (32 NT) per wave.  Panels travel
+// through a ring of S LDS slots by LDS-DMA: a stage is the block's rows of one panel of A and of B (64 contiguous bytes a
+// row: a wave-instruction copies 16 whole rows) and their dwords of scales.  Slot c' of row r holds piece c' ^ ((r / 2) & 3)
+// (the swizzle is applied to the DMA's source address): the b128 fragment reads of 8 neighbouring rows then fall on
+// different banks.  One raw barrier per stage, placed between its two halves: behind it every wave has both halves of stage
+// t in registers, so slot t is refilled with stage t + S, and the first fragments of stage t + 1 are read while the second
+// half of stage t multiplies.  The ring is retired by counted vmcnt waits: the loop issues nothing but DMAs.
+//
+// The result goes through LDS once (32 rows of a wave at a time) so that rows leave in runs of 16-byte stores: for the
+// narrow inner dimensions of an entity table (256 columns: two panels) writing the outputs is what the call costs.
+template <typename T, int MT, int NT, int S>
+__global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(const Mx4Args a) {
+  constexpr int BM = 64 * MT, BN = 64 * NT;
+  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, STAGE = A_BYTES + B_BYTES + (BM + BN) * 4;
+  constexpr int CH = 2 * MT, DMAS = CH + CH / 4;             // 16-row copies / all copies per wave and stage
+  static_assert(MT == NT && MT % 2 == 0, "the waves share a stage's copies evenly, and a half has a product per fragment");
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, half = lane >> 5;
+
+  // tile order: each XCD takes a contiguous part of the list; the list runs through 8 tiles of rows at a time, so the tiles
+  // in flight on one XCD share their panels in its L2
+  const int64_t total = (int64_t)a.m_tiles * a.n_tiles, per = (total + BKG_XCDS - 1) / BKG_XCDS;
+  const int64_t t = (int64_t)(blockIdx.x % BKG_XCDS) * per + blockIdx.x / BKG_XCDS;
+  if (blockIdx.x / BKG_XCDS >= per || t >= total) return;
+  const int64_t in_band = 8 * (int64_t)a.n_tiles, band = t / in_band, at = t - band * in_band;
+  const int band_m = (int)min((int64_t)8, a.m_tiles - band * 8);
+  const int64_t m0 = (band * 8 + at % band_m) * BM, n0 = at / band_m * BN;
+
+  // this wave's share of a stage's copies: waves 0 and 1 copy A's 4 MT chunks of 16 rows and MT chunks of 64 scales, waves 2
+  // and 3 B's
+  const bool of_a = wave < 2;
+  const int64_t rows = of_a ? a.m : a.n, r0 = of_a ? m0 : n0;
+  const unsigned char* const codes = of_a ? a.ca : a.cb;
+  const uint32_t* const scales = of_a ? a.sa : a.sb;
+  int64_t src[CH], ssrc[CH / 4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < CH; ++j)
+    src[j] = min(r0 + ((wave & 1) * CH + j) * 16 + (lane >> 2), rows - 1) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < CH / 4; ++j) ssrc[j] = min(r0 + ((wave & 1) * (CH / 4) + j) * 64 + lane, rows - 1);
+  auto copy = [&](int stage, int slot, int j) {              // copy j of this wave's DMAS of a stage
+    const int64_t k = min(stage, a.steps - 1);               // (past the end: valid memory, never read)
+    unsigned char* base = lds + slot * STAGE;
+    if (j < CH)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(codes + k * rows * 64 + src[j]),
+                                       (__attribute__((address_space(3))) void*)(base + (wave * CH + j) * 1024), 16, 0, 0);
+    else
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(scales + k * rows + ssrc[j - CH]),
+          (__attribute__((address_space(3))) void*)(base + A_BYTES + B_BYTES + (wave * (CH / 4) + j - CH) * 256), 4, 0, 0);
+  };
+
+  const int wm = (wave & 1) * 32 * MT, wn = (wave >> 1) * 32 * NT;
+  struct Frags { mx_i32x4 a[MT], b[NT]; };
+  struct Scales { uint32_t a[MT], b[NT]; };
+  const int swz = (l31 >> 1) & 3;
+  auto read = [&](int slot, int h, Frags& f, int i) {        // fragment i of the MT + NT
+    const unsigned char* base = lds + slot * STAGE + l31 * 64 + (((2 * h + half) ^ swz) * 16);
+    if (i < MT) f.a[i] = *reinterpret_cast<const mx_i32x4*>(base + (wm + 32 * i) * 64);
+    else f.b[i - MT] = *reinterpret_cast<const mx_i32x4*>(base + A_BYTES + (wn + 32 * (i - MT)) * 64);
+  };
+  auto read_scales = [&](int slot, Scales& s) {              // (as they lie: byte `half` is not yet in front)
+    const unsigned char* base = lds + slot * STAGE + A_BYTES + B_BYTES + l31 * 4;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) s.a[i] = *reinterpret_cast<const uint32_t*>(base + (wm + 32 * i) * 4);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) s.b[j] = *reinterpret_cast<const uint32_t*>(base + (BM + wn + 32 * j) * 4);
+  };
+  // (hipcc would sink the reads that a later iteration uses in front of that use: this keeps them where they are written)
+  auto pin = [&](Frags& f, Scales& s) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(f.a[i]), "+v"(s.a[i]));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(f.b[j]), "+v"(s.b[j]));
+  };
+
+  mx_f32x16 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  int64_t ra[2], rb[2];                          // (rows behind the last one read the last one; their results are dropped)
+
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    ra[i] = min(m0 + i * 32 + l31, a.m - 1);
-    rb[i] = min(n0 + i * 32 + l31, a.n - 1);
-  }
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int j = 0; j < DMAS; ++j) copy(s, s, j);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * DMAS) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  Frags f0, f1;
+  Scales sc, sn;
+#pragma unroll
+  for (int i = 0; i < MT + NT; ++i) read(0, 0, f0, i);
+  read_scales(0, sn);
+  pin(f0, sn);
+  int slot = 0;
   for (int st = 0; st < a.steps; ++st) {
-    uint4 va[2][2], vb[2][2];
-    uint32_t xa[2], xb[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      xa[i] = a.sa[ra[i] * a.steps + st] >> (8 * half);
-      xb[i] = a.sb[rb[i] * a.steps + st] >> (8 * half);
+    for (int i = 0; i < MT; ++i) sc.a[i] = sn.a[i] >> (8 * half);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        va[i][h] = *reinterpret_cast<const uint4*>(a.ca + ra[i] * pitch + st * 16 + 8 * h + 4 * half);
-        vb[i][h] = *reinterpret_cast<const uint4*>(a.cb + rb[i] * pitch + st * 16 + 8 * h + 4 * half);
+    for (int j = 0; j < NT; ++j) sc.b[j] = sn.b[j] >> (8 * half);
+    // first half: the second half's fragments are read between the products
+#pragma unroll
+    for (int x = 0; x < MT * NT; ++x) {
+      const int i = x / NT, j = x % NT;
+      acc[i][j] = mx_mfma<0>(f0.a[i], f0.b[j], acc[i][j], sc.a[i], sc.b[j]);
+      if (x < MT + NT) read(slot, 1, f1, x);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // this wave's reads of stage st and its copies of stage st + 1 are complete; behind the barrier everyone's are
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_waitcnt vmcnt(%0)" ::"n"((S - 2) * DMAS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    // second half: the next stage's first fragments are read and the freed slot's copies issued between the products
+    const int next = slot + 1 == S ? 0 : slot + 1;
+#pragma unroll
+    for (int x = 0; x < MT * NT; ++x) {
+      const int i = x / NT, j = x % NT;
+      acc[i][j] = mx_mfma<1>(f1.a[i], f1.b[j], acc[i][j], sc.a[i], sc.b[j]);
+#pragma unroll
+      for (int y = x * (MT + NT) / (MT * NT); y < (x + 1) * (MT + NT) / (MT * NT); ++y) read(next, 0, f0, y);
+      if (x == 0) read_scales(next, sn);
+#pragma unroll
+      for (int y = x * DMAS / (MT * NT); y < (x + 1) * DMAS / (MT * NT); ++y) copy(st + S, slot, y);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    pin(f0, sn);
+    slot = next;
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the copies past the last panel
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+
+  // ---- the wave's 32 MT rows of 32 NT columns, 32 rows at a time
+  constexpr int WN = 32 * NT, PITCH = WN + 4;                  // floats
+  float* mine = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
+  static_assert(4 * 32 * PITCH * 4 <= S * STAGE, "the results' staging area lies in the ring");
+  T* out = static_cast<T*>(a.out);
+  constexpr int VE = 16 / sizeof(T), LPR = WN / VE, RPI = 64 / LPR;   // elements per store, lanes per row, rows per store
+  const int col = (lane % LPR) * VE;
+  const int64_t nc = n0 + wn + col;
+  float bias[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) bias[e] = a.bias && nc + e < a.n ? a.bias[nc + e] : 0.f;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[(8 * (r >> 2) + 4 * half + (r & 3)) * PITCH + 32 * j + l31] = acc[i][j][r];
+    // (a wave's LDS operations complete in order and the area is its own: no barrier)
+    const int64_t mr = m0 + wm + 32 * i;
+#pragma unroll
+    for (int r = 0; r < 32 / RPI; ++r) {
+      const int row = r * RPI + lane / LPR;
+      Pack<T, VE> o;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) o.v[e] = (T)(mine[row * PITCH + col + e] + bias[e]);
+      if (mr + row < a.m) {
+        T* dst = out + (mr + row) * a.ldo + nc;
+        if (a.wide && nc + VE <= a.n) *reinterpret_cast<Pack<T, VE>*>(dst) = o;
+        else
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+            if (nc + e < a.n) dst[e] = o.v[e];
       }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(va[i][0]), mx_operand(vb[j][0]), acc[i][j], 4, 4,
-                                                                    0, (int)xa[i], 0, (int)xb[j]);
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(va[i][1]), mx_operand(vb[j][1]), acc[i][j], 4, 4,
-                                                                    2, (int)xa[i], 2, (int)xb[j]);
-      }
   }
-  T* out = (T*)a.out;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t n = n0 + j * 32 + l31;
-    if (n >= a.n) continue;
-    const float b = a.bias ? a.bias[n] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t m = m0 + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (m < a.m) out[m * a.ldo + n] = (T)(acc[i][j][r] + b);
-      }
-  }
+}
+
+template <typename T, int MT, int NT, int S>
+static void mx4_launch(Mx4Args a, hipStream_t s) {
+  constexpr int LDS = S * (64 * (MT + NT) * 64 + 64 * (MT + NT) * 4);
+  static const bool set = hipFuncSetAttribute((const void*)mx4_tile_kernel<T, MT, NT, S>,
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, LDS) == hipSuccess;
+  (void)set;
+  a.m_tiles = (int)((a.m + 64 * MT - 1) / (64 * MT));
+  a.n_tiles = (int)((a.n + 64 * NT - 1) / (64 * NT));
+  const int64_t total = (int64_t)a.m_tiles * a.n_tiles;
+  const unsigned grid = (unsigned)((total + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS);
+  hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, S>), dim3(grid), dim3(256), LDS, s, a);
 }
 
 static int64_t mx4_steps(int64_t cols) { return (cols + MX_K - 1) / MX_K; }
@@ -234,10 +375,14 @@ extern "C" int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t
   BKG_ARG((uintptr_t)a_codes % 16 == 0 && (uintptr_t)b_codes % 16 == 0 && (uintptr_t)a_scales % 4 == 0 &&
               (uintptr_t)b_scales % 4 == 0 && (uintptr_t)out % type_bytes(type) == 0,
           "bkg_mx4_matmul: misaligned buffer");
-  const Mx4Args a{(const uint32_t*)a_codes, (const uint32_t*)a_scales, m, (const uint32_t*)b_codes, (const uint32_t*)b_scales, n,
-                  (int)mx4_steps(cols), bias, out, ldo};
-  BKG_ARG((n + 127) / 128 < 65536, "bkg_mx4_matmul: table too long");
-  const dim3 grid((unsigned)((m + 127) / 128), (unsigned)((n + 127) / 128));
-  BKG_BY_TYPE(type, hipLaunchKernelGGL((mx4_matmul_kernel<T>), grid, dim3(256), 0, (hipStream_t)stream, a));
+  BKG_ARG((m + 127) / 128 * ((n + 127) / 128) < (1ll << 31) - 8, "bkg_mx4_matmul: too many tiles for one launch");
+  BKG_ARG(!bias || (uintptr_t)bias % 4 == 0, "bkg_mx4_matmul: misaligned bias");
+  Mx4Args a{(const unsigned char*)a_codes, (const uint32_t*)a_scales, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales,
+            n, (int)mx4_steps(cols), 0, 0, bias, out, ldo, access_bytes(out, 0, ldo * type_bytes(type)) == 16};
+  hipStream_t s = (hipStream_t)stream;
+  // 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128
+  if ((m + 255) / 256 * ((n + 255) / 256) >= 192 && a.steps >= 8) BKG_BY_TYPE(type, (mx4_launch<T, 4, 4, 4>(a, s)));
+  else if (a.steps <= 2) BKG_BY_TYPE(type, (mx4_launch<T, 2, 2, 2>(a, s)));
+  else BKG_BY_TYPE(type, (mx4_launch<T, 2, 2, 4>(a, s)));
   return check_launch("bkg_mx4_matmul");
 }

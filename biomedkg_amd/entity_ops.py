@@ -186,16 +186,17 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, redu
 
 # ----------------------------------------------------------------------------- microscaled 4-bit tables
 class Mx4Table:
-    """A ``[rows, cols]`` table in microscaled 4 bits (:func:`mx4_quantize`): ``codes`` uint8 ``[rows, P / 2]`` (two columns a
-    byte, the lower one in the low nibble) and ``scales`` uint8 ``[rows, P / 32]`` (the exponent of each 32 columns + 127,
-    255: the block held an infinity or NaN), ``P`` = ``cols`` rounded up to 128.  0.53 bytes a value."""
+    """A ``[rows, cols]`` table in microscaled 4 bits (:func:`mx4_quantize`), in panels of 128 columns (the last one padded
+    with zeros): ``codes`` uint8 ``[panels, rows, 64]`` (two columns a byte, the lower one in the low nibble) and ``scales``
+    uint8 ``[panels, rows, 4]`` (the exponent of each 32 columns + 127; 255: the block held an infinity or NaN).  0.53 bytes a
+    value."""
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes, scales, shape):
         self.codes, self.scales, self.shape = codes, scales, tuple(shape)
         rows, cols = self.shape
-        p = (cols + 127) // 128 * 128
-        for t, want, what in ((codes, (rows, p // 2), "codes"), (scales, (rows, p // 32), "scales")):
+        panels = (cols + 127) // 128
+        for t, want, what in ((codes, (panels, rows, 64), "codes"), (scales, (panels, rows, 4), "scales")):
             if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
                 raise ValueError(f"Mx4Table: {what} must be contiguous uint8 {want} for a table of {self.shape}")
 
@@ -223,9 +224,9 @@ def mx4_quantize(x):
     if cols > 2 ** 24 or rows >= 2 ** 31:
         raise ValueError("mx4_quantize: at most 2^24 columns and 2^31 - 1 rows")
     x = _rows(x.detach())
-    p = (cols + 127) // 128 * 128
-    codes = torch.empty(rows, p // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(rows, p // 32, dtype=torch.uint8, device=x.device)
+    panels = (cols + 127) // 128
+    codes = torch.empty(panels, rows, 64, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(panels, rows, 4, dtype=torch.uint8, device=x.device)
     L.call("bkg_mx4_quantize", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, codes.data_ptr(), scales.data_ptr(),
            L.stream())
     return Mx4Table(codes, scales, (rows, cols))

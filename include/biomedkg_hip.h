@@ -667,8 +667,9 @@ int bkg_distill_forward(const void* x, int32_t type, int64_t ldx, int64_t rows, 
 int bkg_distill_backward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, const void* ids, int32_t ids_i32,
                          int64_t ld_ids, const void* t, int32_t t_type, int64_t ld_t, int32_t k, float temp,
                          const float* row_stats, const float* g, int32_t g_step, float coef, void* d, int64_t ldd, void* stream);
-/* Microscaled 4-bit tables.  codes [rows, P / 2] and scales [rows, P / 32] bytes, P = cols rounded up to 128; two columns a
- * byte (lower one in the low nibble), a scale byte is the exponent of 32 columns + 127 (255: the block is NaN). */
+/* Microscaled 4-bit tables in panels of 128 columns: codes [panels, rows, 64] and scales [panels, rows, 4] bytes (codes 16-byte,
+ * scales 4-byte aligned); two columns a byte (the lower one in the low nibble), a scale byte is the exponent of 32 columns +
+ * 127 (255: the block is NaN). */
 int bkg_mx4_quantize(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t cols, void* codes, void* scales, void* stream);
 int bkg_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int32_t type, int64_t ldo,
                        void* stream);

@@ -394,12 +394,13 @@ def check_mx4(x):
     code, e, value = plain_mx4(x)
     rows, cols = x.shape
     p = (cols + 127) // 128 * 128
-    got = torch.stack([q.codes.cpu() & 15, q.codes.cpu() >> 4], 2).view(rows, p).long()
+    codes = q.codes.cpu().permute(1, 0, 2).reshape(rows, p // 2)
+    got = torch.stack([codes & 15, codes >> 4], 2).view(rows, p).long()
     live = torch.repeat_interleave(e != 128, 32, dim=1)[:, :cols]
     assert torch.equal(torch.where(live, got[:, :cols], 0), torch.where(live, code[:, :cols], 0))
     assert int(got[:, cols:].max() if p > cols else 0) == 0                # padded columns are zeros
     blocks = (cols + 31) // 32
-    assert torch.equal(q.scales.cpu()[:, :blocks].long(), e.long() + 127)
+    assert torch.equal(q.scales.cpu().permute(1, 0, 2).reshape(rows, p // 32)[:, :blocks].long(), e.long() + 127)
     for dt in (torch.float32, torch.bfloat16):
         check(ops.mx4_dequantize(q, dt), value, 0.0)
     h, t = half_step(torch.float16)
@@ -436,7 +437,7 @@ def test_mx4_quantize_strides():
     check_mx4(big.t()[:50])
     check_mx4(big[:1].expand(4, 333))
     check_mx4(torch.randn(20, 264, generator=gen).to(torch.bfloat16).cuda()[:, 8:])
-    assert ops.mx4_quantize(big[:0]).codes.shape == (0, 192)
+    assert ops.mx4_quantize(big[:0]).codes.shape == (3, 0, 64)
 
 
 def check_linear(x, w, bias, out_dtype, got=None):
@@ -458,7 +459,7 @@ def check_linear(x, w, bias, out_dtype, got=None):
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 130, 256), (3, 17, 33), (16, 300, 128), (17, 64, 129), (33, 129, 200),
                                    (130, 257, 256), (64, 1000, 768), (300, 70, 1000), (257, 513, 384), (5, 5000, 256),
-                                   (129, 128, 2048)])
+                                   (129, 128, 2048), (4099, 4100, 1100), (3, 70000, 1025)])
 @pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                        (torch.float16, torch.float32), (torch.bfloat16, torch.float16)])
 def test_mx4_linear(m, n, k, dtype, out):
@@ -580,7 +581,7 @@ def test_entity_ops_refuse_cpu_tensors():
         ops.topk_distill_loss(w, torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2))
     with pytest.raises(L.HipLibraryError):
         ops.mx4_quantize(w)
-    table = ops.Mx4Table(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8), (4, 8))
+    table = ops.Mx4Table(torch.zeros(1, 4, 64, dtype=torch.uint8), torch.zeros(1, 4, 4, dtype=torch.uint8), (4, 8))
     with pytest.raises(L.HipLibraryError):
         ops.mx4_linear(w, table)
     with pytest.raises(L.HipLibraryError):
@@ -615,7 +616,7 @@ def test_entity_ops_refuse_bad_arguments():
     with pytest.raises(TypeError):
         ops.mx4_dequantize(w)
     with pytest.raises(ValueError):
-        ops.Mx4Table(torch.zeros(4, 63, dtype=torch.uint8), torch.zeros(4, 4, dtype=torch.uint8), (4, 8))
+        ops.Mx4Table(torch.zeros(1, 4, 63, dtype=torch.uint8), torch.zeros(1, 4, 4, dtype=torch.uint8), (4, 8))
 
 
 @pytest.mark.gpu
