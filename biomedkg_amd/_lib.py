@@ -166,8 +166,8 @@ SIGNATURES = {
     "bkg_embed_grad_workspace_bytes": (I64, [I64, I64]),
     "bkg_embed_grad": (I32, [P, I32, I64, I64, P, I32, I64, I64, I64, F32, P, P, I64, P]),
     "bkg_distill_workspace_floats": (I64, [I64, I64, I32]),
-    "bkg_distill_forward": (I32, [P, I32, I64, I64, I64, P, I32, I64, P, I32, I64, I32, F32, F32, P, P, P, P, P]),
-    "bkg_distill_backward": (I32, [P, I32, I64, I64, I64, P, I32, I64, P, I32, I64, I32, F32, P, P, I32, F32, P, I64, P]),
+    "bkg_distill_forward": (I32, [P, I32, I64, I64, I64, P, I32, I64, P, I32, I64, I32, F32, F32, P, P, P, P, P, I64, P]),
+    "bkg_distill_backward": (I32, [P, I32, I64, I64, I64, P, I32, I64, P, I32, I64, I32, F32, P, P, I32, F32, I32, P, I64, P]),
     "bkg_mx4_quantize": (I32, [P, I32, I64, I64, I64, P, P, P]),
     "bkg_mx4_dequantize": (I32, [P, P, I64, I64, P, I32, I64, P]),
     "bkg_mx4_matmul": (I32, [P, P, I64, P, P, I64, I64, P, P, I32, I64, P]),

@@ -6,13 +6,17 @@
 // (an id that occurs twice takes both entries' q).  A row without a usable entry, or whose logits are all -inf, is left out:
 // loss 0, gradient 0.  K = 1 is cross entropy.
 //
-// Bound by HBM: the forward reads x once (running maximum and sum of exponentials in fp32, one pass), the backward reads x
-// and writes its gradient.
+// Bound by HBM: x is read once for the running maximum and sum of exponentials (fp32, one pass), and once more where the
+// gradient is written.  A training call writes the gradient of the mean / sum in the FORWARD, behind each row's (or the whole
+// batch's) statistics, while the logits still lie in the caches: HBM sees them once.  That gradient is for an upstream
+// factor of 1; the backward launch looks at the factor on the device and returns at once if it is 1, else it computes the
+// gradient again from the logits (kd_regrad).
 #include "rowtypes.h"
 
 namespace bkg {
 
-constexpr int KD_THREADS = 256;
+constexpr int KD_THREADS = 256;                  // blocks that share a row
+constexpr int KD_ROW_THREADS = 1024;             // a block that has a row to itself
 constexpr int KD_MAX_K = 1024;
 constexpr float KD_LOG2E = 1.4426950408889634f, KD_LN2 = 0.6931471805599453f;
 
@@ -21,15 +25,25 @@ struct KdTeacher {
   const void* t; int t_type; int64_t ld_t;
   int k;
 };
-struct KdRow { float m, sum, tmax, tsum; };      // max and sum of exp of x / T around it; the same of the usable entries.
-                                                 // tsum = 0: no usable entry; sum = 0: the logits are all -inf
+struct KdRow { float m, sum, tmax, tsum; };      // max of x and sum of exp2(c (x - max)), c = log2(e) / T; the same of the usable
+                                                 // entries.  tsum = sum = 0: the row is left out
+struct KdArgs {
+  const void* x; int64_t ldx; int v, parts;
+  float c, temp;
+  KdTeacher te;
+  float* part;                                   // [rows][parts][2]
+  KdRow* rows; float* losses;
+  void* d; int64_t ldd;                          // the gradient (null: none)
+  const float* g; int g_step; float coef;        // d = g[row g_step] coef (p - q); g null: 1
+  int64_t n_rows;
+};
 
-__device__ __forceinline__ float kd_exp(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float kd_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// (m, s) joined with (m2, s2): s exp(m) + s2 exp(m2); c = log2(e) / T.  -inf maxima carry s = 0 or NaN.
+// (m, s) joined with (m2, s2): sums around the larger maximum.  -inf maxima carry s = 0 or NaN.
 __device__ __forceinline__ void kd_join(float& m, float& s, float m2, float s2, float c) {
   const float mm = fmaxf(m, m2), ref = mm == -INFINITY ? 0.f : mm;
-  s = s * kd_exp((m - ref) * c) + s2 * kd_exp((m2 - ref) * c);
+  s = s * kd_exp2((m - ref) * c) + s2 * kd_exp2((m2 - ref) * c);
   m = mm;
 }
 
@@ -75,53 +89,52 @@ template <typename T> struct KdSpan {
   }
 };
 
-// per-row partial (max, sum): part[(row * parts + p) * 2]
-template <typename T>
-__global__ __launch_bounds__(KD_THREADS) void kd_stats_kernel(const T* __restrict__ x, int64_t ldx, int v, int parts, float c,
-                                                              float* __restrict__ part) {
+// Running maximum and sum of this thread's columns.  exp2(c (x - m)), not exp2(c x - c m): the difference is exact near the
+// maximum whatever the row's offset, and logits at the type's lowest or largest value do not overflow.
+template <typename T, int THREADS>
+__device__ __forceinline__ void kd_stats(const T* __restrict__ xr, const KdSpan<T>& sp, float c, float& m, float& s) {
   constexpr int VE = KdSpan<T>::VE, U = 4;
-  __shared__ float red_m[KD_THREADS / 64], red_s[KD_THREADS / 64];
-  const int64_t row = blockIdx.x / parts;
-  const int p = blockIdx.x % parts;
-  const T* xr = x + row * ldx;
-  const KdSpan<T> sp(xr, v, p, parts);
   const Pack<T, VE>* xv = reinterpret_cast<const Pack<T, VE>*>(xr + sp.first);
-  float m = -INFINITY, s = 0.f;
+  float ref = 0.f;                                                    // m, 0 while m = -inf
   auto one = [&](float f) {
-    if (f > m) { s *= kd_exp((m - f) * c); m = f; }                  // (s = 0 while m = -inf)
-    s += kd_exp((f - (m == -INFINITY ? 0.f : m)) * c);
+    if (f > m) { s *= kd_exp2((m - f) * c); m = ref = f; }            // (s = 0 while m = -inf)
+    s += kd_exp2((f - ref) * c);
   };
-  for (int i = threadIdx.x; i < sp.head; i += KD_THREADS) one(widen(xr[i]));
-  for (int i = sp.tail0 + threadIdx.x; i < sp.tail1; i += KD_THREADS) one(widen(xr[i]));
-  for (int i = sp.v0 + threadIdx.x; i < sp.v1; i += KD_THREADS * U) {
+  for (int i = threadIdx.x; i < sp.head; i += THREADS) one(widen(xr[i]));
+  for (int i = sp.tail0 + threadIdx.x; i < sp.tail1; i += THREADS) one(widen(xr[i]));
+  auto pack = [&](const Pack<T, VE>& r) {
+    float f[VE], top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) { f[j] = widen(r.v[j]); top = fmaxf(top, f[j]); }
+    if (top > m) { s *= kd_exp2((m - top) * c); m = ref = top; }
+#pragma unroll
+    for (int j = 0; j < VE; ++j) s += kd_exp2((f[j] - ref) * c);
+  };
+  int i = sp.v0 + threadIdx.x;
+  for (; i + (U - 1) * THREADS < sp.v1; i += THREADS * U) {
     Pack<T, VE> r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u * KD_THREADS < sp.v1) r[u] = xv[i + u * KD_THREADS];
+    for (int u = 0; u < U; ++u) r[u] = xv[i + u * THREADS];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u * KD_THREADS >= sp.v1) break;
-      float f[VE], top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < VE; ++j) { f[j] = widen(r[u].v[j]); top = fmaxf(top, f[j]); }
-      if (top > m) { s *= kd_exp((m - top) * c); m = top; }
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int j = 0; j < VE; ++j) s += kd_exp((f[j] - ref) * c);
-    }
+    for (int u = 0; u < U; ++u) pack(r[u]);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) kd_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
-  if ((threadIdx.x & 63) == 0) { red_m[threadIdx.x >> 6] = m; red_s[threadIdx.x >> 6] = s; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < KD_THREADS / 64; ++w) kd_join(m, s, red_m[w], red_s[w], c);
-    part[2 * (int64_t)blockIdx.x] = m;
-    part[2 * (int64_t)blockIdx.x + 1] = s;
-  }
+  for (; i < sp.v1; i += THREADS) pack(xv[i]);
 }
 
-// The row's teacher entries into LDS: id (or -1 where not usable) and t; returns (tmax, tsum).
+// The block's (m, s) from its threads'; every thread gets it.
+template <int THREADS>
+__device__ __forceinline__ void kd_block_join(float& m, float& s, float c, float* red) {        // red: 2 THREADS / 64 floats
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) kd_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) { red[2 * (threadIdx.x >> 6)] = m; red[2 * (threadIdx.x >> 6) + 1] = s; }
+  __syncthreads();
+  m = red[0]; s = red[1];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) kd_join(m, s, red[2 * w], red[2 * w + 1], c);
+}
+
+// The row's teacher entries into LDS: id (-1 where not usable) and t.
 __device__ __forceinline__ void kd_load_teacher(const KdTeacher& te, int64_t row, int v, int* __restrict__ id_lds,
                                                 float* __restrict__ t_lds) {
   for (int j = threadIdx.x; j < te.k; j += blockDim.x) {
@@ -137,41 +150,148 @@ __device__ __forceinline__ void kd_load_teacher(const KdTeacher& te, int64_t row
   __syncthreads();
 }
 
-// One block per row: the parts joined, the teacher's softmax, the loss; rows[row] keeps what the backward needs.
-template <typename T>
-__global__ __launch_bounds__(KD_THREADS) void kd_rows_kernel(const T* __restrict__ x, int64_t ldx, int v, int parts, float c,
-                                                             float temp, const KdTeacher te, const float* __restrict__ part,
-                                                             KdRow* __restrict__ rows, float* __restrict__ losses) {
-  __shared__ int id_lds[KD_MAX_K];
-  __shared__ float t_lds[KD_MAX_K], red[KD_THREADS / 64];
-  const int64_t row = blockIdx.x;
-  float m = -INFINITY, s = 0.f;
-  for (int p = 0; p < parts; ++p) kd_join(m, s, part[2 * (row * parts + p)], part[2 * (row * parts + p) + 1], c);
-  kd_load_teacher(te, row, v, id_lds, t_lds);
-  float tm = -INFINITY;
+// The usable entries' maximum and sum (the sum is 0 without one); t_lds becomes q.
+__device__ __forceinline__ void kd_teacher_softmax(int k, float c, const int* __restrict__ id_lds, float* __restrict__ t_lds,
+                                                   float* red, float& tm, float& ts) {
+  tm = -INFINITY;
   bool any = false;
-  for (int j = threadIdx.x; j < te.k; j += KD_THREADS)
+  for (int j = threadIdx.x; j < k; j += blockDim.x)
     if (id_lds[j] >= 0) { tm = fmaxf(tm, t_lds[j]); any = true; }
   tm = kd_block_max(tm, red);
   any = __syncthreads_or(any);
-  float ts = 0.f;
-  for (int j = threadIdx.x; j < te.k; j += KD_THREADS)
-    if (id_lds[j] >= 0) ts += kd_exp((t_lds[j] - tm) * c);
+  ts = 0.f;
+  for (int j = threadIdx.x; j < k; j += blockDim.x)
+    if (id_lds[j] >= 0) ts += kd_exp2((t_lds[j] - tm) * c);
   ts = kd_block_sum(ts, red);
-  const float ln_s = KD_LN2 * __builtin_amdgcn_logf(s), ln_ts = KD_LN2 * __builtin_amdgcn_logf(ts);
-  const float inv_t = c * KD_LN2, inv_ts = 1.f / ts;
+  if (!any) ts = 0.f;
+}
+
+// The row's loss from its statistics, in every thread (t_lds still holds t).
+template <typename T>
+__device__ __forceinline__ float kd_loss(const KdArgs& a, const T* __restrict__ xr, const int* __restrict__ id_lds,
+                                         const float* __restrict__ t_lds, float m, float s, float tm, float ts, float* red) {
+  const float ln_s = KD_LN2 * __builtin_amdgcn_logf(s), ln_ts = KD_LN2 * __builtin_amdgcn_logf(ts), inv_ts = 1.f / ts;
+  const float inv_t = a.c * KD_LN2;
   float loss = 0.f;
-  for (int j = threadIdx.x; j < te.k; j += KD_THREADS) {
+  for (int j = threadIdx.x; j < a.te.k; j += blockDim.x) {
     if (id_lds[j] < 0) continue;
-    const float q = kd_exp((t_lds[j] - tm) * c) * inv_ts;
-    const float ln_q = (t_lds[j] - tm) * inv_t - ln_ts, ln_p = (widen(x[row * ldx + id_lds[j]]) - m) * inv_t - ln_s;
+    const float q = kd_exp2((t_lds[j] - tm) * a.c) * inv_ts;
+    const float ln_q = (t_lds[j] - tm) * inv_t - ln_ts, ln_p = (widen(xr[id_lds[j]]) - m) * inv_t - ln_s;
     if (!(q == 0.f)) loss += q * (ln_q - ln_p);
   }
-  loss = kd_block_sum(loss, red);
+  return a.temp * a.temp * kd_block_sum(loss, red);
+}
+
+// The block's part of the row's gradient, scale (p - q).  id_lds / t_lds hold the teacher's entries.
+template <typename T, int THREADS>
+__device__ __forceinline__ void kd_write_grad(const KdArgs& a, const T* __restrict__ xr, T* __restrict__ dr, const KdSpan<T>& sp,
+                                              const KdRow& rw, float scale, const int* __restrict__ id_lds,
+                                              float* __restrict__ t_lds) {
+  constexpr int VE = KdSpan<T>::VE, U = 4;
+  const bool off = rw.tsum == 0.f && rw.sum == 0.f;
+  const float ps = off ? 0.f : scale / rw.sum, c = a.c, ref = rw.m == -INFINITY ? 0.f : rw.m;
+  auto value = [&](float f) { return off ? 0.f : kd_exp2((f - ref) * c) * ps; };
+  for (int i = threadIdx.x; i < sp.head; i += THREADS) dr[i] = (T)value(widen(xr[i]));
+  for (int i = sp.tail0 + threadIdx.x; i < sp.tail1; i += THREADS) dr[i] = (T)value(widen(xr[i]));
+  const Pack<T, VE>* xv = reinterpret_cast<const Pack<T, VE>*>(xr + sp.first);
+  T* dv = dr + sp.first;
+  auto pack = [&](Pack<T, VE> r, int i) {
+#pragma unroll
+    for (int j = 0; j < VE; ++j) r.v[j] = (T)value(widen(r.v[j]));
+    store16(dv + (int64_t)i * VE, r);
+  };
+  if ((reinterpret_cast<uintptr_t>(dv) & 15) == 0) {
+    int i = sp.v0 + threadIdx.x;
+    for (; i + (U - 1) * THREADS < sp.v1; i += THREADS * U) {
+      Pack<T, VE> r[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) r[u] = xv[i + u * THREADS];
+#pragma unroll
+      for (int u = 0; u < U; ++u) pack(r[u], i + u * THREADS);
+    }
+    for (; i < sp.v1; i += THREADS) pack(xv[i], i);
+  } else {                                                            // x and d begin at different places of 16 bytes
+    for (int i = sp.v0 * VE + threadIdx.x; i < sp.v1 * VE; i += THREADS) dv[i] = (T)value(widen(xr[sp.first + i]));
+  }
+  if (off) return;
+  const float inv_ts = 1.f / rw.tsum;
+  for (int j = threadIdx.x; j < a.te.k; j += THREADS) t_lds[j] = kd_exp2((t_lds[j] - rw.tmax) * c) * inv_ts;
+  __syncthreads();                                                    // (also orders the stores above before the ones below)
+  for (int j = threadIdx.x; j < a.te.k; j += THREADS) {               // the entries' columns are written again, whole
+    const int id = id_lds[j];
+    if (id < 0 || !sp.mine(id)) continue;
+    bool first = true;
+    float q = 0.f;
+    for (int i = 0; i < a.te.k; ++i) {
+      const bool same = id_lds[i] == id;
+      first = first && (i >= j || !same);
+      q += same ? t_lds[i] : 0.f;
+    }
+    if (first) dr[id] = (T)(value(widen(xr[id])) - scale * q);
+  }
+}
+
+// ---- a row per block: statistics, loss and (d given) the gradient of its own loss
+template <typename T>
+__global__ __launch_bounds__(KD_ROW_THREADS) void kd_row_kernel(const KdArgs a) {
+  __shared__ int id_lds[KD_MAX_K];
+  __shared__ float t_lds[KD_MAX_K], red[2 * KD_ROW_THREADS / 64];
+  const int64_t row = blockIdx.x;
+  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+  const KdSpan<T> sp(xr, a.v, 0, 1);
+  float m = -INFINITY, s = 0.f, tm, ts;
+  kd_load_teacher(a.te, row, a.v, id_lds, t_lds);
+  kd_stats<T, KD_ROW_THREADS>(xr, sp, a.c, m, s);
+  kd_block_join<KD_ROW_THREADS>(m, s, a.c, red);
+  kd_teacher_softmax(a.te.k, a.c, id_lds, t_lds, red, tm, ts);
+  const float loss = kd_loss(a, xr, id_lds, t_lds, m, s, tm, ts, red);
+  const bool off = ts == 0.f || (m == -INFINITY && s == 0.f);
+  const KdRow rw{m, off ? 0.f : s, tm, off ? 0.f : ts};
   if (threadIdx.x == 0) {
-    const bool off = !any || (m == -INFINITY && s == 0.f);
-    losses[row] = off ? 0.f : temp * temp * loss;
-    rows[row] = KdRow{m, off ? 0.f : s, tm, off ? 0.f : ts};
+    a.losses[row] = off ? 0.f : loss;
+    a.rows[row] = rw;
+  }
+  if (a.d) kd_write_grad<T, KD_ROW_THREADS>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, rw, a.coef, id_lds, t_lds);
+}
+
+// ---- few rows: a.parts blocks share one.  First the parts' statistics ...
+template <typename T>
+__global__ __launch_bounds__(KD_THREADS) void kd_part_kernel(const KdArgs a) {
+  __shared__ float red[2 * KD_THREADS / 64];
+  const int64_t row = blockIdx.x / a.parts;
+  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+  const KdSpan<T> sp(xr, a.v, blockIdx.x % a.parts, a.parts);
+  float m = -INFINITY, s = 0.f;
+  kd_stats<T, KD_THREADS>(xr, sp, a.c, m, s);
+  kd_block_join<KD_THREADS>(m, s, a.c, red);
+  if (threadIdx.x == 0) { a.part[2 * (int64_t)blockIdx.x] = m; a.part[2 * (int64_t)blockIdx.x + 1] = s; }
+}
+// ... then, joined, the row's loss (part 0) and the parts' gradients (d given; else the grid is one block per row)
+template <typename T>
+__global__ __launch_bounds__(KD_THREADS) void kd_join_kernel(const KdArgs a) {
+  __shared__ int id_lds[KD_MAX_K];
+  __shared__ float t_lds[KD_MAX_K], red[2 * KD_THREADS / 64];
+  const int64_t row = a.d ? blockIdx.x / a.parts : blockIdx.x;
+  const int p = a.d ? blockIdx.x % a.parts : 0;
+  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+  kd_load_teacher(a.te, row, a.v, id_lds, t_lds);
+  float m = -INFINITY, s = 0.f, tm, ts;
+  for (int i = threadIdx.x; i < a.parts; i += KD_THREADS)
+    kd_join(m, s, a.part[2 * (row * a.parts + i)], a.part[2 * (row * a.parts + i) + 1], a.c);
+  kd_block_join<KD_THREADS>(m, s, a.c, red);
+  kd_teacher_softmax(a.te.k, a.c, id_lds, t_lds, red, tm, ts);
+  const bool off = ts == 0.f || (m == -INFINITY && s == 0.f);
+  const KdRow rw{m, off ? 0.f : s, tm, off ? 0.f : ts};
+  if (p == 0) {
+    const float loss = kd_loss(a, xr, id_lds, t_lds, m, s, tm, ts, red);
+    if (threadIdx.x == 0) {
+      a.losses[row] = off ? 0.f : loss;
+      a.rows[row] = rw;
+    }
+  }
+  if (a.d) {
+    const KdSpan<T> sp(xr, a.v, p, a.parts);
+    kd_write_grad<T, KD_THREADS>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, rw, a.coef, id_lds, t_lds);
   }
 }
 
@@ -185,50 +305,20 @@ __global__ __launch_bounds__(1024) void kd_sum_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) out[0] = scale * s;
 }
 
-// d[row, :] = g_row * coef * (p - q); g: one value per row (g_step = 1) or one for all (0)
+// ---- the gradient from the kept row statistics.  unless_one: d already holds the gradient for g = 1.
 template <typename T>
-__global__ __launch_bounds__(KD_THREADS) void kd_grad_kernel(const T* __restrict__ x, int64_t ldx, int v, int parts, float c,
-                                                             const KdTeacher te, const KdRow* __restrict__ rows,
-                                                             const float* __restrict__ g, int g_step, float coef,
-                                                             T* __restrict__ d, int64_t ldd, int same_phase) {
-  constexpr int VE = KdSpan<T>::VE;
+__global__ __launch_bounds__(KD_THREADS) void kd_regrad_kernel(const KdArgs a, int unless_one) {
   __shared__ int id_lds[KD_MAX_K];
-  __shared__ float q_lds[KD_MAX_K];
-  const int64_t row = blockIdx.x / parts;
-  const int p = blockIdx.x % parts;
-  const T* xr = x + row * ldx;
-  T* dr = d + row * ldd;
-  const KdSpan<T> sp(xr, v, p, parts);
-  const KdRow rw = rows[row];
-  const bool off = rw.tsum == 0.f && rw.sum == 0.f;
-  const float scale = g[row * g_step] * coef, ps = off ? 0.f : scale / rw.sum;
-  auto value = [&](float f) { return off ? 0.f : kd_exp((f - rw.m) * c) * ps; };
-  for (int i = threadIdx.x; i < sp.head; i += KD_THREADS) dr[i] = (T)value(widen(xr[i]));
-  for (int i = sp.tail0 + threadIdx.x; i < sp.tail1; i += KD_THREADS) dr[i] = (T)value(widen(xr[i]));
-  const Pack<T, VE>* xv = reinterpret_cast<const Pack<T, VE>*>(xr + sp.first);
-  for (int i = sp.v0 + threadIdx.x; i < sp.v1; i += KD_THREADS) {
-    Pack<T, VE> r = xv[i];
-#pragma unroll
-    for (int j = 0; j < VE; ++j) r.v[j] = (T)value(widen(r.v[j]));
-    if (same_phase) *(reinterpret_cast<Pack<T, VE>*>(dr + sp.first) + i) = r;
-    else
-#pragma unroll
-      for (int j = 0; j < VE; ++j) dr[sp.first + i * VE + j] = r.v[j];
-  }
-  if (off) return;
-  kd_load_teacher(te, row, v, id_lds, q_lds);                         // (its barrier also orders the stores above)
-  const float inv_ts = 1.f / rw.tsum;
-  for (int j = threadIdx.x; j < te.k; j += KD_THREADS) q_lds[j] = kd_exp((q_lds[j] - rw.tmax) * c) * inv_ts;
-  __syncthreads();
-  for (int j = threadIdx.x; j < te.k; j += KD_THREADS) {              // the entries' columns are written again, whole
-    const int id = id_lds[j];
-    if (id < 0 || !sp.mine(id)) continue;
-    bool first = true;
-    for (int i = 0; i < j; ++i) first = first && id_lds[i] != id;
-    if (!first) continue;
-    float q = 0.f;
-    for (int i = j; i < te.k; ++i) q += id_lds[i] == id ? q_lds[i] : 0.f;
-    dr[id] = (T)(value(widen(xr[id])) - scale * q);
+  __shared__ float t_lds[KD_MAX_K];
+  if (unless_one && a.g[0] == 1.f) return;
+  for (int64_t b = blockIdx.x; b < a.n_rows * a.parts; b += gridDim.x) {
+    const int64_t row = b / a.parts;
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+    const KdSpan<T> sp(xr, a.v, (int)(b % a.parts), a.parts);
+    __syncthreads();                                                  // (the entries of the block's last row are done with)
+    kd_load_teacher(a.te, row, a.v, id_lds, t_lds);
+    kd_write_grad<T, KD_THREADS>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, a.rows[row], a.g[row * a.g_step] * a.coef, id_lds,
+                                 t_lds);
   }
 }
 
@@ -263,37 +353,43 @@ extern "C" int64_t bkg_distill_workspace_floats(int64_t rows, int64_t v, int32_t
   return rows <= 0 || v <= 0 ? 0 : 2 * rows * kd_parts(rows, v, type_bytes(type));
 }
 
+// Few rows are shared by several blocks; from 192 rows on a block per row keeps three quarters of the CUs or more at work.
+static bool kd_row_per_block(int64_t rows) { return rows >= 192; }
+
 extern "C" int bkg_distill_forward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, const void* ids,
                                    int32_t ids_i32, int64_t ld_ids, const void* t, int32_t t_type, int64_t ld_t, int32_t k,
                                    float temp, float sum_scale, float* workspace, float* row_stats, float* losses, float* loss,
-                                   void* stream) {
+                                   void* d, int64_t ldd, void* stream) {
   if (const int rc = kd_check("bkg_distill_forward", x, type, ldx, rows, v, k, t_type, temp)) return rc;
   BKG_ARG(ids && t && workspace && row_stats && losses, "bkg_distill_forward: null buffer");
+  const int e = type_bytes(type);
+  BKG_ARG(!d || (ldd >= v && (uintptr_t)d % e == 0), "bkg_distill_forward: misaligned gradient or overlapping rows");
   hipStream_t s = (hipStream_t)stream;
-  const int parts = kd_parts(rows, v, type_bytes(type));
-  const float c = KD_LOG2E / temp;
-  const KdTeacher te{ids, ids_i32, ld_ids, t, t_type, ld_t, k};
-  BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_stats_kernel<T>), dim3((unsigned)(rows * parts)), dim3(KD_THREADS), 0, s, (const T*)x,
-                                       ldx, (int)v, parts, c, workspace));
-  BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_rows_kernel<T>), dim3((unsigned)rows), dim3(KD_THREADS), 0, s, (const T*)x, ldx, (int)v,
-                                       parts, c, temp, te, workspace, (KdRow*)row_stats, losses));
+  KdArgs a{x, ldx, (int)v, kd_parts(rows, v, e), KD_LOG2E / temp, temp, {ids, ids_i32, ld_ids, t, t_type, ld_t, k},
+           workspace, (KdRow*)row_stats, losses, d, ldd, nullptr, 0, temp * sum_scale, rows};
+  if (kd_row_per_block(rows)) {
+    BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_row_kernel<T>), dim3((unsigned)rows), dim3(KD_ROW_THREADS), 0, s, a));
+  } else {
+    BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_part_kernel<T>), dim3((unsigned)(rows * a.parts)), dim3(KD_THREADS), 0, s, a));
+    BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_join_kernel<T>), dim3((unsigned)(d ? rows * a.parts : rows)), dim3(KD_THREADS), 0, s, a));
+  }
   if (loss) hipLaunchKernelGGL(kd_sum_kernel, dim3(1), dim3(1024), 0, s, losses, rows, sum_scale, loss);
   return check_launch("bkg_distill_forward");
 }
 
 extern "C" int bkg_distill_backward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, const void* ids,
                                     int32_t ids_i32, int64_t ld_ids, const void* t, int32_t t_type, int64_t ld_t, int32_t k,
-                                    float temp, const float* row_stats, const float* g, int32_t g_step, float coef, void* d,
-                                    int64_t ldd, void* stream) {
+                                    float temp, const float* row_stats, const float* g, int32_t g_step, float coef,
+                                    int32_t unless_one, void* d, int64_t ldd, void* stream) {
   if (const int rc = kd_check("bkg_distill_backward", x, type, ldx, rows, v, k, t_type, temp)) return rc;
   const int e = type_bytes(type);
   BKG_ARG(ids && t && row_stats && g && d && ldd >= v && (uintptr_t)d % e == 0, "bkg_distill_backward: null or misaligned buffer");
+  BKG_ARG(!unless_one || g_step == 0, "bkg_distill_backward: a kept gradient has one upstream factor");
   hipStream_t s = (hipStream_t)stream;
-  const int parts = kd_parts(rows, v, e);
-  const float c = KD_LOG2E / temp;
-  const KdTeacher te{ids, ids_i32, ld_ids, t, t_type, ld_t, k};
-  const int same = ((uintptr_t)x - (uintptr_t)d) % 16 == 0 && ((ldx - ldd) * e) % 16 == 0;
-  BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_grad_kernel<T>), dim3((unsigned)(rows * parts)), dim3(KD_THREADS), 0, s, (const T*)x,
-                                       ldx, (int)v, parts, c, te, (const KdRow*)row_stats, g, g_step, coef, (T*)d, ldd, same));
+  KdArgs a{x, ldx, (int)v, kd_parts(rows, v, e), KD_LOG2E / temp, temp, {ids, ids_i32, ld_ids, t, t_type, ld_t, k},
+           nullptr, (KdRow*)row_stats, nullptr, d, ldd, g, g_step, coef, rows};
+  // (a launch that may have nothing to do keeps its grid small and loops)
+  const int64_t all = rows * a.parts, grid = unless_one && all > 2048 ? 2048 : all;
+  BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_regrad_kernel<T>), dim3((unsigned)grid), dim3(KD_THREADS), 0, s, a, unless_one));
   return check_launch("bkg_distill_backward");
 }

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
       Pack<T, N> o;
 #pragma unroll
       for (int j = 0; j < N; ++j) o.v[j] = v[h * N + j];
-      reinterpret_cast<Pack<T, N>*>(p)[h] = o;
+      store16(p + h * N, o);
     }
   } else {
     for (int j = 0; j < 8 && c + j < cols; ++j) p[j] = v[j];
@@ -269,11 +269,16 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   static_assert(4 * 32 * PITCH * 4 <= S * STAGE, "the results' staging area lies in the ring");
   T* out = static_cast<T*>(a.out);
   constexpr int VE = 16 / sizeof(T), LPR = WN / VE, RPI = 64 / LPR;   // elements per store, lanes per row, rows per store
-  const int col = (lane % LPR) * VE;
-  const int64_t nc = n0 + wn + col;
+  const int64_t nw = n0 + wn;                                  // the wave's first column
+  const bool wide = a.wide && nw + WN <= a.n;
+  const int col = wide ? (lane % LPR) * VE : lane;
   float bias[VE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) bias[e] = a.bias && nc + e < a.n ? a.bias[nc + e] : 0.f;
+  for (int e = 0; e < VE; ++e) bias[e] = 0.f;
+  if (a.bias) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) bias[e] = a.bias[min(nw + (wide ? col + e : col + 64 * e), a.n - 1)];
+  }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -282,20 +287,21 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
       for (int r = 0; r < 16; ++r) mine[(8 * (r >> 2) + 4 * half + (r & 3)) * PITCH + 32 * j + l31] = acc[i][j][r];
     // (a wave's LDS operations complete in order and the area is its own: no barrier)
     const int64_t mr = m0 + wm + 32 * i;
+    if (wide) {
 #pragma unroll
-    for (int r = 0; r < 32 / RPI; ++r) {
-      const int row = r * RPI + lane / LPR;
-      Pack<T, VE> o;
+      for (int r = 0; r < 32 / RPI; ++r) {
+        const int row = r * RPI + lane / LPR;
+        Pack<T, VE> o;
 #pragma unroll
-      for (int e = 0; e < VE; ++e) o.v[e] = (T)(mine[row * PITCH + col + e] + bias[e]);
-      if (mr + row < a.m) {
-        T* dst = out + (mr + row) * a.ldo + nc;
-        if (a.wide && nc + VE <= a.n) *reinterpret_cast<Pack<T, VE>*>(dst) = o;
-        else
-#pragma unroll
-          for (int e = 0; e < VE; ++e)
-            if (nc + e < a.n) dst[e] = o.v[e];
+        for (int e = 0; e < VE; ++e) o.v[e] = (T)(mine[row * PITCH + col + e] + bias[e]);
+        if (mr + row < a.m) store16(out + (mr + row) * a.ldo + nw + col, o);
       }
+    } else {                                                   // the last columns, or rows that are not 16-byte aligned
+      const int rows_here = (int)min((int64_t)32, a.m - mr);
+      for (int row = 0; row < rows_here; ++row)
+#pragma unroll
+        for (int e = 0; e < WN / 64; ++e)
+          if (nw + col + 64 * e < a.n) out[(mr + row) * a.ldo + nw + col + 64 * e] = (T)(mine[row * PITCH + col + 64 * e] + bias[e]);
     }
   }
 }

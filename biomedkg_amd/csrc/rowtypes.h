@@ -14,7 +14,14 @@ __device__ __forceinline__ float widen(_Float16 v) { return (float)v; }
 // N consecutive elements as one access (N * sizeof(T) = 2 .. 16 bytes, aligned to their size)
 template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
 
-// log2 of the largest access in bytes (<= 16) that `bytes`, a row of it and its start are all multiples of
+// A 16-byte pack written as ONE store.  (As a plain struct copy hipcc splits it into element stores where another branch
+// writes the same elements one by one: a request per lane instead of one per 64 bytes.)
+typedef int rt_i32x4 __attribute__((ext_vector_type(4)));
+template <typename T> __device__ __forceinline__ void store16(T* p, const Pack<T, 16 / sizeof(T)>& v) {
+  *reinterpret_cast<rt_i32x4*>(p) = __builtin_bit_cast(rt_i32x4, v);
+}
+
+// the largest access in bytes (<= 16) that `bytes`, a row of it and its start are all multiples of
 static inline int access_bytes(const void* p, int64_t row_bytes, int64_t ld_bytes) {
   const uint64_t all = (uint64_t)(uintptr_t)p | (uint64_t)row_bytes | (uint64_t)ld_bytes | 16u;
   return (int)(all & (~all + 1));

@@ -64,18 +64,25 @@ class _Embedding(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        (ids,) = ctx.saved_tensors
-        v, d = ctx.shape
-        n = ids.numel()
-        g = _rows(g.reshape(n, d))
-        dw = torch.empty(v, d, dtype=ctx.dtype, device=g.device)
-        ws_bytes = L.lib().bkg_embed_grad_workspace_bytes(n, d)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device)
-        L.call("bkg_embed_grad", g.data_ptr(), _TYPE[ctx.dtype], g.stride(0), d, ids.data_ptr(), ids.dtype == torch.int32, n, v,
-               ctx.pad, ctx.scale, dw.data_ptr(), ws.data_ptr(), ws_bytes, L.stream())
-        return dw, None, None, None
+        # (the plain path is once_differentiable's without its wrapping: gradients are recorded only under create_graph)
+        return (_embedding_backward_once if torch.is_grad_enabled() else _embedding_backward)(ctx, g)
+
+
+def _embedding_backward(ctx, g):
+    (ids,) = ctx.saved_tensors
+    v, d = ctx.shape
+    n = ids.numel()
+    g = _rows(g.reshape(n, d))
+    dw = torch.empty(v, d, dtype=ctx.dtype, device=g.device)
+    ws_bytes = L.lib().bkg_embed_grad_workspace_bytes(n, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device)
+    L.call("bkg_embed_grad", g.data_ptr(), _TYPE[ctx.dtype], g.stride(0), d, ids.data_ptr(), ids.dtype == torch.int32, n, v,
+           ctx.pad, ctx.scale, dw.data_ptr(), ws.data_ptr(), ws_bytes, L.stream())
+    return dw, None, None, None
+
+
+_embedding_backward_once = once_differentiable(_embedding_backward)
 
 
 def embedding(weight, ids, scale=1.0, padding_idx=None):
@@ -106,7 +113,7 @@ def embedding(weight, ids, scale=1.0, padding_idx=None):
 
 
 # ----------------------------------------------------------------------------- distillation
-def _distill_forward(x, ids, t, temp, sum_scale, want_sum):
+def _distill_forward(x, ids, t, temp, sum_scale, want_sum, d=None):
     rows, v = x.shape
     dev, xt = x.device, _TYPE[x.dtype]
     ws = torch.empty(L.lib().bkg_distill_workspace_floats(rows, v, xt), dtype=torch.float32, device=dev)
@@ -115,29 +122,50 @@ def _distill_forward(x, ids, t, temp, sum_scale, want_sum):
     loss = torch.empty((), dtype=torch.float32, device=dev) if want_sum else None
     L.call("bkg_distill_forward", x.data_ptr(), xt, x.stride(0), rows, v, ids.data_ptr(), ids.dtype == torch.int32, ids.stride(0),
            t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), temp, sum_scale, ws.data_ptr(), stats.data_ptr(),
-           losses.data_ptr(), L.ptr(loss), L.stream())
+           losses.data_ptr(), L.ptr(loss), L.ptr(d), v, L.stream())
     return (loss if want_sum else losses), stats
 
 
 class _TopkDistill(torch.autograd.Function):
+    """A reduced loss leaves its gradient (for an upstream factor of 1) with the forward, while the logits lie in the caches;
+    the first backward hands it out -- the launch there looks at the factor on the device and computes the gradient again
+    where it is not 1.  A later backward over the same graph, a captured one, and reduction "none" compute it afresh."""
+
     @staticmethod
     def forward(ctx, x, ids, t, temp, mean, want_sum):
-        out, stats = _distill_forward(x, ids, t, temp, 1.0 / x.size(0) if mean else 1.0, want_sum)
+        sum_scale = 1.0 / x.size(0) if mean else 1.0
+        d = None
+        if want_sum and not torch.cuda.is_current_stream_capturing():
+            d = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out, stats = _distill_forward(x, ids, t, temp, sum_scale, want_sum, d)
         ctx.save_for_backward(x, ids, t, stats)
-        ctx.temp, ctx.coef, ctx.g_step = temp, (temp / x.size(0) if mean else temp), int(not want_sum)
+        ctx.made, ctx.temp, ctx.coef, ctx.g_step = d, temp, temp * sum_scale, int(not want_sum)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        x, ids, t, stats = ctx.saved_tensors
-        rows, v = x.shape
-        g = g.to(torch.float32).contiguous()
+        if not torch.is_grad_enabled():
+            return _distill_backward(ctx, g)
+        # (the gradient depends on the logits too: a second derivative is refused even where g itself records none)
+        return _distill_backward_once(ctx, g if g.requires_grad else g.detach().requires_grad_())
+
+
+def _distill_backward(ctx, g):
+    x, ids, t, stats = ctx.saved_tensors
+    rows, v = x.shape
+    d, ctx.made = ctx.made, None
+    kept = d is not None and not torch.cuda.is_current_stream_capturing()
+    if not kept:
         d = torch.empty(rows, v, dtype=x.dtype, device=x.device)
-        L.call("bkg_distill_backward", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, v, ids.data_ptr(),
-               ids.dtype == torch.int32, ids.stride(0), t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), ctx.temp,
-               stats.data_ptr(), g.data_ptr(), ctx.g_step, ctx.coef, d.data_ptr(), v, L.stream())
-        return d, None, None, None, None, None
+    if g.dtype != torch.float32 or not g.is_contiguous():
+        g = g.to(torch.float32).contiguous()
+    L.call("bkg_distill_backward", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, v, ids.data_ptr(), ids.dtype == torch.int32,
+           ids.stride(0), t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), ctx.temp, stats.data_ptr(), g.data_ptr(),
+           ctx.g_step, ctx.coef, kept, d.data_ptr(), v, L.stream())
+    return d, None, None, None, None, None
+
+
+_distill_backward_once = once_differentiable(_distill_backward)
 
 
 def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, reduction="batchmean"):
@@ -146,7 +174,8 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, redu
 
     Per row ``T^2 * KL(q || p)`` over the K entries with ``q = softmax(teacher_logits / T)`` over the row's usable entries and
     ``p = softmax(logits / T)`` over all V columns; the gradient is ``T * (p - q)`` in ``logits``'s type, statistics and sums in
-    fp32 (csrc/distill.hip).  ``K = 1`` is cross entropy.  An entry is not usable if its id lies outside ``[0, V)`` (padding:
+    fp32 (csrc/distill.hip).  ``K = 1`` is cross entropy.  A reduced loss that records gradients computes its gradient within
+    the forward call (one pass over the logits less; the backward repeats it only for an upstream factor other than 1).  An entry is not usable if its id lies outside ``[0, V)`` (padding:
     -1) or its logit is ``-inf``; an id that occurs twice counts twice.  A row without a usable entry, or whose logits are all
     ``-inf``, is left out: loss 0, gradient 0.  A usable entry whose student logit is ``-inf`` makes the loss ``inf``; NaN stays
     NaN.

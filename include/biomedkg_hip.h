@@ -658,15 +658,18 @@ int64_t bkg_embed_grad_workspace_bytes(int64_t n, int64_t d);
 int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t d, const void* ids, int32_t ids_i32, int64_t n,
                    int64_t n_rows, int64_t pad, float scale, void* dw, void* workspace, int64_t workspace_bytes, void* stream);
 /* Distillation from a teacher's k best entries per row (csrc/distill.hip has the formulas).  losses [rows] = the rows' losses,
- * loss (nullable) = sum_scale * their sum; row_stats [rows, 4] is what the backward needs. */
+ * loss (nullable) = sum_scale * their sum; row_stats [rows, 4] is what the backward needs.  d (nullable) [rows, v], x's type:
+ * the gradient of sum_scale * the losses' sum. */
 int64_t bkg_distill_workspace_floats(int64_t rows, int64_t v, int32_t type);
 int bkg_distill_forward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, const void* ids, int32_t ids_i32,
                         int64_t ld_ids, const void* t, int32_t t_type, int64_t ld_t, int32_t k, float temp, float sum_scale,
-                        float* workspace, float* row_stats, float* losses, float* loss, void* stream);
-/* d [rows, v] = g[row * g_step] * coef * (softmax(x / temp) - q) in x's type (coef: temp, or temp / rows for the mean) */
+                        float* workspace, float* row_stats, float* losses, float* loss, void* d, int64_t ldd, void* stream);
+/* d [rows, v] = g[row * g_step] * coef * (softmax(x / temp) - q) in x's type (coef: temp * sum_scale).  unless_one (g_step 0):
+ * d already holds the forward's gradient, and nothing is written if g[0] (on the device) is 1. */
 int bkg_distill_backward(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, const void* ids, int32_t ids_i32,
                          int64_t ld_ids, const void* t, int32_t t_type, int64_t ld_t, int32_t k, float temp,
-                         const float* row_stats, const float* g, int32_t g_step, float coef, void* d, int64_t ldd, void* stream);
+                         const float* row_stats, const float* g, int32_t g_step, float coef, int32_t unless_one, void* d,
+                         int64_t ldd, void* stream);
 /* Microscaled 4-bit tables in panels of 128 columns: codes [panels, rows, 64] and scales [panels, rows, 4] bytes (codes 16-byte,
  * scales 4-byte aligned); two columns a byte (the lower one in the low nibble), a scale byte is the exponent of 32 columns +
  * 127 (255: the block is NaN). */

@@ -302,6 +302,39 @@ def test_distill_repeated_ids_and_strides(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 260])
+def test_distill_large_offsets_and_lowest_values(rows):
+    """softmax does not see a row's offset; a row that is the type's lowest value everywhere is uniform"""
+    x, ids, t = make_distill(rows, 700, 5, torch.float32, 17)
+    x = (x * 8).round() / 8                                  # (eighths: 5e4 + x is exact)
+    x[0] += 5e4
+    x[1] -= 5e4
+    x[2] = torch.finfo(torch.float32).min
+    check_distill(x, ids, t, 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,v,k", [(200, 3001, 9), (193, 20, 3), (300, 9000, 40), (191, 9001, 7), (4, 70001, 64)])
+def test_distill_rows_on_both_sides_of_the_split(dtype, rows, v, k):
+    check_distill(*make_distill(rows, v, k, dtype, rows + v + k), 1.25)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x, ids, t = make_distill(3, 50, 4, torch.float32, 18)
+    xx = x.detach().requires_grad_()
+    g, = torch.autograd.grad(ops.topk_distill_loss(xx * xx, ids, t), xx, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    w = torch.randn(5, 8, device="cuda", requires_grad=True)
+    out = ops.embedding(w * w, torch.tensor([1, 2], device="cuda"))
+    g, = torch.autograd.grad((out * out).sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
 def test_distill_k1_is_cross_entropy():
     x, ids, _ = make_distill(40, 1234, 1, torch.float32, 14)
     xx = x.detach().requires_grad_()
