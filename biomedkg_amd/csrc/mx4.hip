@@ -8,17 +8,42 @@
 // scales per row), so the product has no tail in its inner dimension and reads neighbouring rows of a panel as one run.
 //
 // Dividing by s only moves the exponent, so quantisation has one rounding and is the same whatever the input's type.
+#include <algorithm>
+
 #include "rowtypes.h"
 
 namespace bkg {
 
 constexpr int MX_K = 128;                       // columns a row is padded to a multiple of
 
+static int64_t mx4_steps(int64_t cols) { return (cols + MX_K - 1) / MX_K; }
+
 typedef int mx_i32x4 __attribute__((ext_vector_type(4)));
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
+typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
 typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
 
-// ---- 8 values of a row per lane, 4 lanes per block: 16-byte loads of a bf16 / fp16 row, a dword of codes out.
+// ---- 8 values of a row per lane, 4 lanes per block, 16 lanes per panel.  Every lane of the wave takes part; returns the
+// lane's dword of codes and, in the first lane of 16, the panel's dword of scales.
+struct Mx4Piece { uint32_t codes, scales; };
+__device__ __forceinline__ Mx4Piece mx4_piece(const float (&f)[8]) {
+  uint32_t top = 0;                             // largest magnitude's bits (infinities and NaN are the largest)
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+  top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+  const uint32_t field = top >> 23;             // floor(log2) + 127; 0 for zeros and denormals: their E is clamped anyway
+  const uint32_t byte = field == 255u ? 255u : (field > 2u ? field - 2u : 0u);
+  const float inv = __uint_as_float((254u - byte) << 23);               // 2^-E (255: unused)
+  uint32_t q = 0;
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[0] * inv, f[1] * inv, 1.0f, 0);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2] * inv, f[3] * inv, 1.0f, 1);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4] * inv, f[5] * inv, 1.0f, 2);
+  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6] * inv, f[7] * inv, 1.0f, 3);
+  const uint32_t b1 = __shfl_down((int)byte, 4, 64), b2 = __shfl_down((int)byte, 8, 64), b3 = __shfl_down((int)byte, 12, 64);
+  return Mx4Piece{byte == 255u ? 0u : q, byte | (b1 << 8) | (b2 << 16) | (b3 << 24)};
+}
+
 // ALIGNED: the rows' 8-value pieces are 16-byte aligned (fp32: two accesses).
 template <typename T, bool ALIGNED>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int cols,
@@ -46,25 +71,11 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__
         if (c + j < cols) f[j] = widen(p[j]);
     }
   }
-  uint32_t top = 0;                             // largest magnitude's bits (infinities and NaN are the largest)
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
-  top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
-  top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
-  const uint32_t field = top >> 23;             // floor(log2) + 127; 0 for zeros and denormals: their E is clamped anyway
-  const uint32_t byte = field == 255u ? 255u : (field > 2u ? field - 2u : 0u);
-  const float inv = __uint_as_float((254u - byte) << 23);               // 2^-E (255: unused)
-  uint32_t q = 0;
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[0] * inv, f[1] * inv, 1.0f, 0);
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2] * inv, f[3] * inv, 1.0f, 1);
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4] * inv, f[5] * inv, 1.0f, 2);
-  q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6] * inv, f[7] * inv, 1.0f, 3);
-  if (byte == 255u) q = 0;
-  const uint32_t b1 = __shfl_down((int)byte, 4, 64), b2 = __shfl_down((int)byte, 8, 64), b3 = __shfl_down((int)byte, 12, 64);
+  const Mx4Piece q = mx4_piece(f);
   if (row < rows) {
     const int64_t at_row = (int64_t)(piece >> 4) * rows + row;                    // (panel, row)
-    codes[at_row * 16 + (piece & 15)] = q;
-    if ((piece & 15) == 0) scales[at_row] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
+    codes[at_row * 16 + (piece & 15)] = q.codes;
+    if ((piece & 15) == 0) scales[at_row] = q.scales;
   }
 }
 
@@ -109,11 +120,30 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
 // of row l % 32, block l / 32, and that block's scale byte; the result's column is B's row l % 32.  A panel of 128 columns is
 // two such products (h = 0, 1): lane half `half` takes the panel's 16-byte piece 2 h + half and byte 2 h + half of its dword
 // of scales.
+// 32 staged result rows of a wave (PITCH floats apart, 16-byte aligned), W columns, as 16-byte stores: LPR lanes a row.
+template <typename T, int W, int PITCH, bool GUARD>
+__device__ __forceinline__ void mx_store_rows(const float* mine, const float* bias, T* dst, int64_t ldo, int64_t rows_left, int lane) {
+  constexpr int VE = 16 / sizeof(T), LPR = W / VE, RPI = 64 / LPR, N = 32 / RPI;
+  const int col = (lane % LPR) * VE, row0 = lane / LPR;
+  mx_f32x4 v[N][VE / 4];
+#pragma unroll
+  for (int r = 0; r < N; ++r)
+#pragma unroll
+    for (int q = 0; q < VE / 4; ++q) v[r][q] = *reinterpret_cast<const mx_f32x4*>(mine + (r * RPI + row0) * PITCH + col + 4 * q);
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    Pack<T, VE> o;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) o.v[e] = (T)(v[r][e / 4][e % 4] + bias[e]);
+    if (!GUARD || r * RPI + row0 < rows_left) store16(dst + (r * RPI + row0) * ldo + col, o);
+  }
+}
+
 struct Mx4Args {
   const unsigned char* ca; const uint32_t* sa; int64_t m;
   const unsigned char* cb; const uint32_t* sb; int64_t n;
   int steps;                                     // panels of 128 columns
-  int m_tiles, n_tiles;
+  int m_tiles, n_tiles, band;
   const float* bias;
   void* out; int64_t ldo;
   int wide;                                      // the rows of `out` take aligned 16-byte stores
@@ -151,9 +181,9 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   const int64_t total = (int64_t)a.m_tiles * a.n_tiles, per = (total + BKG_XCDS - 1) / BKG_XCDS;
   const int64_t t = (int64_t)(blockIdx.x % BKG_XCDS) * per + blockIdx.x / BKG_XCDS;
   if (blockIdx.x / BKG_XCDS >= per || t >= total) return;
-  const int64_t in_band = 8 * (int64_t)a.n_tiles, band = t / in_band, at = t - band * in_band;
-  const int band_m = (int)min((int64_t)8, a.m_tiles - band * 8);
-  const int64_t m0 = (band * 8 + at % band_m) * BM, n0 = at / band_m * BN;
+  const int64_t in_band = a.band * (int64_t)a.n_tiles, band = t / in_band, at = t - band * in_band;
+  const int band_m = (int)min((int64_t)a.band, a.m_tiles - band * a.band);
+  const int64_t m0 = (band * a.band + at % band_m) * BM, n0 = at / band_m * BN;
 
   // this wave's share of a stage's copies: waves 0 and 1 copy A's 4 MT chunks of 16 rows and MT chunks of 64 scales, waves 2
   // and 3 B's
@@ -268,7 +298,7 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
   static_assert(4 * 32 * PITCH * 4 <= S * STAGE, "the results' staging area lies in the ring");
   T* out = static_cast<T*>(a.out);
-  constexpr int VE = 16 / sizeof(T), LPR = WN / VE, RPI = 64 / LPR;   // elements per store, lanes per row, rows per store
+  constexpr int VE = 16 / sizeof(T), LPR = WN / VE;          // elements per store, lanes per row
   const int64_t nw = n0 + wn;                                  // the wave's first column
   const bool wide = a.wide && nw + WN <= a.n;
   const int col = wide ? (lane % LPR) * VE : lane;
@@ -288,14 +318,7 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
     // (a wave's LDS operations complete in order and the area is its own: no barrier)
     const int64_t mr = m0 + wm + 32 * i;
     if (wide) {
-#pragma unroll
-      for (int r = 0; r < 32 / RPI; ++r) {
-        const int row = r * RPI + lane / LPR;
-        Pack<T, VE> o;
-#pragma unroll
-        for (int e = 0; e < VE; ++e) o.v[e] = (T)(mine[row * PITCH + col + e] + bias[e]);
-        if (mr + row < a.m) store16(out + (mr + row) * a.ldo + nw + col, o);
-      }
+      mx_store_rows<T, WN, PITCH, true>(mine, bias, out + mr * a.ldo + nw, a.ldo, a.m - mr, lane);
     } else {                                                   // the last columns, or rows that are not 16-byte aligned
       const int rows_here = (int)min((int64_t)32, a.m - mr);
       for (int row = 0; row < rows_here; ++row)
@@ -303,6 +326,235 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
         for (int e = 0; e < WN / 64; ++e)
           if (nw + col + 64 * e < a.n) out[(mr + row) * a.ldo + nw + col + 64 * e] = (T)(mine[row * PITCH + col + 64 * e] + bias[e]);
     }
+  }
+}
+
+// Narrow inner dimension (one or two panels: an entity table of up to 256 columns), many outputs: the call is the writing of
+// its outputs.  A block keeps its 128 rows of A in registers (32 at two panels) and walks a range of B's 128-row tiles: tile
+// t + 1 travels into the other of two LDS slots while tile t multiplies and its results leave, so loads, products and stores
+// overlap within a block too, and only B moves (the tiled kernel above loads both operands per 128 x 128 outputs and has
+// nothing in flight while a block stores: 95 against ... us for 1021 x 130000 x 256 in bf16).
+//
+// (Dynamic LDS: reading a static array that LDS-DMAs write makes hipcc wait for every copy in flight.)
+constexpr int MS_PITCH = 64 + 4;                           // floats of a staged result row
+constexpr int ms_lds(int steps) { return 2 * steps * (128 * 64 + 128 * 4) + 4 * 32 * MS_PITCH * 4; }
+template <typename T, int STEPS, bool BIAS>
+__global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
+  constexpr int SLOT = STEPS * (128 * 64 + 128 * 4), PITCH = MS_PITCH;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  unsigned char* const ring = lds;
+  float* const stage = reinterpret_cast<float*>(lds + 2 * SLOT);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, half = lane >> 5;
+  const XcdSlot xs = xcd_slot(blockIdx.x, a.m_tiles);      // the row tiles of one range of B share an XCD's L2
+  const int64_t t0 = (int64_t)xs.outer * a.band, t1 = min(t0 + a.band, (int64_t)a.n_tiles);
+  if (t0 >= t1) return;
+  const int64_t m0 = (int64_t)xs.inner * 128;
+  const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+
+  // copies of a tile: per panel 8 chunks of 16 rows (two a wave) and two of 64 scales (waves 0 and 1: panel 0's, 2 and 3:
+  // panel 1's; with one panel waves 2 and 3 copy it a second time: every wave issues the same number)
+  constexpr int DMAS = 2 * STEPS + 1;
+  auto copy_tile = [&](int64_t tile, int slot) {
+    const int64_t n0 = min(tile, (int64_t)a.n_tiles - 1) * 128;
+    unsigned char* base = ring + slot * SLOT;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int64_t r = min(n0 + (wave * 2 + j) * 16 + (lane >> 2), a.n - 1);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(a.cb + (st * a.n + r) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16),
+            (__attribute__((address_space(3))) void*)(base + st * 8192 + (wave * 2 + j) * 1024), 16, 0, 0);
+      }
+    const int st = STEPS == 2 ? wave >> 1 : 0;
+    const int64_t r = min(n0 + (wave & 1) * 64 + lane, a.n - 1);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.sb + st * a.n + r),
+                                     (__attribute__((address_space(3))) void*)(base + STEPS * 8192 + st * 512 + (wave & 1) * 256), 4, 0, 0);
+  };
+
+  mx_i32x4 fa[2][STEPS][2];
+  uint32_t xa[2][STEPS];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t r = min(m0 + wm + 32 * i + l31, a.m - 1);
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      xa[i][st] = a.sa[st * a.m + r] >> (8 * half);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        fa[i][st][h] = *reinterpret_cast<const mx_i32x4*>(a.ca + (st * a.m + r) * 64 + (2 * h + half) * 16);
+    }
+  }
+  copy_tile(t0, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st)
+      asm volatile("" : "+v"(fa[i][st][0]), "+v"(fa[i][st][1]), "+v"(xa[i][st]));
+
+  constexpr int VE = 16 / sizeof(T), LPR = 64 / VE, RPI = 64 / LPR, STORES = 2 * 32 / RPI;
+  float* mine = stage + wave * 32 * PITCH;
+  T* out = static_cast<T*>(a.out);
+  const int64_t mw = m0 + wm;
+  const bool rows_full = a.wide && mw + 64 <= a.m;
+  bool stores_known = false;                               // the last tile's STORES are behind the current tile's copies
+  int slot = 0;
+  for (int64_t t = t0; t < t1; ++t) {
+    // this wave's copies of tile t have landed: only the last tile's stores were issued behind them (vmcnt retires in order;
+    // where their number is not known -- a guarded tile -- wait for everything)
+    if (stores_known) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                          // everyone's have, and everyone is done with the other slot
+    asm volatile("" ::: "memory");
+    const int64_t nw = t * 128 + wn;
+    const bool wide = rows_full && nw + 64 <= a.n;
+    const int col = wide ? (lane % LPR) * VE : lane;
+    float bias[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) bias[e] = BIAS ? a.bias[min(nw + (wide ? col + e : col), a.n - 1)] : 0.f;
+    copy_tile(t + 1, slot ^ 1);                            // (past the range: valid memory, never read)
+    const unsigned char* base = ring + slot * SLOT;
+    mx_f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      uint32_t xb[2];
+      mx_i32x4 fb[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        xb[j] = *reinterpret_cast<const uint32_t*>(base + STEPS * 8192 + st * 512 + (wn + 32 * j + l31) * 4) >> (8 * half);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          fb[j][h] = *reinterpret_cast<const mx_i32x4*>(base + st * 8192 + (wn + 32 * j + l31) * 64 +
+                                                        (((2 * h + half) ^ ((l31 >> 1) & 3)) * 16));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          acc[i][j] = mx_mfma<0>(fa[i][st][0], fb[j][0], acc[i][j], xa[i][st], xb[j]);
+          acc[i][j] = mx_mfma<1>(fa[i][st][1], fb[j][1], acc[i][j], xa[i][st], xb[j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mine[(8 * (r >> 2) + 4 * half + (r & 3)) * PITCH + 32 * j + l31] = acc[i][j][r];
+      const int64_t mr = mw + 32 * i;
+      if (wide) {
+        mx_store_rows<T, 64, PITCH, false>(mine, bias, out + mr * a.ldo + nw, a.ldo, 32, lane);
+      } else {
+        const int rows_here = (int)min((int64_t)32, a.m - mr);
+        for (int row = 0; row < rows_here; ++row)
+          if (nw + col < a.n) out[(mr + row) * a.ldo + nw + col] = (T)(mine[row * PITCH + col] + bias[0]);
+      }
+    }
+    stores_known = wide;
+    slot ^= 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the copies past the range
+}
+
+// A few rows (m <= 32): B streams from memory straight into the matrix cores, a 32-row tile of it per wave (KSPLIT: per
+// block, the waves share the panels and add their sums in wave order).  PACKED: A lies packed in memory; else the block
+// packs x itself (into LDS) while its first tiles are on their way: one launch, no scratch memory.
+struct Mx4X { const void* x; int type; int64_t ldx; int cols; };
+template <typename T, bool PACKED, bool KSPLIT>
+__global__ __launch_bounds__(256) void mx4_few_kernel(const Mx4Args a, const Mx4X x) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];       // A: [panel][32 rows][64], [panel][32] scales
+  __shared__ float sums[KSPLIT ? 3 * 16 * 64 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, half = lane >> 5;
+  const int64_t n0 = (KSPLIT ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave) * 32;
+  const int64_t rb = min(n0 + l31, a.n - 1), ra = min((int64_t)l31, a.m - 1);
+  constexpr int D = KSPLIT ? 4 : 1, AHEAD = 2;
+  const int first = KSPLIT ? wave : 0;
+  mx_i32x4 vb[AHEAD][2];
+  uint32_t xb[AHEAD];
+  auto load = [&](int st, int at) {
+    const int64_t s = min(st, a.steps - 1);
+    xb[at] = a.sb[s * a.n + rb];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) vb[at][h] = *reinterpret_cast<const mx_i32x4*>(a.cb + (s * a.n + rb) * 64 + (2 * h + half) * 16);
+  };
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) load(first + u * D, u);
+  if constexpr (!PACKED) {
+    const int pieces = a.steps * 16;
+    uint32_t* xs = reinterpret_cast<uint32_t*>(lds + a.steps * 2048);
+    for (int p = threadIdx.x; p < 32 * pieces; p += 256) {                  // (32 * pieces is a multiple of 256)
+      const int row = p / pieces, piece = p - row * pieces, c = piece * 8;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] = 0.f;
+        if (row < a.m && c + j < x.cols) {
+          const int64_t at = row * x.ldx + c + j;
+          f[j] = x.type == BKG_T_F32    ? static_cast<const float*>(x.x)[at]
+                 : x.type == BKG_T_BF16 ? widen(static_cast<const __bf16*>(x.x)[at])
+                                        : widen(static_cast<const _Float16*>(x.x)[at]);
+        }
+      }
+      const Mx4Piece q = mx4_piece(f);
+      const int st = piece >> 4, w = piece & 15;                            // word w of the row's 16: 16-byte piece w / 4, swizzled
+      *reinterpret_cast<uint32_t*>(lds + st * 2048 + row * 64 + (((w >> 2) ^ ((row >> 1) & 3)) * 16) + (w & 3) * 4) = q.codes;
+      if (w == 0) xs[st * 32 + row] = q.scales;
+    }
+    __syncthreads();
+  }
+  mx_f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  auto multiply = [&](int st, int at) {
+    mx_i32x4 va[2];
+    uint32_t xa;
+    if constexpr (PACKED) {
+      xa = a.sa[st * a.m + ra];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) va[h] = *reinterpret_cast<const mx_i32x4*>(a.ca + (st * a.m + ra) * 64 + (2 * h + half) * 16);
+    } else {
+      xa = *reinterpret_cast<const uint32_t*>(lds + a.steps * 2048 + st * 128 + l31 * 4);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        va[h] = *reinterpret_cast<const mx_i32x4*>(lds + st * 2048 + l31 * 64 + (((2 * h + half) ^ ((l31 >> 1) & 3)) * 16));
+    }
+    acc = mx_mfma<0>(va[0], vb[at][0], acc, xa >> (8 * half), xb[at] >> (8 * half));
+    acc = mx_mfma<1>(va[1], vb[at][1], acc, xa >> (8 * half), xb[at] >> (8 * half));
+  };
+  for (int st = first; st < a.steps; st += AHEAD * D) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (st + u * D < a.steps) {
+        multiply(st + u * D, u);
+        load(st + (u + AHEAD) * D, u);
+      }
+  }
+  if constexpr (KSPLIT) {
+    if (wave > 0)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sums[((wave - 1) * 16 + r) * 64 + lane] = acc[r];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[r] += sums[(w * 16 + r) * 64 + lane];
+  }
+  const int64_t n = n0 + l31;
+  if (n >= a.n) return;
+  const float b = a.bias ? a.bias[n] : 0.f;
+  T* out = static_cast<T*>(a.out);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int m = 8 * (r >> 2) + 4 * half + (r & 3);
+    if (m < a.m) out[m * a.ldo + n] = (T)(acc[r] + b);
   }
 }
 
@@ -318,8 +570,6 @@ static void mx4_launch(Mx4Args a, hipStream_t s) {
   const unsigned grid = (unsigned)((total + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS);
   hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, S>), dim3(grid), dim3(256), LDS, s, a);
 }
-
-static int64_t mx4_steps(int64_t cols) { return (cols + MX_K - 1) / MX_K; }
 
 }  // namespace bkg
 
@@ -372,23 +622,90 @@ extern "C" int bkg_mx4_dequantize(const void* codes, const void* scales, int64_t
   return check_launch("bkg_mx4_dequantize");
 }
 
+static int mx4_check_product(int64_t m, int64_t n, int64_t cols, const void* b_codes, const void* b_scales, const float* bias,
+                             const void* out, int32_t type, int64_t ldo) {
+  BKG_ARG(type >= 0 && type <= 2 && m >= 0 && n >= 0 && cols > 0 && cols <= (1 << 24) && m < (1ll << 31) && n < (1ll << 31),
+          "bkg_mx4 product: bad sizes or type (1 to 2^24 columns, rows below 2^31)");
+  if (m == 0 || n == 0) return 0;
+  BKG_ARG(b_codes && b_scales && out && ldo >= n, "bkg_mx4 product: null buffer or overlapping rows");
+  BKG_ARG((uintptr_t)b_codes % 16 == 0 && (uintptr_t)b_scales % 4 == 0 && (uintptr_t)out % type_bytes(type) == 0 &&
+              (uintptr_t)bias % 4 == 0,
+          "bkg_mx4 product: misaligned buffer");
+  BKG_ARG((m + 127) / 128 * ((n + 127) / 128) < (1ll << 31) - 64, "bkg_mx4 product: too many tiles for one launch");
+  return 0;
+}
+
+template <typename T, bool PACKED>
+static void mx4_few_launch(const Mx4Args& a, const Mx4X& x, hipStream_t s) {
+  const int64_t tiles = (a.n + 31) / 32;
+  const size_t lds = PACKED ? 0 : (size_t)a.steps * (2048 + 128);
+  // a wave per tile keeps the chip busy from 2048 tiles on; below that, and with panels to share, the waves of a block
+  if (tiles >= 2048 || a.steps < 4)
+    hipLaunchKernelGGL((mx4_few_kernel<T, PACKED, false>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), lds, s, a, x);
+  else
+    hipLaunchKernelGGL((mx4_few_kernel<T, PACKED, true>), dim3((unsigned)tiles), dim3(256), lds, s, a, x);
+}
+
+template <typename T, int STEPS>
+static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
+  a.m_tiles = (int)((a.m + 127) / 128);
+  a.n_tiles = (int)((a.n + 127) / 128);
+  const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(a.n_tiles, 512 / a.m_tiles));     // two blocks per CU
+  a.band = (int)((a.n_tiles + ranges - 1) / ranges);
+  const dim3 grid(xcd_grid((a.n_tiles + a.band - 1) / a.band, a.m_tiles));
+  static const bool set =                                    // (more dynamic LDS than a kernel gets unasked)
+      hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS, false>, hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess &&
+      hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS, true>, hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess;
+  (void)set;
+  if (a.bias) hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS, true>), grid, dim3(256), ms_lds(STEPS), s, a);
+  else hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS, false>), grid, dim3(256), ms_lds(STEPS), s, a);
+}
+
+// rows of x that a product packs within its one launch: at most 32, and few enough values that every block packs them anew
+static bool mx4_packs_itself(int64_t m, int64_t cols) { return m <= 32 && m * mx4_steps(cols) * MX_K <= 8192; }
+
+template <typename T>
+static void mx4_product(const Mx4Args& a, hipStream_t s) {
+  if (a.m <= 32) mx4_few_launch<T, true>(a, Mx4X{}, s);
+  else if (a.steps == 1) mx4_stream_launch<T, 1>(a, s);
+  else if (a.steps == 2) mx4_stream_launch<T, 2>(a, s);
+  // 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128
+  else if ((a.m + 255) / 256 * ((a.n + 255) / 256) >= 192 && a.steps >= 8) mx4_launch<T, 4, 4, 4>(a, s);
+  else mx4_launch<T, 2, 2, 4>(a, s);
+}
+
 extern "C" int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t m, const void* b_codes, const void* b_scales,
                               int64_t n, int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* stream) {
-  BKG_ARG(type >= 0 && type <= 2 && m >= 0 && n >= 0 && cols > 0 && cols <= (1 << 24) && m < (1ll << 31) && n < (1ll << 31),
-          "bkg_mx4_matmul: bad sizes or type (1 to 2^24 columns, rows below 2^31)");
+  if (const int rc = mx4_check_product(m, n, cols, b_codes, b_scales, bias, out, type, ldo)) return rc;
   if (m == 0 || n == 0) return 0;
-  BKG_ARG(a_codes && a_scales && b_codes && b_scales && out && ldo >= n, "bkg_mx4_matmul: null buffer or overlapping rows");
-  BKG_ARG((uintptr_t)a_codes % 16 == 0 && (uintptr_t)b_codes % 16 == 0 && (uintptr_t)a_scales % 4 == 0 &&
-              (uintptr_t)b_scales % 4 == 0 && (uintptr_t)out % type_bytes(type) == 0,
-          "bkg_mx4_matmul: misaligned buffer");
-  BKG_ARG((m + 127) / 128 * ((n + 127) / 128) < (1ll << 31) - 8, "bkg_mx4_matmul: too many tiles for one launch");
-  BKG_ARG(!bias || (uintptr_t)bias % 4 == 0, "bkg_mx4_matmul: misaligned bias");
-  Mx4Args a{(const unsigned char*)a_codes, (const uint32_t*)a_scales, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales,
-            n, (int)mx4_steps(cols), 0, 0, bias, out, ldo, access_bytes(out, 0, ldo * type_bytes(type)) == 16};
-  hipStream_t s = (hipStream_t)stream;
-  // 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128
-  if ((m + 255) / 256 * ((n + 255) / 256) >= 192 && a.steps >= 8) BKG_BY_TYPE(type, (mx4_launch<T, 4, 4, 4>(a, s)));
-  else if (a.steps <= 2) BKG_BY_TYPE(type, (mx4_launch<T, 2, 2, 2>(a, s)));
-  else BKG_BY_TYPE(type, (mx4_launch<T, 2, 2, 4>(a, s)));
+  BKG_ARG(a_codes && a_scales && (uintptr_t)a_codes % 16 == 0 && (uintptr_t)a_scales % 4 == 0, "bkg_mx4_matmul: null or misaligned buffer");
+  const Mx4Args a{(const unsigned char*)a_codes, (const uint32_t*)a_scales, m, (const unsigned char*)b_codes,
+                  (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 8, bias, out, ldo,
+                  access_bytes(out, 0, ldo * type_bytes(type)) == 16};
+  BKG_BY_TYPE(type, mx4_product<T>(a, (hipStream_t)stream));
   return check_launch("bkg_mx4_matmul");
+}
+
+extern "C" int64_t bkg_mx4_linear_workspace_bytes(int64_t m, int64_t cols) {
+  return m <= 0 || cols <= 0 || mx4_packs_itself(m, cols) ? 0 : mx4_steps(cols) * m * 68;
+}
+
+extern "C" int bkg_mx4_linear(const void* x, int32_t x_type, int64_t ldx, int64_t m, const void* b_codes, const void* b_scales,
+                              int64_t n, int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  if (const int rc = mx4_check_product(m, n, cols, b_codes, b_scales, bias, out, type, ldo)) return rc;
+  if (m == 0 || n == 0) return 0;
+  BKG_ARG(x && x_type >= 0 && x_type <= 2 && (uintptr_t)x % type_bytes(x_type) == 0, "bkg_mx4_linear: null or misaligned x");
+  if (!mx4_packs_itself(m, cols)) {
+    BKG_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= bkg_mx4_linear_workspace_bytes(m, cols),
+            "bkg_mx4_linear: workspace below bkg_mx4_linear_workspace_bytes or misaligned");
+    unsigned char* codes = (unsigned char*)workspace;
+    unsigned char* scales = codes + mx4_steps(cols) * m * 64;
+    if (const int rc = bkg_mx4_quantize(x, x_type, ldx, m, cols, codes, scales, stream)) return rc;
+    return bkg_mx4_matmul(codes, scales, m, b_codes, b_scales, n, cols, bias, out, type, ldo, stream);
+  }
+  const Mx4Args a{nullptr, nullptr, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 8,
+                  bias, out, ldo, 0};
+  BKG_BY_TYPE(type, (mx4_few_launch<T, false>(a, Mx4X{x, x_type, ldx, (int)cols}, (hipStream_t)stream)));
+  return check_launch("bkg_mx4_linear");
 }

@@ -284,28 +284,31 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     if not isinstance(table, Mx4Table):
         raise TypeError("mx4_linear: the table must be an Mx4Table (mx4_quantize)")
     n, cols = table.shape
-    if isinstance(x, Mx4Table):
-        lead, xq = (x.shape[0],), x
-        if x.shape[1] != cols:
-            raise ValueError(f"mx4_linear: {x.shape[1]} columns against a table of {cols}")
-        out_dtype = out_dtype or torch.float32
-        _same_device("mx4_linear", x.codes, table.codes, bias)
-    else:
-        if x.dim() == 0 or x.size(-1) != cols:
-            raise ValueError(f"mx4_linear: x {tuple(x.shape)} against a table of {cols} columns")
-        _type_of(x, "mx4_linear")
-        _same_device("mx4_linear", x, table.codes, bias)
-        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-            raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
-        lead = x.shape[:-1]
-        out_dtype = out_dtype or x.dtype
-        xq = mx4_quantize(x.reshape(-1, cols))
-    if out_dtype not in _TYPE:
-        raise TypeError(f"mx4_linear: out_dtype float32, bfloat16 or float16, got {out_dtype}")
     if bias is not None and (bias.shape != (n,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise ValueError(f"mx4_linear: bias must be contiguous fp32 [{n}]")
-    m = xq.shape[0]
-    out = torch.empty(m, n, dtype=out_dtype, device=table.device)
-    L.call("bkg_mx4_matmul", xq.codes.data_ptr(), xq.scales.data_ptr(), m, table.codes.data_ptr(), table.scales.data_ptr(), n,
-           cols, L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.stream())
-    return out.view(*lead, n)
+    packed = isinstance(x, Mx4Table)
+    if (x.shape[-1] if len(x.shape) else -1) != cols:
+        raise ValueError(f"mx4_linear: x {tuple(x.shape)} against a table of {cols} columns")
+    out_dtype = out_dtype or (torch.float32 if packed else x.dtype)
+    if out_dtype not in _TYPE:
+        raise TypeError(f"mx4_linear: out_dtype float32, bfloat16 or float16, got {out_dtype}")
+    if packed:
+        _same_device("mx4_linear", x.codes, table.codes, bias)
+        m = x.shape[0]
+        out = torch.empty(m, n, dtype=out_dtype, device=table.device)
+        L.call("bkg_mx4_matmul", x.codes.data_ptr(), x.scales.data_ptr(), m, table.codes.data_ptr(), table.scales.data_ptr(), n,
+               cols, L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.stream())
+        return out
+    xt = _type_of(x, "mx4_linear")
+    _same_device("mx4_linear", x, table.codes, bias)
+    if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
+        raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
+    lead = x.shape[:-1]
+    x2 = _rows(x if x.dim() == 2 else x.reshape(-1, cols))
+    m = x2.size(0)
+    out = torch.empty(lead + (n,), dtype=out_dtype, device=x.device)
+    ws_bytes = L.lib().bkg_mx4_linear_workspace_bytes(m, cols)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+    L.call("bkg_mx4_linear", x2.data_ptr(), xt, x2.stride(0), m, table.codes.data_ptr(), table.scales.data_ptr(), n, cols,
+           L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
+    return out

@@ -492,7 +492,9 @@ def check_linear(x, w, bias, out_dtype, got=None):
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 130, 256), (3, 17, 33), (16, 300, 128), (17, 64, 129), (33, 129, 200),
                                    (130, 257, 256), (64, 1000, 768), (300, 70, 1000), (257, 513, 384), (5, 5000, 256),
-                                   (129, 128, 2048), (4099, 4100, 1100), (3, 70000, 1025)])
+                                   (129, 128, 2048), (4099, 4100, 1100), (3, 70000, 1025), (33, 5000, 128),
+                                   (700, 3000, 100), (200, 1024, 256), (1000, 2049, 250), (8200, 200, 256), (20, 40, 5000),
+                                   (32, 65600, 300), (1, 1, 8192), (2, 600, 4000)])
 @pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                        (torch.float16, torch.float32), (torch.bfloat16, torch.float16)])
 def test_mx4_linear(m, n, k, dtype, out):
