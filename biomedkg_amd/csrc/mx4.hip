@@ -330,74 +330,84 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
 }
 
 // Narrow inner dimension (one or two panels: an entity table of up to 256 columns), many outputs: the call is the writing of
-// its outputs.  A block keeps its 128 rows of A in registers (32 at two panels) and walks a range of B's 128-row tiles: tile
-// t + 1 travels into the other of two LDS slots while tile t multiplies and its results leave, so loads, products and stores
-// overlap within a block too, and only B moves (the tiled kernel above loads both operands per 128 x 128 outputs and has
-// nothing in flight while a block stores: 95 against ... us for 1021 x 130000 x 256 in bf16).
+// its outputs.  A block keeps its 128 rows of B in registers (32 at two panels) and walks A's 128-row tiles: tile t + 1
+// travels into the other of two LDS slots while tile t multiplies and its results leave, so loads, products and stores
+// overlap within a block too, and only A moves, out of the L2.  All blocks walk the rows of the output from the top, next to
+// each other: what is written at one time is a band of whole rows, not a column of it -- whole DRAM pages, as far as they go
+// (1021 x 130000 x 256 in bf16: 72 us walking B's tiles past A).
 //
 // (Dynamic LDS: reading a static array that LDS-DMAs write makes hipcc wait for every copy in flight.)
 constexpr int MS_PITCH = 64 + 4;                           // floats of a staged result row
 constexpr int ms_lds(int steps) { return 2 * steps * (128 * 64 + 128 * 4) + 4 * 32 * MS_PITCH * 4; }
-template <typename T, int STEPS, bool BIAS>
+template <typename T, int STEPS>
 __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
   constexpr int SLOT = STEPS * (128 * 64 + 128 * 4), PITCH = MS_PITCH;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   unsigned char* const ring = lds;
   float* const stage = reinterpret_cast<float*>(lds + 2 * SLOT);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, half = lane >> 5;
-  const XcdSlot xs = xcd_slot(blockIdx.x, a.m_tiles);      // the row tiles of one range of B share an XCD's L2
-  const int64_t t0 = (int64_t)xs.outer * a.band, t1 = min(t0 + a.band, (int64_t)a.n_tiles);
+  // block -> (a part of A's tiles, a tile of B): the XCDs take contiguous runs of B's tiles
+  const int per_xcd = (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS, local = blockIdx.x / BKG_XCDS % per_xcd;
+  const int64_t bt = (int64_t)(blockIdx.x % BKG_XCDS) * per_xcd + local;
+  if (bt >= a.n_tiles) return;
+  const int64_t t0 = (int64_t)(blockIdx.x / BKG_XCDS / per_xcd) * a.band, t1 = min(t0 + a.band, (int64_t)a.m_tiles);
   if (t0 >= t1) return;
-  const int64_t m0 = (int64_t)xs.inner * 128;
+  const int64_t n0 = bt * 128;
   const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
 
   // copies of a tile: per panel 8 chunks of 16 rows (two a wave) and two of 64 scales (waves 0 and 1: panel 0's, 2 and 3:
   // panel 1's; with one panel waves 2 and 3 copy it a second time: every wave issues the same number)
   constexpr int DMAS = 2 * STEPS + 1;
   auto copy_tile = [&](int64_t tile, int slot) {
-    const int64_t n0 = min(tile, (int64_t)a.n_tiles - 1) * 128;
+    const int64_t m0 = min(tile, (int64_t)a.m_tiles - 1) * 128;
     unsigned char* base = ring + slot * SLOT;
 #pragma unroll
     for (int st = 0; st < STEPS; ++st)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int64_t r = min(n0 + (wave * 2 + j) * 16 + (lane >> 2), a.n - 1);
+        const int64_t r = min(m0 + (wave * 2 + j) * 16 + (lane >> 2), a.m - 1);
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(a.cb + (st * a.n + r) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16),
+            (const __attribute__((address_space(1))) void*)(a.ca + (st * a.m + r) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16),
             (__attribute__((address_space(3))) void*)(base + st * 8192 + (wave * 2 + j) * 1024), 16, 0, 0);
       }
     const int st = STEPS == 2 ? wave >> 1 : 0;
-    const int64_t r = min(n0 + (wave & 1) * 64 + lane, a.n - 1);
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.sb + st * a.n + r),
+    const int64_t r = min(m0 + (wave & 1) * 64 + lane, a.m - 1);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.sa + st * a.m + r),
                                      (__attribute__((address_space(3))) void*)(base + STEPS * 8192 + st * 512 + (wave & 1) * 256), 4, 0, 0);
   };
 
-  mx_i32x4 fa[2][STEPS][2];
-  uint32_t xa[2][STEPS];
+  mx_i32x4 fb[2][STEPS][2];
+  uint32_t xb[2][STEPS];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t r = min(m0 + wm + 32 * i + l31, a.m - 1);
+  for (int j = 0; j < 2; ++j) {
+    const int64_t r = min(n0 + wn + 32 * j + l31, a.n - 1);
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
-      xa[i][st] = a.sa[st * a.m + r] >> (8 * half);
+      xb[j][st] = a.sb[st * a.n + r] >> (8 * half);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        fa[i][st][h] = *reinterpret_cast<const mx_i32x4*>(a.ca + (st * a.m + r) * 64 + (2 * h + half) * 16);
+        fb[j][st][h] = *reinterpret_cast<const mx_i32x4*>(a.cb + (st * a.n + r) * 64 + (2 * h + half) * 16);
     }
   }
+  constexpr int VE = 16 / sizeof(T), LPR = 64 / VE, RPI = 64 / LPR, STORES = 2 * 32 / RPI;
+  const int64_t nw = n0 + wn;
+  const bool cols_full = a.wide && nw + 64 <= a.n;
+  const int col = cols_full ? (lane % LPR) * VE : lane;
+  float bias[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) bias[e] = a.bias ? a.bias[min(nw + (cols_full ? col + e : col), a.n - 1)] : 0.f;
   copy_tile(t0, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int st = 0; st < STEPS; ++st)
-      asm volatile("" : "+v"(fa[i][st][0]), "+v"(fa[i][st][1]), "+v"(xa[i][st]));
+      asm volatile("" : "+v"(fb[i][st][0]), "+v"(fb[i][st][1]), "+v"(xb[i][st]));
+#pragma unroll
+  for (int e = 0; e < VE; ++e) asm volatile("" : "+v"(bias[e]));
 
-  constexpr int VE = 16 / sizeof(T), LPR = 64 / VE, RPI = 64 / LPR, STORES = 2 * 32 / RPI;
   float* mine = stage + wave * 32 * PITCH;
   T* out = static_cast<T*>(a.out);
-  const int64_t mw = m0 + wm;
-  const bool rows_full = a.wide && mw + 64 <= a.m;
   bool stores_known = false;                               // the last tile's STORES are behind the current tile's copies
   int slot = 0;
   for (int64_t t = t0; t < t1; ++t) {
@@ -407,12 +417,8 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();                          // everyone's have, and everyone is done with the other slot
     asm volatile("" ::: "memory");
-    const int64_t nw = t * 128 + wn;
-    const bool wide = rows_full && nw + 64 <= a.n;
-    const int col = wide ? (lane % LPR) * VE : lane;
-    float bias[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) bias[e] = BIAS ? a.bias[min(nw + (wide ? col + e : col), a.n - 1)] : 0.f;
+    const int64_t mw = t * 128 + wm;
+    const bool wide = cols_full && mw + 64 <= a.m;
     copy_tile(t + 1, slot ^ 1);                            // (past the range: valid memory, never read)
     const unsigned char* base = ring + slot * SLOT;
     mx_f32x16 acc[2][2];
@@ -424,22 +430,22 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
-      uint32_t xb[2];
-      mx_i32x4 fb[2][2];
+      uint32_t xa[2];
+      mx_i32x4 fa[2][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        xb[j] = *reinterpret_cast<const uint32_t*>(base + STEPS * 8192 + st * 512 + (wn + 32 * j + l31) * 4) >> (8 * half);
+      for (int i = 0; i < 2; ++i) {
+        xa[i] = *reinterpret_cast<const uint32_t*>(base + STEPS * 8192 + st * 512 + (wm + 32 * i + l31) * 4) >> (8 * half);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          fb[j][h] = *reinterpret_cast<const mx_i32x4*>(base + st * 8192 + (wn + 32 * j + l31) * 64 +
+          fa[i][h] = *reinterpret_cast<const mx_i32x4*>(base + st * 8192 + (wm + 32 * i + l31) * 64 +
                                                         (((2 * h + half) ^ ((l31 >> 1) & 3)) * 16));
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          acc[i][j] = mx_mfma<0>(fa[i][st][0], fb[j][0], acc[i][j], xa[i][st], xb[j]);
-          acc[i][j] = mx_mfma<1>(fa[i][st][1], fb[j][1], acc[i][j], xa[i][st], xb[j]);
+          acc[i][j] = mx_mfma<0>(fa[i][0], fb[j][st][0], acc[i][j], xa[i], xb[j][st]);
+          acc[i][j] = mx_mfma<1>(fa[i][1], fb[j][st][1], acc[i][j], xa[i], xb[j][st]);
         }
     }
 #pragma unroll
@@ -451,6 +457,8 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
       const int64_t mr = mw + 32 * i;
       if (wide) {
         mx_store_rows<T, 64, PITCH, false>(mine, bias, out + mr * a.ldo + nw, a.ldo, 32, lane);
+      } else if (cols_full) {
+        mx_store_rows<T, 64, PITCH, true>(mine, bias, out + mr * a.ldo + nw, a.ldo, a.m - mr, lane);
       } else {
         const int rows_here = (int)min((int64_t)32, a.m - mr);
         for (int row = 0; row < rows_here; ++row)
@@ -650,15 +658,14 @@ template <typename T, int STEPS>
 static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
   a.m_tiles = (int)((a.m + 127) / 128);
   a.n_tiles = (int)((a.n + 127) / 128);
-  const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(a.n_tiles, 512 / a.m_tiles));     // two blocks per CU
-  a.band = (int)((a.n_tiles + ranges - 1) / ranges);
-  const dim3 grid(xcd_grid((a.n_tiles + a.band - 1) / a.band, a.m_tiles));
-  static const bool set =                                    // (more dynamic LDS than a kernel gets unasked)
-      hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS, false>, hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess &&
-      hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS, true>, hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess;
+  // parts of A's tiles: so many that two blocks per CU are there
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(a.m_tiles, 512 / a.n_tiles));
+  a.band = (int)((a.m_tiles + parts - 1) / parts);
+  const int64_t blocks = (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS * ((a.m_tiles + a.band - 1) / a.band);
+  static const bool set = hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS>,   // (more than a kernel gets unasked)
+                                              hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess;
   (void)set;
-  if (a.bias) hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS, true>), grid, dim3(256), ms_lds(STEPS), s, a);
-  else hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS, false>), grid, dim3(256), ms_lds(STEPS), s, a);
+  hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS>), dim3((unsigned)blocks), dim3(256), ms_lds(STEPS), s, a);
 }
 
 // rows of x that a product packs within its one launch: at most 32, and few enough values that every block packs them anew
