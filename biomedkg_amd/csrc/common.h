@@ -46,10 +46,21 @@ static inline int check_launch(const char* what) {
 
 // Stable ascending sort of an embedding lookup's ids with their positions (graph.hip): key = the id, or n_rows where the id
 // lies outside [0, n_rows) or equals pad (those entries come last).  sorted_keys / perm [n]; scratch: 2 n words + workspace
-// of embed_sort_workspace_bytes(n).
+// of embed_sort_workspace_bytes(n).  Up to EMBED_SMALL_SORT ids it is one launch, whose idle CUs also clear `zero`.
+constexpr int64_t EMBED_SMALL_SORT = 8192;
+struct EmbedZero {
+  uint4* p; int64_t n16;                          // whole 16-byte words
+  unsigned char* tail; int n_tail;                // < 16 bytes behind them
+  uint32_t *pad_keys, *pad_perm; int n_pad;       // the words behind the sorted entries (null: none; <= 256 of them)
+};
+__device__ __forceinline__ void embed_zero(int64_t i, const EmbedZero& z) {
+  if (z.pad_keys && i < z.n_pad) { z.pad_keys[i] = 0xFFFFFFFFu; z.pad_perm[i] = 0u; }
+  if (i < z.n16) z.p[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (i < z.n_tail) z.tail[i] = 0;
+}
 int64_t embed_sort_workspace_bytes(int64_t n);
 int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, uint32_t* scratch, uint32_t* sorted_keys,
-               uint32_t* perm, void* workspace, int64_t workspace_bytes, hipStream_t s);
+               uint32_t* perm, void* workspace, int64_t workspace_bytes, const EmbedZero& zero, hipStream_t s);
 
 static inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 

@@ -8,27 +8,29 @@
 //
 // The gradient needs no atomics: the ids are sorted (stable, carrying positions), and every run of equal ids is summed in
 // position order.  Runs are very uneven in a graph -- most entities occur a few times, a hub in a percent of all edges -- so
-// the work is cut by ENTRIES, not by rows: a lane group takes the runs that start in its chunk of sorted entries.  A run
-// longer than EG_LONG entries is left out there and summed by windows of EG_LONG entries (one lane group each) whose fp32
-// partial rows a last launch adds in order.
+// the work is cut by ENTRIES, not by rows: a lane group takes a chunk of the sorted entries, writes the rows of the runs that
+// lie in it and leaves an fp32 partial row for a run that crosses either border; a last launch adds those in order.  (Giving
+// a run to the group it starts in, up to a length, balances worse: 303 against ... us for a million skewed ids.)
 #include "rowtypes.h"
 
 namespace bkg {
 
-constexpr int EG_LONG = 64;
-constexpr int EG_PAD = EG_LONG + 2 * 8;             // words behind the sorted entries that steps of 8 and looks ahead reach
+constexpr int EG_U = 8;                             // entries per step: their rows are in flight together
+constexpr int EG_PAD = 4 * EG_U;                    // words behind the sorted entries that the steps ahead reach
 constexpr int64_t EMBED_MAX_D = 1 << 20;            // (column tiles are the grid's y extent)
 
 __device__ __forceinline__ int64_t embed_id(const void* __restrict__ ids, int ids_i32, int64_t i) {
   return ids_i32 ? (int64_t)static_cast<const int32_t*>(ids)[i] : static_cast<const int64_t*>(ids)[i];
 }
 
+constexpr int EMBED_UNROLL = 4;
+
 // A lane group of 2^lpr_log2 lanes copies a row's VEC-wide columns of tile blockIdx.y; UNROLL rows in flight per group.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ w, int64_t ldw, int64_t n_rows, int d,
                                                          const void* __restrict__ ids, int ids_i32, int64_t n, float scale,
                                                          T* __restrict__ out, int64_t ldo, int lpr_log2) {
-  constexpr int UNROLL = 4;
+  constexpr int UNROLL = EMBED_UNROLL;
   const int lig = threadIdx.x & ((1 << lpr_log2) - 1), groups = 256 >> lpr_log2;
   const int c = (((int)blockIdx.y << lpr_log2) + lig) * VEC;
   if (c >= d) return;
@@ -58,24 +60,12 @@ struct EmbedGradArgs {
   const uint32_t* keys; const uint32_t* perm;      // [n] sorted (key n_rows = no gradient), then EG_PAD all-ones words
   int64_t n, n_rows;
   float scale;
-  int d, lpr_log2, chunk;
-  int64_t n_chunks;                                // lane groups over entries; the rest of the grid are windows
-  int64_t n_windows;
-  float* part;                                     // [2 n_windows][d] partial rows of long runs (2 j: the run over window j's
-};                                                 // first entry, 2 j + 1: the run that starts inside it and leaves it)
+  int d, lpr_log2;
+  int chunk;                                       // entries per lane group, a multiple of EG_U
+  int64_t n_chunks;
+  float* part;                                     // [2 n_chunks][d] partial rows: 2 j: the run that comes into chunk j,
+};                                                 // 2 j + 1: the run that starts in it and goes on behind it
 
-// Is the run of key k around entry p (keys[p] == k) longer than EG_LONG entries?  It is iff the entries of k within
-// EG_LONG of p on either side are more than EG_LONG; the ends by binary search.
-__device__ __forceinline__ bool run_is_long(const uint32_t* __restrict__ keys, int64_t n, int64_t p, uint32_t k) {
-  int64_t lo = p - EG_LONG < 0 ? 0 : p - EG_LONG, hi = p;        // first entry of k in [p - EG_LONG, p]
-  while (lo < hi) { const int64_t m = (lo + hi) >> 1; if (keys[m] < k) lo = m + 1; else hi = m; }
-  const int64_t beg = lo;
-  lo = p + 1; hi = p + EG_LONG + 1 > n ? n : p + EG_LONG + 1;    // first entry past k in (p, p + EG_LONG]
-  while (lo < hi) { const int64_t m = (lo + hi) >> 1; if (keys[m] <= k) lo = m + 1; else hi = m; }
-  return lo - beg > EG_LONG;
-}
-
-constexpr int EG_U = 8;                            // entries per step: their rows are in flight together
 struct EgWords { uint32_t w[EG_U]; };
 __device__ __forceinline__ EgWords eg_words(const uint32_t* __restrict__ p) {      // (32-byte aligned; reads into the pad)
   EgWords o;
@@ -84,6 +74,10 @@ __device__ __forceinline__ EgWords eg_words(const uint32_t* __restrict__ p) {   
   o.w[4] = b.x; o.w[5] = b.y; o.w[6] = b.z; o.w[7] = b.w;
   return o;
 }
+template <typename T, int VEC> struct EgStep {
+  EgWords key;
+  Pack<T, VEC> row[EG_U];
+};
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const EmbedGradArgs a, const T* __restrict__ g, int64_t ldg,
@@ -91,134 +85,163 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const EmbedGradArgs a, 
   const int lig = threadIdx.x & ((1 << a.lpr_log2) - 1), groups = 256 >> a.lpr_log2;
   const int c = (((int)blockIdx.y << a.lpr_log2) + lig) * VEC;
   if (c >= a.d) return;
-  const int64_t group = (int64_t)blockIdx.x * groups + (threadIdx.x >> a.lpr_log2);
+  const int64_t j = (int64_t)blockIdx.x * groups + (threadIdx.x >> a.lpr_log2);
+  if (j >= a.n_chunks) return;
+  const int64_t beg = j * a.chunk, last = beg + a.chunk < a.n ? beg + a.chunk : a.n;
   const T* gc = g + c;
+  const uint32_t none = (uint32_t)a.n_rows;
+  const uint32_t before = beg > 0 ? a.keys[beg - 1] : 0xFFFFFFFFu, behind = a.keys[last];   // (all ones behind the last entry)
   float acc[VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  if (group < a.n_chunks) {                                     // ---- the runs that start in these entries
-    const int64_t beg = group * a.chunk, last = beg + a.chunk < a.n ? beg + a.chunk : a.n;
-    uint32_t cur = beg > 0 ? a.keys[beg - 1] : 0xFFFFFFFFu;
-    bool mine = false;                                          // is `cur` a run of this group (and not a long one)?
-    EgWords k = eg_words(a.keys + beg), pm = eg_words(a.perm + beg), kl = eg_words(a.keys + beg + EG_LONG);
-    for (int64_t e = beg; e < last || mine; e += EG_U) {
-      bool live[EG_U];
-      Pack<T, VEC> r[EG_U];
-      uint32_t run = cur;
-      bool on = mine;
+  for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
+  uint32_t cur = before;                           // the run being added; the one that comes in goes to a partial row
+  bool came_in = true;
+  // the sum of run `cur` leaves: a row, or a partial one (slot: -1 none)
+  auto leave = [&](int64_t slot) {
+    if (cur < none) {
+      if (slot < 0) {
+        Pack<T, VEC> o;
 #pragma unroll
-      for (int u = 0; u < EG_U; ++u) {
-        if (k.w[u] != run) {
-          run = k.w[u];
-          on = e + u < last && run < (uint32_t)a.n_rows && kl.w[u] != run;
-        }
-        live[u] = on;
-      }
+        for (int v = 0; v < VEC; ++v) o.v[v] = (T)(acc[v] * a.scale);
+        *reinterpret_cast<Pack<T, VEC>*>(dw + (int64_t)cur * ldw + c) = o;
+      } else {
+        Pack<float, VEC> o;
 #pragma unroll
-      for (int u = 0; u < EG_U; ++u)
-        if (live[u]) r[u] = *reinterpret_cast<const Pack<T, VEC>*>(gc + (int64_t)pm.w[u] * ldg);
-      const EgWords kn = k;
-      const int64_t en = e + EG_U < a.n ? e + EG_U : e;         // (a group that stops here reads its own entries again)
-      k = eg_words(a.keys + en); pm = eg_words(a.perm + en); kl = eg_words(a.keys + en + EG_LONG);
-      if (en == e)
-#pragma unroll
-        for (int u = 0; u < EG_U; ++u) k.w[u] = 0xFFFFFFFFu;
-#pragma unroll
-      for (int u = 0; u < EG_U; ++u) {
-        if (kn.w[u] != cur) {
-          if (mine) {
-            Pack<T, VEC> o;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) { o.v[j] = (T)(acc[j] * a.scale); acc[j] = 0.f; }
-            *reinterpret_cast<Pack<T, VEC>*>(dw + (int64_t)cur * ldw + c) = o;
-          }
-          cur = kn.w[u];
-          mine = live[u];
-        }
-        if (live[u])
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[j] += widen(r[u].v[j]);
+        for (int v = 0; v < VEC; ++v) o.v[v] = acc[v];
+        *reinterpret_cast<Pack<float, VEC>*>(a.part + slot * a.d + c) = o;
       }
     }
-    return;
-  }
-  // ---- a window of EG_LONG entries: the parts of long runs in it
-  const int64_t j = group - a.n_chunks;
-  if (j >= a.n_windows) return;
-  const int64_t p = j * EG_LONG, q = p + EG_LONG < a.n ? p + EG_LONG : a.n;
-  const uint32_t k0 = a.keys[p], k1 = a.keys[q - 1];
-  // (candidates by one look each: a run longer than EG_LONG that covers the window's first entry either covers the whole
-  // window or reaches back past it)
-  const bool head = k0 < (uint32_t)a.n_rows && (k1 == k0 || (p > 0 && a.keys[p - 1] == k0)) && run_is_long(a.keys, a.n, p, k0);
-  const bool tail = k1 != k0 && q < a.n && a.keys[q] == k1 && k1 < (uint32_t)a.n_rows && run_is_long(a.keys, a.n, q - 1, k1);
-  for (int which = 0; which < 2; ++which) {
-    if (!(which ? tail : head)) continue;
-    const uint32_t key = which ? k1 : k0;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) acc[v] = 0.f;
-    EgWords k = eg_words(a.keys + p), pm = eg_words(a.perm + p);
-    for (int64_t e = p; e < q; e += EG_U) {
-      Pack<T, VEC> r[EG_U];
+  };
+  // two steps at work: step s + 1's rows are loaded while step s's are added, and the words of step s + 2 behind them
+  EgWords k, pm;
+  auto words = [&](int64_t e) { k = eg_words(a.keys + e); pm = eg_words(a.perm + e); };      // (e <= n + EG_U: into the pad)
+  auto issue = [&](int64_t e, EgStep<T, VEC>& s) {
+    s.key = k;
 #pragma unroll
-      for (int u = 0; u < EG_U; ++u)
-        if (k.w[u] == key) r[u] = *reinterpret_cast<const Pack<T, VEC>*>(gc + (int64_t)pm.w[u] * ldg);
-      const EgWords kn = k;
-      k = eg_words(a.keys + e + EG_U); pm = eg_words(a.perm + e + EG_U);
+    for (int u = 0; u < EG_U; ++u)
+      if (e + u < last && k.w[u] < none) s.row[u] = *reinterpret_cast<const Pack<T, VEC>*>(gc + (int64_t)pm.w[u] * ldg);
+  };
+  auto consume = [&](int64_t e, const EgStep<T, VEC>& s) {
 #pragma unroll
-      for (int u = 0; u < EG_U; ++u)
-        if (kn.w[u] == key)
+    for (int u = 0; u < EG_U; ++u) {
+      if (e + u >= last) break;
+      if (s.key.w[u] != cur) {
+        if (e + u > beg) leave(came_in ? 2 * j : -1);          // (nothing came in: `before` is not this chunk's)
+        cur = s.key.w[u];
+        came_in = false;
+      }
+      if (s.key.w[u] < none)
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) acc[v] += widen(r[u].v[v]);
+        for (int v = 0; v < VEC; ++v) acc[v] += widen(s.row[u].v[v]);
     }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) a.part[(2 * j + which) * a.d + c + v] = acc[v];
+  };
+  EgStep<T, VEC> s0, s1;
+  words(beg);
+  issue(beg, s0);
+  words(beg + EG_U);
+  for (int64_t e = beg; e < last; e += 2 * EG_U) {
+    issue(e + EG_U, s1);
+    words(e + 2 * EG_U < a.n ? e + 2 * EG_U : beg);
+    consume(e, s0);
+    issue(e + 2 * EG_U, s0);
+    words(e + 3 * EG_U < a.n ? e + 3 * EG_U : beg);
+    consume(e + EG_U, s1);
   }
+  leave(came_in ? 2 * j : behind == cur ? 2 * j + 1 : -1);
 }
 
-// Window j in which a long run starts adds that run's partial rows and writes the row: four waves take a quarter of the
-// windows each, in order, and their sums are added in order.
-template <typename T>
-__global__ __launch_bounds__(256) void embed_grad_long_kernel(const EmbedGradArgs a, T* __restrict__ dw, int64_t ldw) {
-  __shared__ float quarter[4][64];
-  const int64_t j = blockIdx.x, p = j * EG_LONG, q = p + EG_LONG < a.n ? p + EG_LONG : a.n;
-  const uint32_t k0 = a.keys[p], k1 = a.keys[q - 1];
-  uint32_t k;
-  int64_t slot;
-  if (k0 < (uint32_t)a.n_rows && k1 == k0 && (p == 0 || a.keys[p - 1] != k0) && run_is_long(a.keys, a.n, p, k0)) {
-    k = k0; slot = 2 * j;
-  } else if (k1 != k0 && q < a.n && a.keys[q] == k1 && k1 < (uint32_t)a.n_rows && run_is_long(a.keys, a.n, q - 1, k1)) {
-    k = k1; slot = 2 * j + 1;
-  } else {
-    return;
-  }
-  int64_t lo = q, hi = a.n;                                     // the run's end: the first entry past k
-  while (lo < hi) { const int64_t m = (lo + hi) >> 1; if (a.keys[m] <= k) lo = m + 1; else hi = m; }
-  const int64_t count = (lo - 1) / EG_LONG - j;                 // windows behind this one that it reaches
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t w0 = j + 1 + count * wave / 4, w1 = j + 1 + count * (wave + 1) / 4;
-  for (int c0 = 0; c0 < a.d; c0 += 64) {
-    const int c = c0 + lane;
-    float s = 0.f;
-    if (c < a.d) {
-      if (wave == 0) s = a.part[slot * a.d + c];
+// The rows of runs that cross borders of chunks: the chunk a run starts in adds the run's partial rows.  A block looks after
+// EG_FINISH chunks.  A run over few chunks is a wave's work, the waves side by side; for a longer one the block's eight waves
+// take an eighth of its chunks each, in order, and their sums are added in order.  Columns: 4 per lane (d a multiple of 4) or 1.
+constexpr int EG_FINISH = 32, EG_FEW = 8;
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<float, VEC> eg_add_parts(const EmbedGradArgs& a, int64_t w0, int64_t w1, int c, Pack<float, VEC> s) {
 #pragma unroll 8
-      for (int64_t w = w0; w < w1; ++w) s += a.part[2 * w * a.d + c];
+  for (int64_t w = w0; w < w1; ++w) {
+    const Pack<float, VEC> r = *reinterpret_cast<const Pack<float, VEC>*>(a.part + 2 * w * a.d + c);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s.v[v] += r.v[v];
+  }
+  return s;
+}
+template <typename T, int VEC>
+__global__ __launch_bounds__(512) void embed_grad_finish_kernel(const EmbedGradArgs a, T* __restrict__ dw, int64_t ldw) {
+  __shared__ float eighth[8][64][VEC];
+  __shared__ int n_few, n_many;
+  __shared__ int few[EG_FINISH], few_count[EG_FINISH], many[EG_FINISH];
+  if (threadIdx.x == 0) n_few = n_many = 0;
+  __syncthreads();
+  const int64_t j0 = (int64_t)blockIdx.x * EG_FINISH;
+  if (threadIdx.x < EG_FINISH) {
+    const int64_t j = j0 + threadIdx.x, beg = j * a.chunk, q = beg + a.chunk;
+    if (q < a.n) {
+      const uint32_t k1 = a.keys[q - 1];
+      if (k1 < (uint32_t)a.n_rows && a.keys[q] == k1 && !(a.keys[beg] == k1 && beg > 0 && a.keys[beg - 1] == k1)) {
+        int count = 1;                                          // chunks behind this one that the run reaches, as far as EG_FEW
+        while (count < EG_FEW && q + (int64_t)count * a.chunk < a.n && a.keys[q + (int64_t)count * a.chunk] == k1) ++count;
+        if (count < EG_FEW) {
+          const int at = atomicAdd(&n_few, 1);                  // (their order does not matter: each writes a row of its own)
+          few[at] = threadIdx.x; few_count[at] = count;
+        } else {
+          many[atomicAdd(&n_many, 1)] = threadIdx.x;
+        }
+      }
     }
-    __syncthreads();
-    quarter[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && c < a.d)
-      dw[(int64_t)k * ldw + c] = (T)((((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane]) * a.scale);
+  }
+  __syncthreads();
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, total_few = n_few, total_many = n_many;
+  for (int i = wave; i < total_few; i += 8) {
+    const int64_t j = j0 + few[i];
+    const uint32_t k = a.keys[(j + 1) * a.chunk - 1];
+    for (int c = lane * VEC; c < a.d; c += 64 * VEC) {
+      const Pack<float, VEC> s = eg_add_parts<T, VEC>(a, j + 1, j + 1 + few_count[i], c,
+                                                      *reinterpret_cast<const Pack<float, VEC>*>(a.part + (2 * j + 1) * a.d + c));
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) dw[(int64_t)k * ldw + c + v] = (T)(s.v[v] * a.scale);
+    }
+  }
+  for (int i = 0; i < total_many; ++i) {
+    const int64_t j = j0 + many[i], q = (j + 1) * a.chunk;
+    const uint32_t k = a.keys[q - 1];
+    int64_t last = q, span = a.n - q;                           // the run's last entry lies in [last, last + span): 512 looks a round
+    while (span > 1) {
+      const int64_t step = (span + 511) / 512, at = last + threadIdx.x * step;
+      last += (__syncthreads_count(at < last + span && a.keys[at < a.n ? at : a.n - 1] == k) - 1) * step;
+      span = step;
+      if (last + span > a.n) span = a.n - last;
+    }
+    const int64_t count = last / a.chunk - j;                   // chunks behind this one that it reaches
+    const int64_t w0 = j + 1 + count * wave / 8, w1 = j + 1 + count * (wave + 1) / 8;
+    for (int c0 = 0; c0 < a.d; c0 += 64 * VEC) {
+      const int c = c0 + lane * VEC;
+      Pack<float, VEC> s;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) s.v[v] = 0.f;
+      if (c < a.d) {
+        if (wave == 0) s = *reinterpret_cast<const Pack<float, VEC>*>(a.part + (2 * j + 1) * a.d + c);
+        s = eg_add_parts<T, VEC>(a, w0, w1, c, s);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) eighth[wave][lane][v] = s.v[v];
+      __syncthreads();
+      if (wave == 0 && c < a.d) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          float sum = eighth[0][lane][v];
+#pragma unroll
+          for (int x = 1; x < 8; ++x) sum += eighth[x][lane][v];
+          dw[(int64_t)k * ldw + c + v] = (T)(sum * a.scale);
+        }
+      }
+    }
   }
 }
 
-__global__ __launch_bounds__(256) void embed_zero_kernel(uint4* __restrict__ p, int64_t n16, unsigned char* __restrict__ tail,
-                                                         int n_tail, uint32_t* __restrict__ pad_keys,
-                                                         uint32_t* __restrict__ pad_perm) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (pad_keys && i < EG_PAD) { pad_keys[i] = 0xFFFFFFFFu; pad_perm[i] = 0u; }
-  if (i < n16) p[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (i < n_tail) tail[i] = 0;
+__global__ __launch_bounds__(256) void embed_zero_kernel(const EmbedZero z) {
+  embed_zero((int64_t)blockIdx.x * 256 + threadIdx.x, z);
 }
 
 // lanes of a row group: the smallest power of two that covers a row's accesses, at most a wave
@@ -232,7 +255,7 @@ template <typename T, int VEC>
 static void embed_rows_launch(const void* w, int64_t ldw, int64_t n_rows, int64_t d, const void* ids, int ids_i32, int64_t n,
                               float scale, void* out, int64_t ldo, hipStream_t s) {
   const int lpr = lanes_log2(d, VEC);
-  const int64_t per_block = (256 >> lpr) * 4;
+  const int64_t per_block = (256 >> lpr) * EMBED_UNROLL;
   const dim3 grid((unsigned)((n + per_block - 1) / per_block), (unsigned)ceil_div(d, (int64_t)VEC << lpr));
   hipLaunchKernelGGL((embed_rows_kernel<T, VEC>), grid, dim3(256), 0, s, (const T*)w, ldw, n_rows, (int)d, ids, ids_i32, n, scale,
                      (T*)out, ldo, lpr);
@@ -242,15 +265,13 @@ template <typename T, int VEC>
 static void embed_grad_launch(EmbedGradArgs a, const void* g, int64_t ldg, void* dw, int64_t ldw, hipStream_t s) {
   a.lpr_log2 = lanes_log2(a.d, VEC);
   const int groups = 256 >> a.lpr_log2, tiles = ceil_div(a.d, (int64_t)VEC << a.lpr_log2);
-  // entries per group: 64 where that still gives every CU a few thousand lanes of work, down to 4 for short id lists
-  a.chunk = 64;
-  while (a.chunk > 4 && (a.n / a.chunk) * tiles < 8192) a.chunk >>= 1;
-  a.n_chunks = (a.n + a.chunk - 1) / a.chunk;
-  const int64_t all = a.n_chunks + a.n_windows;
-  hipLaunchKernelGGL((embed_grad_kernel<T, VEC>), dim3((unsigned)((all + groups - 1) / groups), tiles), dim3(256), 0, s, a,
+  hipLaunchKernelGGL((embed_grad_kernel<T, VEC>), dim3((unsigned)((a.n_chunks + groups - 1) / groups), tiles), dim3(256), 0, s, a,
                      (const T*)g, ldg, (T*)dw, ldw);
-  if (a.n_windows)
-    hipLaunchKernelGGL((embed_grad_long_kernel<T>), dim3((unsigned)a.n_windows), dim3(256), 0, s, a, (T*)dw, ldw);
+  if (a.n_chunks > 1) {
+    const dim3 grid((unsigned)ceil_div(a.n_chunks, EG_FINISH));
+    if (a.d % 4 == 0) hipLaunchKernelGGL((embed_grad_finish_kernel<T, 4>), grid, dim3(512), 0, s, a, (T*)dw, ldw);
+    else hipLaunchKernelGGL((embed_grad_finish_kernel<T, 1>), grid, dim3(512), 0, s, a, (T*)dw, ldw);
+  }
 }
 
 // FN<T, VEC>(args) for the type and the access width
@@ -273,7 +294,14 @@ static void embed_grad_launch(EmbedGradArgs a, const void* g, int64_t ldg, void*
     }                                                                             \
   } while (0)
 
-static int64_t n_windows_of(int64_t n) { return n > EG_LONG ? (n + EG_LONG - 1) / EG_LONG : 0; }
+// Entries per lane group: 64 from a quarter of a million entries on (16 and less there: more partial rows than rows); fewer
+// where the list is short, so that there are groups for the chip.
+static int embed_chunk(int64_t n) {
+  int chunk = 64;
+  while (chunk > EG_U && n / chunk < 4096) chunk >>= 1;
+  return chunk;
+}
+static int64_t embed_chunks(int64_t n) { return (n + embed_chunk(n) - 1) / embed_chunk(n); }
 static int64_t round256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 
 }  // namespace bkg
@@ -297,7 +325,7 @@ extern "C" int bkg_embed_rows(const void* w, int32_t type, int64_t ldw, int64_t 
 
 extern "C" int64_t bkg_embed_grad_workspace_bytes(int64_t n, int64_t d) {
   if (n <= 0 || d <= 0) return 0;
-  return 2 * round256(4 * (n + EG_PAD)) + 2 * round256(4 * n) + round256(8 * n_windows_of(n) * d) + embed_sort_workspace_bytes(n) + 256;
+  return 2 * round256(4 * (n + EG_PAD)) + 2 * round256(4 * n) + round256(8 * embed_chunks(n) * d) + embed_sort_workspace_bytes(n) + 256;
 }
 
 extern "C" int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t d, const void* ids, int32_t ids_i32, int64_t n,
@@ -319,16 +347,20 @@ extern "C" int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t 
     keys = (uint32_t*)ws; ws += round256(4 * (n + EG_PAD));
     perm = (uint32_t*)ws; ws += round256(4 * (n + EG_PAD));
   }
-  hipLaunchKernelGGL(embed_zero_kernel, dim3((unsigned)((n16 + 256) / 256)), dim3(256), 0, s, (uint4*)dw, n16,
-                     (unsigned char*)dw + n16 * 16, (int)(total - n16 * 16), n ? keys + n : nullptr, n ? perm + n : nullptr);
-  if (n == 0) return check_launch("bkg_embed_grad");
+  const EmbedZero z{(uint4*)dw, n16, (unsigned char*)dw + n16 * 16, (int)(total - n16 * 16), n ? keys + n : nullptr,
+                    n ? perm + n : nullptr, EG_PAD};
+  if (n == 0 || n > EMBED_SMALL_SORT) {
+    hipLaunchKernelGGL(embed_zero_kernel, dim3((unsigned)((n16 + 256) / 256)), dim3(256), 0, s, z);
+    if (n == 0) return check_launch("bkg_embed_grad");
+  }
   BKG_ARG(g && ids, "bkg_embed_grad: null buffer");
   uint32_t* scratch = (uint32_t*)ws; ws += 2 * round256(4 * n);
   EmbedGradArgs a{};
   a.keys = keys; a.perm = perm; a.n = n; a.n_rows = n_rows; a.scale = scale; a.d = (int)d;
-  a.n_windows = n_windows_of(n);
-  a.part = (float*)ws; ws += round256(8 * a.n_windows * d);
-  const int rc = embed_sort(ids, ids_i32, n, n_rows, pad, scratch, keys, perm, ws, embed_sort_workspace_bytes(n), s);
+  a.chunk = embed_chunk(n);
+  a.n_chunks = embed_chunks(n);
+  a.part = (float*)ws; ws += round256(8 * a.n_chunks * d);
+  const int rc = embed_sort(ids, ids_i32, n, n_rows, pad, scratch, keys, perm, ws, embed_sort_workspace_bytes(n), z, s);
   if (rc) return rc;
   int bytes = access_bytes(g, d * e, ldg * e);
   const int ob = access_bytes(dw, d * e, d * e);
