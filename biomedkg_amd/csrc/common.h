@@ -44,10 +44,7 @@ static inline int check_launch(const char* what) {
     }                                                                                            \
   } while (0)
 
-// Stable ascending sort of an embedding lookup's ids with their positions (graph.hip): key = the id, or n_rows where the id
-// lies outside [0, n_rows) or equals pad (those entries come last).  sorted_keys / perm [n]; scratch: 2 n words + workspace
-// of embed_sort_workspace_bytes(n).  Up to EMBED_SMALL_SORT ids it is one launch, whose idle CUs also clear `zero`.
-constexpr int64_t EMBED_SMALL_SORT = 8192;
+// Memory an embedding gradient clears beside its sort.
 struct EmbedZero {
   uint4* p; int64_t n16;                          // whole 16-byte words
   unsigned char* tail; int n_tail;                // < 16 bytes behind them
@@ -58,9 +55,16 @@ __device__ __forceinline__ void embed_zero(int64_t i, const EmbedZero& z) {
   if (i < z.n16) z.p[i] = make_uint4(0u, 0u, 0u, 0u);
   if (i < z.n_tail) z.tail[i] = 0;
 }
-int64_t embed_sort_workspace_bytes(int64_t n);
-int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, uint32_t* scratch, uint32_t* sorted_keys,
-               uint32_t* perm, void* workspace, int64_t workspace_bytes, const EmbedZero& zero, hipStream_t s);
+// The sort key of an embedding lookup's id: the id, or n_rows for an entry whose gradient goes nowhere (those come last).
+__device__ __forceinline__ uint32_t embed_key(const void* __restrict__ ids, int ids_i32, int64_t i, int64_t n_rows, int64_t pad) {
+  const int64_t v = ids_i32 ? (int64_t)static_cast<const int32_t*>(ids)[i] : static_cast<const int64_t*>(ids)[i];
+  return (v < 0 || v >= n_rows || v == pad) ? (uint32_t)n_rows : (uint32_t)v;
+}
+// Stable ascending sort of up to EMBED_SMALL_SORT such keys with their positions, in one launch whose other blocks clear
+// `zero` (graph.hip).
+constexpr int64_t EMBED_SMALL_SORT = 8192;
+int embed_small_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, int bits, uint32_t* sorted_keys,
+                     uint32_t* perm, const EmbedZero& zero, hipStream_t s);
 
 static inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 

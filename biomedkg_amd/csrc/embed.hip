@@ -244,6 +244,181 @@ __global__ __launch_bounds__(256) void embed_zero_kernel(const EmbedZero z) {
   embed_zero((int64_t)blockIdx.x * 256 + threadIdx.x, z);
 }
 
+// ---- the sort of longer id lists: stable radix passes over ES_BITS-bit digits, (key, position) pairs.  A block counts its
+// ES_TILE entries' digits (the first pass makes the keys from the ids); a block per digit turns the counts into offsets; the
+// third launch ranks the tile's entries -- its waves take 64 neighbouring entries at a time, lanes with equal digits find
+// each other by ballots, a counter per wave and digit holds what came before -- and writes them where they belong.
+// A million ids below 130001 in two passes: ... us, against 75 us for the graph structures' device sort (and its fills).
+constexpr int ES_BITS = 9, ES_DIGITS = 1 << ES_BITS, ES_THREADS = 1024, ES_WAVES = ES_THREADS / 64, ES_ITEMS = 4;
+constexpr int ES_TILE = ES_THREADS * ES_ITEMS;
+
+struct EmbedSort {
+  const void* ids; int ids_i32; int64_t n_rows, pad;   // first pass (ids not null): keys from the ids, positions 0 .. n - 1
+  const uint32_t *key_in, *val_in;
+  uint32_t *key_out, *val_out;
+  int64_t n;
+  int n_blocks, shift;
+  uint32_t* counts;                                    // [ES_DIGITS][n_blocks]
+  uint32_t* totals;                                    // [ES_DIGITS]
+};
+__device__ __forceinline__ uint32_t es_key(const EmbedSort& a, int64_t i) {
+  return a.ids ? embed_key(a.ids, a.ids_i32, i, a.n_rows, a.pad) : a.key_in[i];
+}
+
+// (the blocks behind the sort's clear memory)
+__global__ __launch_bounds__(ES_THREADS) void embed_count_kernel(const EmbedSort a, const EmbedZero z) {
+  __shared__ uint32_t count[ES_DIGITS];
+  if ((int)blockIdx.x >= a.n_blocks) {
+    embed_zero((int64_t)(blockIdx.x - a.n_blocks) * ES_THREADS + threadIdx.x, z);
+    return;
+  }
+  for (int d = threadIdx.x; d < ES_DIGITS; d += ES_THREADS) count[d] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * ES_TILE;
+  uint32_t k[ES_ITEMS];
+#pragma unroll
+  for (int r = 0; r < ES_ITEMS; ++r) {
+    const int64_t i = i0 + r * ES_THREADS + threadIdx.x;
+    k[r] = i < a.n ? es_key(a, i) : 0u;
+  }
+#pragma unroll
+  for (int r = 0; r < ES_ITEMS; ++r)
+    if (i0 + r * ES_THREADS + threadIdx.x < a.n) atomicAdd(&count[(k[r] >> a.shift) & (ES_DIGITS - 1)], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < ES_DIGITS; d += ES_THREADS) a.counts[(int64_t)d * a.n_blocks + blockIdx.x] = count[d];
+}
+
+// block d: the counts of digit d become their exclusive prefix sums over the blocks; totals[d] their sum
+__global__ __launch_bounds__(256) void embed_offsets_kernel(uint32_t* __restrict__ counts, int n_blocks, uint32_t* __restrict__ totals) {
+  __shared__ uint32_t wave_sums[4];
+  uint32_t* row = counts + (int64_t)blockIdx.x * n_blocks;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t carry = 0;
+  for (int b0 = 0; b0 < n_blocks; b0 += 256) {
+    const int b = b0 + threadIdx.x;
+    const uint32_t v = b < n_blocks ? row[b] : 0u;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = __shfl_up((int)s, o, 64);
+      if (lane >= o) s += u;
+    }
+    if (lane == 63) wave_sums[wave] = s;
+    __syncthreads();
+    uint32_t before = carry, all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += wave_sums[w];
+      all += wave_sums[w];
+    }
+    if (b < n_blocks) row[b] = before + s - v;
+    carry += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+__global__ __launch_bounds__(ES_THREADS) void embed_scatter_kernel(const EmbedSort a) {
+  __shared__ uint32_t seen[ES_WAVES][ES_DIGITS];       // entries of the digit in this wave so far; then where the wave's first goes
+  __shared__ uint32_t wave_sums[ES_WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int d = threadIdx.x; d < ES_WAVES * ES_DIGITS; d += ES_THREADS) (&seen[0][0])[d] = 0;
+  const int64_t i0 = (int64_t)blockIdx.x * ES_TILE + wave * (64 * ES_ITEMS) + lane;
+  uint32_t key[ES_ITEMS], val[ES_ITEMS], rank[ES_ITEMS];
+#pragma unroll
+  for (int r = 0; r < ES_ITEMS; ++r) {
+    const int64_t i = i0 + 64 * r;
+    key[r] = i < a.n ? es_key(a, i) : 0u;
+    val[r] = a.ids ? (uint32_t)i : i < a.n ? a.val_in[i] : 0u;
+  }
+  // where each digit begins: the totals' exclusive prefix sums (threads 0 .. ES_DIGITS - 1), plus this block's offset
+  uint32_t start = 0;
+  {
+    const uint32_t v = threadIdx.x < ES_DIGITS ? a.totals[threadIdx.x] : 0u;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = __shfl_up((int)s, o, 64);
+      if (lane >= o) s += u;
+    }
+    if (lane == 63) wave_sums[wave] = s;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) start += wave_sums[w];
+    start += s - v;
+    if (threadIdx.x < ES_DIGITS) start += a.counts[(int64_t)threadIdx.x * a.n_blocks + blockIdx.x];
+  }
+#pragma unroll
+  for (int r = 0; r < ES_ITEMS; ++r) {
+    const bool live = i0 + 64 * r < a.n;
+    const uint32_t d = (key[r] >> a.shift) & (ES_DIGITS - 1);
+    uint64_t peers = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < ES_BITS; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1u);
+      peers &= ((d >> b) & 1u) ? set : ~set;
+    }
+    const uint32_t below = __popcll(peers & ((1ull << lane) - 1));
+    const uint32_t base = seen[wave][d];               // (a wave's LDS operations complete in order)
+    rank[r] = base + below;
+    asm volatile("" ::: "memory");
+    if (live && below == 0) seen[wave][d] = base + __popcll(peers);
+    asm volatile("" ::: "memory");
+  }
+  __syncthreads();
+  if (threadIdx.x < ES_DIGITS) {
+    uint32_t at = start;
+#pragma unroll
+    for (int w = 0; w < ES_WAVES; ++w) {
+      const uint32_t c = seen[w][threadIdx.x];
+      seen[w][threadIdx.x] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ES_ITEMS; ++r)
+    if (i0 + 64 * r < a.n) {
+      const uint32_t at = seen[wave][(key[r] >> a.shift) & (ES_DIGITS - 1)] + rank[r];
+      a.key_out[at] = key[r];
+      a.val_out[at] = val[r];
+    }
+}
+
+static int64_t round256(int64_t b) { return (b + 255) & ~(int64_t)255; }
+static int es_blocks(int64_t n) { return (int)((n + ES_TILE - 1) / ES_TILE); }
+// two more pairs of arrays to pass through, the counts and the totals
+static int64_t embed_sort_bytes(int64_t n) {
+  return n <= EMBED_SMALL_SORT ? 0 : 2 * round256(4 * n) + round256(4 * (int64_t)ES_DIGITS * (es_blocks(n) + 1));
+}
+
+// Stable ascending sort of the ids' keys with their positions; `zero` is cleared beside it.
+static int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, uint32_t* keys, uint32_t* perm,
+                      unsigned char* ws, const EmbedZero& zero, hipStream_t s) {
+  int bits = 1;
+  while (bits < 32 && (1ull << bits) <= (uint64_t)n_rows) ++bits;      // (keys go up to n_rows itself)
+  if (n <= EMBED_SMALL_SORT) return embed_small_sort(ids, ids_i32, n, n_rows, pad, bits, keys, perm, zero, s);
+  uint32_t* other_keys = (uint32_t*)ws;
+  uint32_t* other_perm = (uint32_t*)(ws + round256(4 * n));
+  uint32_t* counts = (uint32_t*)(ws + 2 * round256(4 * n));
+  EmbedSort a{ids, ids_i32, n_rows, pad, nullptr, nullptr, nullptr, nullptr, n, es_blocks(n), 0, counts,
+              counts + (int64_t)ES_DIGITS * es_blocks(n)};
+  const int passes = (bits + ES_BITS - 1) / ES_BITS;
+  for (int p = 0; p < passes; ++p) {                                   // the last pass ends in keys / perm
+    const bool to_result = (passes - 1 - p) % 2 == 0;
+    a.key_out = to_result ? keys : other_keys;
+    a.val_out = to_result ? perm : other_perm;
+    a.shift = p * ES_BITS;
+    const unsigned clear = p == 0 ? (unsigned)((zero.n16 + ES_THREADS) / ES_THREADS) : 0u;
+    hipLaunchKernelGGL(embed_count_kernel, dim3(a.n_blocks + clear), dim3(ES_THREADS), 0, s, a, zero);
+    hipLaunchKernelGGL(embed_offsets_kernel, dim3(ES_DIGITS), dim3(256), 0, s, a.counts, a.n_blocks, a.totals);
+    hipLaunchKernelGGL(embed_scatter_kernel, dim3(a.n_blocks), dim3(ES_THREADS), 0, s, a);
+    a.ids = nullptr;
+    a.key_in = a.key_out;
+    a.val_in = a.val_out;
+  }
+  return check_launch("bkg_embed_grad: sort");
+}
+
 // lanes of a row group: the smallest power of two that covers a row's accesses, at most a wave
 static int lanes_log2(int64_t d, int vec) {
   int l = 0;
@@ -302,8 +477,6 @@ static int embed_chunk(int64_t n) {
   return chunk;
 }
 static int64_t embed_chunks(int64_t n) { return (n + embed_chunk(n) - 1) / embed_chunk(n); }
-static int64_t round256(int64_t b) { return (b + 255) & ~(int64_t)255; }
-
 }  // namespace bkg
 
 using namespace bkg;
@@ -325,7 +498,7 @@ extern "C" int bkg_embed_rows(const void* w, int32_t type, int64_t ldw, int64_t 
 
 extern "C" int64_t bkg_embed_grad_workspace_bytes(int64_t n, int64_t d) {
   if (n <= 0 || d <= 0) return 0;
-  return 2 * round256(4 * (n + EG_PAD)) + 2 * round256(4 * n) + round256(8 * embed_chunks(n) * d) + embed_sort_workspace_bytes(n) + 256;
+  return 2 * round256(4 * (n + EG_PAD)) + round256(8 * embed_chunks(n) * d) + embed_sort_bytes(n);
 }
 
 extern "C" int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t d, const void* ids, int32_t ids_i32, int64_t n,
@@ -349,18 +522,17 @@ extern "C" int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t 
   }
   const EmbedZero z{(uint4*)dw, n16, (unsigned char*)dw + n16 * 16, (int)(total - n16 * 16), n ? keys + n : nullptr,
                     n ? perm + n : nullptr, EG_PAD};
-  if (n == 0 || n > EMBED_SMALL_SORT) {
+  if (n == 0) {
     hipLaunchKernelGGL(embed_zero_kernel, dim3((unsigned)((n16 + 256) / 256)), dim3(256), 0, s, z);
-    if (n == 0) return check_launch("bkg_embed_grad");
+    return check_launch("bkg_embed_grad");
   }
   BKG_ARG(g && ids, "bkg_embed_grad: null buffer");
-  uint32_t* scratch = (uint32_t*)ws; ws += 2 * round256(4 * n);
   EmbedGradArgs a{};
   a.keys = keys; a.perm = perm; a.n = n; a.n_rows = n_rows; a.scale = scale; a.d = (int)d;
   a.chunk = embed_chunk(n);
   a.n_chunks = embed_chunks(n);
   a.part = (float*)ws; ws += round256(8 * a.n_chunks * d);
-  const int rc = embed_sort(ids, ids_i32, n, n_rows, pad, scratch, keys, perm, ws, embed_sort_workspace_bytes(n), z, s);
+  const int rc = embed_sort(ids, ids_i32, n, n_rows, pad, keys, perm, ws, z, s);
   if (rc) return rc;
   int bytes = access_bytes(g, d * e, ldg * e);
   const int ob = access_bytes(dw, d * e, d * e);

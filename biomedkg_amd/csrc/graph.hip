@@ -114,21 +114,7 @@ __global__ void role_incidence_keys_kernel(const int64_t* __restrict__ head, con
   vals[i] = oth | ((uint32_t)rel[t] << 24);
 }
 
-// The sort keys of an embedding lookup (csrc/embed.hip): the id, or n_rows for an entry whose gradient goes nowhere.
-__device__ __forceinline__ uint32_t embed_key(const void* __restrict__ ids, int ids_i32, int64_t i, int64_t n_rows, int64_t pad) {
-  const int64_t v = ids_i32 ? (int64_t)static_cast<const int32_t*>(ids)[i] : static_cast<const int64_t*>(ids)[i];
-  return (v < 0 || v >= n_rows || v == pad) ? (uint32_t)n_rows : (uint32_t)v;
-}
-
-__global__ void embed_keys_kernel(const void* __restrict__ ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad,
-                                  uint32_t* __restrict__ keys, uint32_t* __restrict__ iota) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
-  keys[i] = embed_key(ids, ids_i32, i, n_rows, pad);
-  iota[i] = (uint32_t)i;
-}
-
-// small_sort_kernel for these keys: up to 1024 * IPT ids in one launch (positions behind n carry all-ones keys); the blocks
+// small_sort_kernel for the ids of an embedding lookup (csrc/embed.hip): up to 1024 * IPT ids in one launch (positions behind n carry all-ones keys); the blocks
 // behind the first clear the gradient the sort is for
 template <int IPT>
 __global__ __launch_bounds__(1024) void embed_small_sort_kernel(const void* __restrict__ ids, int ids_i32, int n, int64_t n_rows,
@@ -463,33 +449,21 @@ static int sort_edges_impl(const int64_t* lo, const int64_t* hi, int64_t n_lo, i
 }
 
 namespace bkg {
-int64_t embed_sort_workspace_bytes(int64_t n) { return n <= SMALL_SORT_MAX ? 0 : bkg_sort_workspace_bytes(n); }
-
-int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, uint32_t* scratch, uint32_t* sorted_keys,
-               uint32_t* perm, void* workspace, int64_t workspace_bytes, const EmbedZero& zero, hipStream_t s) {
+int embed_small_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, int bits, uint32_t* sorted_keys,
+                     uint32_t* perm, const EmbedZero& zero, hipStream_t s) {
   static_assert(EMBED_SMALL_SORT == SMALL_SORT_MAX, "one launch up to the one-workgroup sort's size");
-  int bits = 1;
-  while (bits < 32 && (1ull << bits) <= (uint64_t)n_rows) ++bits;      // (keys go up to n_rows itself)
-  if (n <= SMALL_SORT_MAX) {
-    // (a position behind n must stay behind every real key in the sorted bits: its low bits are all ones, and a real key
-    // that has them too comes before it because the sort is stable)
-    const unsigned blocks = (unsigned)(1 + (zero.n16 + 1024) / 1024);
-#define BKG_EMBED_SORT_LAUNCH(IPT)                                                                                          \
+  // (a position behind n must stay behind every real key in the sorted bits: its low bits are all ones, and a real key
+  // that has them too comes before it because the sort is stable)
+  const unsigned blocks = (unsigned)(1 + (zero.n16 + 1024) / 1024);
+#define BKG_EMBED_SORT_LAUNCH(IPT)                                                                                         \
   hipLaunchKernelGGL(embed_small_sort_kernel<IPT>, dim3(blocks), dim3(1024), 0, s, ids, ids_i32, (int)n, n_rows, pad, bits, \
                      sorted_keys, perm, zero)
-    if (n <= 1024) BKG_EMBED_SORT_LAUNCH(1);
-    else if (n <= 2048) BKG_EMBED_SORT_LAUNCH(2);
-    else if (n <= 4096) BKG_EMBED_SORT_LAUNCH(4);
-    else BKG_EMBED_SORT_LAUNCH(8);
+  if (n <= 1024) BKG_EMBED_SORT_LAUNCH(1);
+  else if (n <= 2048) BKG_EMBED_SORT_LAUNCH(2);
+  else if (n <= 4096) BKG_EMBED_SORT_LAUNCH(4);
+  else BKG_EMBED_SORT_LAUNCH(8);
 #undef BKG_EMBED_SORT_LAUNCH
-    return check_launch("bkg_embed_grad: sort and clear");
-  }
-  hipLaunchKernelGGL(embed_keys_kernel, grid1(n), dim3(256), 0, s, ids, ids_i32, n, n_rows, pad, scratch, scratch + n);
-  size_t bytes = (size_t)workspace_bytes;
-  hipError_t e = rocprim::radix_sort_pairs<SortConfig>(workspace, bytes, scratch, sorted_keys, scratch + n, perm, (size_t)n, 0,
-                                                       bits, s);
-  if (e != hipSuccess) { set_error("bkg_embed_grad: sort", e); return (int)e; }
-  return check_launch("bkg_embed_grad: sort");
+  return check_launch("bkg_embed_grad: sort and clear");
 }
 }  // namespace bkg
 

@@ -105,6 +105,21 @@ def test_embedding_gradient_of_long_runs(runs, shuffle):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("v", [2, 511, 512, 513, 130000, 262143, 262144, 3000000])
+@pytest.mark.parametrize("n", [8192, 8193, 12288, 50001])
+def test_embedding_gradient_over_many_rows(v, n):
+    """one, two and three passes of the sort, tables with and without a spare bit above the last row"""
+    gen = torch.Generator().manual_seed(v + n)
+    ids = torch.randint(0, v, (n,), generator=gen)
+    ids[:3] = torch.tensor([v - 1, 0, v - 1])
+    w = torch.empty(v, 4).cuda()
+    w.zero_()
+    g = torch.randn(n, 4, generator=gen).cuda()
+    out, dw = run_embedding(w, ids.cuda(), 1.0, None, g)
+    check_embedding(w, ids, 1.0, None, g, out, dw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("id_type", [torch.int64, torch.int32])
 def test_embedding_padding_and_outside_ids(dtype, id_type):
