@@ -16,7 +16,6 @@
 namespace bkg {
 
 constexpr int KD_THREADS = 256;                  // blocks that share a row
-constexpr int KD_ROW_THREADS = 1024;             // a block that has a row to itself
 constexpr int KD_MAX_K = 1024;
 constexpr float KD_LOG2E = 1.4426950408889634f, KD_LN2 = 0.6931471805599453f;
 
@@ -36,6 +35,7 @@ struct KdArgs {
   void* d; int64_t ldd;                          // the gradient (null: none)
   const float* g; int g_step; float coef;        // d = g[row g_step] coef (p - q); g null: 1
   int64_t n_rows;
+  int stream;                                    // the gradient is beyond STREAM_BYTES
 };
 
 __device__ __forceinline__ float kd_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
@@ -100,8 +100,6 @@ __device__ __forceinline__ void kd_stats(const T* __restrict__ xr, const KdSpan<
     if (f > m) { s *= kd_exp2((m - f) * c); m = ref = f; }            // (s = 0 while m = -inf)
     s += kd_exp2((f - ref) * c);
   };
-  for (int i = threadIdx.x; i < sp.head; i += THREADS) one(widen(xr[i]));
-  for (int i = sp.tail0 + threadIdx.x; i < sp.tail1; i += THREADS) one(widen(xr[i]));
   auto pack = [&](const Pack<T, VE>& r) {
     float f[VE], top = -INFINITY;
 #pragma unroll
@@ -119,6 +117,8 @@ __device__ __forceinline__ void kd_stats(const T* __restrict__ xr, const KdSpan<
     for (int u = 0; u < U; ++u) pack(r[u]);
   }
   for (; i < sp.v1; i += THREADS) pack(xv[i]);
+  for (int j = threadIdx.x; j < sp.head; j += THREADS) one(widen(xr[j]));
+  for (int j = sp.tail0 + threadIdx.x; j < sp.tail1; j += THREADS) one(widen(xr[j]));
 }
 
 // The block's (m, s) from its threads'; every thread gets it.
@@ -182,6 +182,28 @@ __device__ __forceinline__ float kd_loss(const KdArgs& a, const T* __restrict__ 
   return a.temp * a.temp * kd_block_sum(loss, red);
 }
 
+// The teacher's columns of a row's gradient (the block's part of them) are written again, whole, once the others are there.
+template <typename T>
+__device__ __forceinline__ void kd_write_entries(const KdArgs& a, const T* __restrict__ xr, T* __restrict__ dr, const KdSpan<T>& sp,
+                                                 const KdRow& rw, float scale, const int* __restrict__ id_lds,
+                                                 float* __restrict__ t_lds) {
+  const float c = a.c, ps = scale / rw.sum, ref = rw.m == -INFINITY ? 0.f : rw.m, inv_ts = 1.f / rw.tsum;
+  for (int j = threadIdx.x; j < a.te.k; j += blockDim.x) t_lds[j] = kd_exp2((t_lds[j] - rw.tmax) * c) * inv_ts;
+  __syncthreads();                                                    // (also orders the stores before it and those below)
+  for (int j = threadIdx.x; j < a.te.k; j += blockDim.x) {
+    const int id = id_lds[j];
+    if (id < 0 || !sp.mine(id)) continue;
+    bool first = true;                                                // (an id that occurs again is its first place's)
+    float q = 0.f;
+    for (int i = 0; i < a.te.k; ++i) {
+      const bool same = id_lds[i] == id;
+      first = first && (i >= j || !same);
+      q += same ? t_lds[i] : 0.f;
+    }
+    if (first) dr[id] = (T)(kd_exp2((widen(xr[id]) - ref) * c) * ps - scale * q);
+  }
+}
+
 // The block's part of the row's gradient, scale (p - q).  id_lds / t_lds hold the teacher's entries.
 template <typename T, int THREADS>
 __device__ __forceinline__ void kd_write_grad(const KdArgs& a, const T* __restrict__ xr, T* __restrict__ dr, const KdSpan<T>& sp,
@@ -198,7 +220,8 @@ __device__ __forceinline__ void kd_write_grad(const KdArgs& a, const T* __restri
   auto pack = [&](Pack<T, VE> r, int i) {
 #pragma unroll
     for (int j = 0; j < VE; ++j) r.v[j] = (T)value(widen(r.v[j]));
-    store16(dv + (int64_t)i * VE, r);
+    if (a.stream) stream16(dv + (int64_t)i * VE, r);
+    else store16(dv + (int64_t)i * VE, r);
   };
   if ((reinterpret_cast<uintptr_t>(dv) & 15) == 0) {
     int i = sp.v0 + threadIdx.x;
@@ -213,45 +236,90 @@ __device__ __forceinline__ void kd_write_grad(const KdArgs& a, const T* __restri
   } else {                                                            // x and d begin at different places of 16 bytes
     for (int i = sp.v0 * VE + threadIdx.x; i < sp.v1 * VE; i += THREADS) dv[i] = (T)value(widen(xr[sp.first + i]));
   }
-  if (off) return;
-  const float inv_ts = 1.f / rw.tsum;
-  for (int j = threadIdx.x; j < a.te.k; j += THREADS) t_lds[j] = kd_exp2((t_lds[j] - rw.tmax) * c) * inv_ts;
-  __syncthreads();                                                    // (also orders the stores above before the ones below)
-  for (int j = threadIdx.x; j < a.te.k; j += THREADS) {               // the entries' columns are written again, whole
-    const int id = id_lds[j];
-    if (id < 0 || !sp.mine(id)) continue;
-    bool first = true;
-    float q = 0.f;
-    for (int i = 0; i < a.te.k; ++i) {
-      const bool same = id_lds[i] == id;
-      first = first && (i >= j || !same);
-      q += same ? t_lds[i] : 0.f;
-    }
-    if (first) dr[id] = (T)(value(widen(xr[id])) - scale * q);
-  }
+  if (!off) kd_write_entries(a, xr, dr, sp, rw, scale, id_lds, t_lds);
 }
 
-// ---- a row per block: statistics, loss and (d given) the gradient of its own loss
-template <typename T>
-__global__ __launch_bounds__(KD_ROW_THREADS) void kd_row_kernel(const KdArgs a) {
+// What a block of N threads that has a row to itself makes of their (m, s) and teacher entries (t, t + N, ..: id -1 for none,
+// its t and its logit xt): the row's statistics and loss, in every thread.  red: [4][waves].
+struct KdDone { KdRow rw; float loss; };
+template <int N> struct KdEntries { int id[KD_MAX_K / N]; float tv[KD_MAX_K / N], xt[KD_MAX_K / N], e[KD_MAX_K / N]; };
+template <int N>
+__device__ __forceinline__ KdDone kd_finish_row(const KdArgs& a, float m, float s, KdEntries<N>& te, float (*red)[N / 64]) {
+  constexpr int W = N / 64, KD_E = KD_MAX_K / N;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float c = a.c;
+  float tm = -INFINITY;
+  bool some = false;
+#pragma unroll
+  for (int x = 0; x < KD_E; ++x)
+    if (te.id[x] >= 0) { tm = fmaxf(tm, te.tv[x]); some = true; }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    kd_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
+    tm = fmaxf(tm, __shfl_xor(tm, o, 64));
+  }
+  some = __ballot(some) != 0;
+  if (lane == 0) { red[0][wave] = m; red[1][wave] = s; red[2][wave] = tm; red[3][wave] = some ? 1.f : 0.f; }
+  __syncthreads();
+  const bool any = __ballot(red[3][lane & (W - 1)] != 0.f) != 0;
+  m = red[0][lane & (W - 1)]; s = red[1][lane & (W - 1)]; tm = red[2][lane & (W - 1)];
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    kd_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
+    tm = fmaxf(tm, __shfl_xor(tm, o, 64));
+  }
+  // the teacher's sum and the loss: sum q (ln q - ln p) = sum e ((t - tm) - (x - m)) / (T sum e) - ln sum e + ln s
+  float ts = 0.f, gap = 0.f;
+#pragma unroll
+  for (int x = 0; x < KD_E; ++x) {
+    te.e[x] = te.id[x] >= 0 ? kd_exp2((te.tv[x] - tm) * c) : 0.f;
+    ts += te.e[x];
+    if (!(te.e[x] == 0.f)) gap += te.e[x] * ((te.tv[x] - tm) - (te.xt[x] - m));
+  }
+  ts = wave_sum(ts); gap = wave_sum(gap);
+  __syncthreads();
+  if (lane == 0) { red[0][wave] = ts; red[1][wave] = gap; }
+  __syncthreads();
+  ts = red[0][lane & (W - 1)]; gap = red[1][lane & (W - 1)];
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) { ts += __shfl_xor(ts, o, 64); gap += __shfl_xor(gap, o, 64); }
+  const bool off = !any || (m == -INFINITY && s == 0.f);
+  const float ln_s = KD_LN2 * __builtin_amdgcn_logf(s), ln_ts = KD_LN2 * __builtin_amdgcn_logf(ts);
+  const float loss = off ? 0.f : a.temp * a.temp * (gap * (c * KD_LN2) / ts - ln_ts + ln_s);
+  return KdDone{KdRow{m, off ? 0.f : s, tm, off ? 0.f : ts}, loss};
+}
+
+// ---- a row per block: statistics, loss and (d given) the gradient of its own loss, for which the row is read again.  At 1024
+// threads two blocks share a CU, and the rows in work (133 MB of 260 KB rows) stay in the Infinity Cache; more, smaller blocks
+// push them out (4096 x 130000 in bf16: 1024 threads 547 us, 512 594, 256 699).  Rows up to KD_SHORT bytes take 512 threads
+// (1021 x 32771 in fp16, loss only: 17 us against 21).  Keeping part of a row on the CU -- 272 KB of registers and LDS, one
+// block per CU, each place filled with the next row's access as its gradient leaves -- took 595 us (nothing moves while it
+// adds up), two smaller blocks with half a row kept 537.
+constexpr int64_t KD_SHORT = 128 << 10;
+template <typename T, int N>
+__global__ __launch_bounds__(N) void kd_row_kernel(const KdArgs a) {
   __shared__ int id_lds[KD_MAX_K];
-  __shared__ float t_lds[KD_MAX_K], red[2 * KD_ROW_THREADS / 64];
+  __shared__ float t_lds[KD_MAX_K], red[4][N / 64];
   const int64_t row = blockIdx.x;
   const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
   const KdSpan<T> sp(xr, a.v, 0, 1);
-  float m = -INFINITY, s = 0.f, tm, ts;
+  float m = -INFINITY, s = 0.f;
   kd_load_teacher(a.te, row, a.v, id_lds, t_lds);
-  kd_stats<T, KD_ROW_THREADS>(xr, sp, a.c, m, s);
-  kd_block_join<KD_ROW_THREADS>(m, s, a.c, red);
-  kd_teacher_softmax(a.te.k, a.c, id_lds, t_lds, red, tm, ts);
-  const float loss = kd_loss(a, xr, id_lds, t_lds, m, s, tm, ts, red);
-  const bool off = ts == 0.f || (m == -INFINITY && s == 0.f);
-  const KdRow rw{m, off ? 0.f : s, tm, off ? 0.f : ts};
-  if (threadIdx.x == 0) {
-    a.losses[row] = off ? 0.f : loss;
-    a.rows[row] = rw;
+  kd_stats<T, N>(xr, sp, a.c, m, s);
+  KdEntries<N> te;
+#pragma unroll
+  for (int x = 0; x < KD_MAX_K / N; ++x) {
+    const int j = threadIdx.x + x * N;
+    te.id[x] = j < a.te.k ? id_lds[j] : -1;
+    te.tv[x] = te.id[x] >= 0 ? t_lds[j] : 0.f;
+    te.xt[x] = te.id[x] >= 0 ? widen(xr[te.id[x]]) : 0.f;
   }
-  if (a.d) kd_write_grad<T, KD_ROW_THREADS>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, rw, a.coef, id_lds, t_lds);
+  const KdDone done = kd_finish_row<N>(a, m, s, te, red);
+  if (threadIdx.x == 0) {
+    a.losses[row] = done.loss;
+    a.rows[row] = done.rw;
+  }
+  if (a.d) kd_write_grad<T, N>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, done.rw, a.coef, id_lds, t_lds);
 }
 
 // ---- few rows: a.parts blocks share one.  First the parts' statistics ...
@@ -342,11 +410,11 @@ static int kd_check(const char* who, const void* x, int32_t type, int64_t ldx, i
 
 using namespace bkg;
 
-#define BKG_BY_TYPE(type, CALL)                          \
+#define BKG_BY_TYPE(type, ...)                          \
   do {                                                   \
-    if ((type) == BKG_T_F32) { using T = float; CALL; }  \
-    else if ((type) == BKG_T_BF16) { using T = __bf16; CALL; } \
-    else { using T = _Float16; CALL; }                   \
+    if ((type) == BKG_T_F32) { using T = float; __VA_ARGS__; }  \
+    else if ((type) == BKG_T_BF16) { using T = __bf16; __VA_ARGS__; } \
+    else { using T = _Float16; __VA_ARGS__; }                   \
   } while (0)
 
 extern "C" int64_t bkg_distill_workspace_floats(int64_t rows, int64_t v, int32_t type) {
@@ -366,9 +434,11 @@ extern "C" int bkg_distill_forward(const void* x, int32_t type, int64_t ldx, int
   BKG_ARG(!d || (ldd >= v && (uintptr_t)d % e == 0), "bkg_distill_forward: misaligned gradient or overlapping rows");
   hipStream_t s = (hipStream_t)stream;
   KdArgs a{x, ldx, (int)v, kd_parts(rows, v, e), KD_LOG2E / temp, temp, {ids, ids_i32, ld_ids, t, t_type, ld_t, k},
-           workspace, (KdRow*)row_stats, losses, d, ldd, nullptr, 0, temp * sum_scale, rows};
-  if (kd_row_per_block(rows)) {
-    BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_row_kernel<T>), dim3((unsigned)rows), dim3(KD_ROW_THREADS), 0, s, a));
+           workspace, (KdRow*)row_stats, losses, d, ldd, nullptr, 0, temp * sum_scale, rows, rows * v * e > STREAM_BYTES};
+  if (kd_row_per_block(rows) && v * e <= KD_SHORT) {
+    BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_row_kernel<T, 512>), dim3((unsigned)rows), dim3(512), 0, s, a));
+  } else if (kd_row_per_block(rows)) {
+    BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_row_kernel<T, 1024>), dim3((unsigned)rows), dim3(1024), 0, s, a));
   } else {
     BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_part_kernel<T>), dim3((unsigned)(rows * a.parts)), dim3(KD_THREADS), 0, s, a));
     BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_join_kernel<T>), dim3((unsigned)(d ? rows * a.parts : rows)), dim3(KD_THREADS), 0, s, a));
@@ -387,7 +457,7 @@ extern "C" int bkg_distill_backward(const void* x, int32_t type, int64_t ldx, in
   BKG_ARG(!unless_one || g_step == 0, "bkg_distill_backward: a kept gradient has one upstream factor");
   hipStream_t s = (hipStream_t)stream;
   KdArgs a{x, ldx, (int)v, kd_parts(rows, v, e), KD_LOG2E / temp, temp, {ids, ids_i32, ld_ids, t, t_type, ld_t, k},
-           nullptr, (KdRow*)row_stats, nullptr, d, ldd, g, g_step, coef, rows};
+           nullptr, (KdRow*)row_stats, nullptr, d, ldd, g, g_step, coef, rows, rows * v * e > STREAM_BYTES};
   // (a launch that may have nothing to do keeps its grid small and loops)
   const int64_t all = rows * a.parts, grid = unless_one && all > 2048 ? 2048 : all;
   BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_regrad_kernel<T>), dim3((unsigned)grid), dim3(KD_THREADS), 0, s, a, unless_one));

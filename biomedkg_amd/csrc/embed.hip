@@ -26,7 +26,9 @@ __device__ __forceinline__ int64_t embed_id(const void* __restrict__ ids, int id
 constexpr int EMBED_UNROLL = 4;
 
 // A lane group of 2^lpr_log2 lanes copies a row's VEC-wide columns of tile blockIdx.y; UNROLL rows in flight per group.
-template <typename T, int VEC>
+// STREAM: a result beyond STREAM_BYTES leaves past the L2s, so that the table's rows stay (a million rows of 512 bytes out of
+// 130000: 168 us written through the L2s, 131 us past them).
+template <typename T, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ w, int64_t ldw, int64_t n_rows, int d,
                                                          const void* __restrict__ ids, int ids_i32, int64_t n, float scale,
                                                          T* __restrict__ out, int64_t ldo, int lpr_log2) {
@@ -52,7 +54,8 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const T* __restrict__ w
     if (i >= n) break;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) r[u].v[j] = (T)(widen(r[u].v[j]) * scale);
-    *reinterpret_cast<Pack<T, VEC>*>(out + i * ldo + c) = r[u];
+    if constexpr (STREAM && sizeof(T) * VEC == 16) stream16(out + i * ldo + c, r[u]);
+    else *reinterpret_cast<Pack<T, VEC>*>(out + i * ldo + c) = r[u];
   }
 }
 
@@ -432,8 +435,12 @@ static void embed_rows_launch(const void* w, int64_t ldw, int64_t n_rows, int64_
   const int lpr = lanes_log2(d, VEC);
   const int64_t per_block = (256 >> lpr) * EMBED_UNROLL;
   const dim3 grid((unsigned)((n + per_block - 1) / per_block), (unsigned)ceil_div(d, (int64_t)VEC << lpr));
-  hipLaunchKernelGGL((embed_rows_kernel<T, VEC>), grid, dim3(256), 0, s, (const T*)w, ldw, n_rows, (int)d, ids, ids_i32, n, scale,
-                     (T*)out, ldo, lpr);
+  if (sizeof(T) * VEC == 16 && n * d * (int64_t)sizeof(T) > STREAM_BYTES)
+    hipLaunchKernelGGL((embed_rows_kernel<T, VEC, sizeof(T) * VEC == 16>), grid, dim3(256), 0, s, (const T*)w, ldw, n_rows, (int)d,
+                       ids, ids_i32, n, scale, (T*)out, ldo, lpr);
+  else
+    hipLaunchKernelGGL((embed_rows_kernel<T, VEC, false>), grid, dim3(256), 0, s, (const T*)w, ldw, n_rows, (int)d, ids, ids_i32, n,
+                       scale, (T*)out, ldo, lpr);
 }
 
 template <typename T, int VEC>

@@ -21,6 +21,13 @@ template <typename T> __device__ __forceinline__ void store16(T* p, const Pack<T
   *reinterpret_cast<rt_i32x4*>(p) = __builtin_bit_cast(rt_i32x4, v);
 }
 
+// The same past the caches (non-temporal): for results beyond STREAM_BYTES, the Infinity Cache's size, which no later call finds
+// there anyway and which would push out what this one still reads.
+constexpr int64_t STREAM_BYTES = 256 << 20;
+template <typename T> __device__ __forceinline__ void stream16(T* p, const Pack<T, 16 / sizeof(T)>& v) {
+  __builtin_nontemporal_store(__builtin_bit_cast(rt_i32x4, v), reinterpret_cast<rt_i32x4*>(p));
+}
+
 // the largest access in bytes (<= 16) that `bytes`, a row of it and its start are all multiples of
 static inline int access_bytes(const void* p, int64_t row_bytes, int64_t ld_bytes) {
   const uint64_t all = (uint64_t)(uintptr_t)p | (uint64_t)row_bytes | (uint64_t)ld_bytes | 16u;

@@ -330,7 +330,8 @@ def test_distill_large_offsets_and_lowest_values(rows):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,v,k", [(200, 3001, 9), (193, 20, 3), (300, 9000, 40), (191, 9001, 7), (4, 70001, 64)])
+@pytest.mark.parametrize("rows,v,k", [(200, 3001, 9), (193, 20, 3), (300, 9000, 40), (191, 9001, 7), (4, 70001, 64),
+                                      (193, 50001, 5), (192, 25000, 8), (200, 70005, 3)])
 def test_distill_rows_on_both_sides_of_the_split(dtype, rows, v, k):
     check_distill(*make_distill(rows, v, k, dtype, rows + v + k), 1.25)
 
