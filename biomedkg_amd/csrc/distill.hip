@@ -36,6 +36,8 @@ struct KdArgs {
   const float* g; int g_step; float coef;        // d = g[row g_step] coef (p - q); g null: 1
   int64_t n_rows;
   int stream;                                    // the gradient is beyond STREAM_BYTES
+  unsigned* done;                                // (parts) rows whose loss is there; the last one's block adds them up:
+  float* loss; float sum_scale;                  // loss[0] = sum_scale * their sum (null: not wanted)
 };
 
 __device__ __forceinline__ float kd_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
@@ -322,6 +324,20 @@ __global__ __launch_bounds__(N) void kd_row_kernel(const KdArgs a) {
   if (a.d) kd_write_grad<T, N>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, done.rw, a.coef, id_lds, t_lds);
 }
 
+// scale * the sum of the rows' losses, in a fixed order (one block)
+template <int N>
+__device__ __forceinline__ void kd_sum(const float* __restrict__ losses, int64_t n, float scale, float* red, float* __restrict__ out) {
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += N) s += losses[i];
+  s = kd_block_sum(s, red);
+  if (threadIdx.x == 0) out[0] = scale * s;
+}
+__global__ __launch_bounds__(1024) void kd_sum_kernel(const float* __restrict__ losses, int64_t n, float scale,
+                                                      float* __restrict__ out) {
+  __shared__ float red[16];
+  kd_sum<1024>(losses, n, scale, red, out);
+}
+
 // ---- few rows: a.parts blocks share one.  First the parts' statistics ...
 template <typename T>
 __global__ __launch_bounds__(KD_THREADS) void kd_part_kernel(const KdArgs a) {
@@ -329,6 +345,7 @@ __global__ __launch_bounds__(KD_THREADS) void kd_part_kernel(const KdArgs a) {
   const int64_t row = blockIdx.x / a.parts;
   const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
   const KdSpan<T> sp(xr, a.v, blockIdx.x % a.parts, a.parts);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;      // (counted by the next launch)
   float m = -INFINITY, s = 0.f;
   kd_stats<T, KD_THREADS>(xr, sp, a.c, m, s);
   kd_block_join<KD_THREADS>(m, s, a.c, red);
@@ -357,20 +374,22 @@ __global__ __launch_bounds__(KD_THREADS) void kd_join_kernel(const KdArgs a) {
       a.rows[row] = rw;
     }
   }
+  if (p == 0 && a.loss) {                        // (which block is the last does not change the sum's order)
+    __shared__ bool last;
+    if (threadIdx.x == 0) {
+      __threadfence();
+      last = atomicAdd(a.done, 1u) == (unsigned)a.n_rows - 1;
+    }
+    __syncthreads();
+    if (last) {
+      __threadfence();
+      kd_sum<KD_THREADS>(a.losses, a.n_rows, a.sum_scale, red, a.loss);
+    }
+  }
   if (a.d) {
     const KdSpan<T> sp(xr, a.v, p, a.parts);
     kd_write_grad<T, KD_THREADS>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, rw, a.coef, id_lds, t_lds);
   }
-}
-
-// out[0] = scale * sum of the rows' losses, in a fixed order
-__global__ __launch_bounds__(1024) void kd_sum_kernel(const float* __restrict__ losses, int64_t n, float scale,
-                                                      float* __restrict__ out) {
-  __shared__ float red[16];
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += losses[i];
-  s = kd_block_sum(s, red);
-  if (threadIdx.x == 0) out[0] = scale * s;
 }
 
 // ---- the gradient from the kept row statistics.  unless_one: d already holds the gradient for g = 1.
@@ -418,7 +437,7 @@ using namespace bkg;
   } while (0)
 
 extern "C" int64_t bkg_distill_workspace_floats(int64_t rows, int64_t v, int32_t type) {
-  return rows <= 0 || v <= 0 ? 0 : 2 * rows * kd_parts(rows, v, type_bytes(type));
+  return rows <= 0 || v <= 0 ? 0 : 2 * rows * kd_parts(rows, v, type_bytes(type)) + 1;
 }
 
 // Few rows are shared by several blocks; from 192 rows on a block per row keeps three quarters of the CUs or more at work.
@@ -434,7 +453,8 @@ extern "C" int bkg_distill_forward(const void* x, int32_t type, int64_t ldx, int
   BKG_ARG(!d || (ldd >= v && (uintptr_t)d % e == 0), "bkg_distill_forward: misaligned gradient or overlapping rows");
   hipStream_t s = (hipStream_t)stream;
   KdArgs a{x, ldx, (int)v, kd_parts(rows, v, e), KD_LOG2E / temp, temp, {ids, ids_i32, ld_ids, t, t_type, ld_t, k},
-           workspace, (KdRow*)row_stats, losses, d, ldd, nullptr, 0, temp * sum_scale, rows, rows * v * e > STREAM_BYTES};
+           workspace, (KdRow*)row_stats, losses, d, ldd, nullptr, 0, temp * sum_scale, rows, rows * v * e > STREAM_BYTES,
+           (unsigned*)(workspace + 2 * rows * kd_parts(rows, v, e)), loss, sum_scale};
   if (kd_row_per_block(rows) && v * e <= KD_SHORT) {
     BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_row_kernel<T, 512>), dim3((unsigned)rows), dim3(512), 0, s, a));
   } else if (kd_row_per_block(rows)) {
@@ -443,7 +463,7 @@ extern "C" int bkg_distill_forward(const void* x, int32_t type, int64_t ldx, int
     BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_part_kernel<T>), dim3((unsigned)(rows * a.parts)), dim3(KD_THREADS), 0, s, a));
     BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_join_kernel<T>), dim3((unsigned)(d ? rows * a.parts : rows)), dim3(KD_THREADS), 0, s, a));
   }
-  if (loss) hipLaunchKernelGGL(kd_sum_kernel, dim3(1), dim3(1024), 0, s, losses, rows, sum_scale, loss);
+  if (loss && kd_row_per_block(rows)) hipLaunchKernelGGL(kd_sum_kernel, dim3(1), dim3(1024), 0, s, losses, rows, sum_scale, loss);
   return check_launch("bkg_distill_forward");
 }
 
@@ -457,7 +477,7 @@ extern "C" int bkg_distill_backward(const void* x, int32_t type, int64_t ldx, in
   BKG_ARG(!unless_one || g_step == 0, "bkg_distill_backward: a kept gradient has one upstream factor");
   hipStream_t s = (hipStream_t)stream;
   KdArgs a{x, ldx, (int)v, kd_parts(rows, v, e), KD_LOG2E / temp, temp, {ids, ids_i32, ld_ids, t, t_type, ld_t, k},
-           nullptr, (KdRow*)row_stats, nullptr, d, ldd, g, g_step, coef, rows, rows * v * e > STREAM_BYTES};
+           nullptr, (KdRow*)row_stats, nullptr, d, ldd, g, g_step, coef, rows, rows * v * e > STREAM_BYTES, nullptr, nullptr, 0.f};
   // (a launch that may have nothing to do keeps its grid small and loops)
   const int64_t all = rows * a.parts, grid = unless_one && all > 2048 ? 2048 : all;
   BKG_BY_TYPE(type, hipLaunchKernelGGL((kd_regrad_kernel<T>), dim3((unsigned)grid), dim3(KD_THREADS), 0, s, a, unless_one));

@@ -32,12 +32,14 @@ def _ids(t, what):
         raise TypeError(f"{what}: expected int64 or int32, got {t.dtype}")
 
 
-def _same_device(what, first, *others):
-    """All tensors on the current device: the library launches on its current stream."""
-    L.require_cuda(first, *others)
-    dev = first.device
+def _on_current_device(what, dev, *others):
+    """Everything on one device, the current one: the library launches on its current stream."""
+    if dev.type != "cuda":
+        raise L.HipLibraryError(f"{what}: biomedkg_amd runs on MI355X only: got tensors on {dev} (there is no CPU fallback)")
     for t in others:
         if t is not None and t.device != dev:
+            if t.device.type != "cuda":
+                raise L.HipLibraryError(f"{what}: biomedkg_amd runs on MI355X only: got a tensor on {t.device}")
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
     if dev.index != torch.cuda.current_device():
         raise ValueError(f"{what}: tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()} "
@@ -47,11 +49,12 @@ def _same_device(what, first, *others):
 # ----------------------------------------------------------------------------- embedding
 def _embed_rows(weight, ids, scale):
     w = _rows(weight)
-    ids = ids if ids.is_contiguous() else ids.contiguous()
-    d = w.size(1)
-    out = torch.empty(ids.shape + (d,), dtype=w.dtype, device=w.device)
-    L.call("bkg_embed_rows", w.data_ptr(), _TYPE[w.dtype], w.stride(0), w.size(0), d, ids.data_ptr(),
-           ids.dtype == torch.int32, ids.numel(), scale, out.data_ptr(), d, L.stream())
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    v, d = w.shape
+    out = w.new_empty(ids.shape + (d,))
+    L.call("bkg_embed_rows", w.data_ptr(), _TYPE[w.dtype], w.stride(0), v, d, ids.data_ptr(), ids.dtype == torch.int32,
+           ids.numel(), scale, out.data_ptr(), d, L.stream())
     return out, ids
 
 
@@ -60,7 +63,7 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, weight, ids, scale, pad):
         out, ids = _embed_rows(weight, ids, scale)
         ctx.save_for_backward(ids)
-        ctx.scale, ctx.pad, ctx.shape, ctx.dtype = scale, pad, weight.shape, weight.dtype
+        ctx.scale, ctx.pad, ctx.shape = scale, pad, weight.shape
         return out
 
     @staticmethod
@@ -73,11 +76,11 @@ def _embedding_backward(ctx, g):
     (ids,) = ctx.saved_tensors
     v, d = ctx.shape
     n = ids.numel()
-    g = _rows(g.reshape(n, d))
-    dw = torch.empty(v, d, dtype=ctx.dtype, device=g.device)
+    g = _rows(g if g.dim() == 2 else g.reshape(n, d))
+    dw = g.new_empty((v, d))
     ws_bytes = L.lib().bkg_embed_grad_workspace_bytes(n, d)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device)
-    L.call("bkg_embed_grad", g.data_ptr(), _TYPE[ctx.dtype], g.stride(0), d, ids.data_ptr(), ids.dtype == torch.int32, n, v,
+    L.call("bkg_embed_grad", g.data_ptr(), _TYPE[g.dtype], g.stride(0), d, ids.data_ptr(), ids.dtype == torch.int32, n, v,
            ctx.pad, ctx.scale, dw.data_ptr(), ws.data_ptr(), ws_bytes, L.stream())
     return dw, None, None, None
 
@@ -97,7 +100,7 @@ def embedding(weight, ids, scale=1.0, padding_idx=None):
         raise ValueError(f"embedding: expected a [V, d] table, got {tuple(weight.shape)}")
     _type_of(weight, "embedding")
     _ids(ids, "embedding ids")
-    _same_device("embedding", weight, ids)
+    _on_current_device("embedding", weight.device, ids)
     v, d = weight.shape
     if v >= 2 ** 31 or ids.numel() >= 2 ** 31 or d > 2 ** 20:
         raise ValueError("embedding: at most 2^31 - 1 rows and ids, 2^20 columns")
@@ -116,14 +119,16 @@ def embedding(weight, ids, scale=1.0, padding_idx=None):
 def _distill_forward(x, ids, t, temp, sum_scale, want_sum, d=None):
     rows, v = x.shape
     dev, xt = x.device, _TYPE[x.dtype]
-    ws = torch.empty(L.lib().bkg_distill_workspace_floats(rows, v, xt), dtype=torch.float32, device=dev)
-    stats = torch.empty(rows, 4, dtype=torch.float32, device=dev)
-    losses = torch.empty(rows, dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev) if want_sum else None
+    # one buffer: the row statistics (kept for the backward), the rows' losses, the launches' scratch
+    n_ws = L.lib().bkg_distill_workspace_floats(rows, v, xt)
+    stats = torch.empty(4 * rows + (rows if want_sum else 0) + n_ws, dtype=torch.float32, device=dev)
+    out = torch.empty(() if want_sum else (rows,), dtype=torch.float32, device=dev)
+    base = stats.data_ptr()
+    losses = base + 16 * rows if want_sum else out.data_ptr()
     L.call("bkg_distill_forward", x.data_ptr(), xt, x.stride(0), rows, v, ids.data_ptr(), ids.dtype == torch.int32, ids.stride(0),
-           t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), temp, sum_scale, ws.data_ptr(), stats.data_ptr(),
-           losses.data_ptr(), L.ptr(loss), L.ptr(d), v, L.stream())
-    return (loss if want_sum else losses), stats
+           t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), temp, sum_scale, base + (20 if want_sum else 16) * rows, base,
+           losses, out.data_ptr() if want_sum else None, L.ptr(d), v, L.stream())
+    return out, stats
 
 
 class _TopkDistill(torch.autograd.Function):
@@ -188,7 +193,7 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, redu
     _type_of(logits, "topk_distill_loss logits")
     _type_of(teacher_logits, "topk_distill_loss teacher logits")
     _ids(teacher_ids, "topk_distill_loss teacher ids")
-    _same_device("topk_distill_loss", logits, teacher_ids, teacher_logits)
+    _on_current_device("topk_distill_loss", logits.device, teacher_ids, teacher_logits)
     if reduction not in ("batchmean", "sum", "none"):
         raise ValueError(f"topk_distill_loss: reduction {reduction!r} (batchmean, sum or none)")
     temp = float(temperature)
@@ -219,23 +224,51 @@ class Mx4Table:
     with zeros): ``codes`` uint8 ``[panels, rows, 64]`` (two columns a byte, the lower one in the low nibble) and ``scales``
     uint8 ``[panels, rows, 4]`` (the exponent of each 32 columns + 127; 255: the block held an infinity or NaN).  0.53 bytes a
     value."""
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("shape", "device", "codes_ptr", "scales_ptr", "_store")
 
     def __init__(self, codes, scales, shape):
-        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
+        self.shape = tuple(shape)
         rows, cols = self.shape
         panels = (cols + 127) // 128
         for t, want, what in ((codes, (panels, rows, 64), "codes"), (scales, (panels, rows, 4), "scales")):
             if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
                 raise ValueError(f"Mx4Table: {what} must be contiguous uint8 {want} for a table of {self.shape}")
+        if codes.device != scales.device:
+            raise ValueError(f"Mx4Table: codes on {codes.device}, scales on {scales.device}")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 4:
+            raise ValueError("Mx4Table: codes must be 16-byte, scales 4-byte aligned")
+        self.device, self.codes_ptr, self.scales_ptr = codes.device, codes.data_ptr(), scales.data_ptr()
+        self._store = (codes, scales)
+
+    @classmethod
+    def _empty(cls, rows, cols, device):
+        """An unwritten table in one piece of memory: the codes, then the scales."""
+        self = cls.__new__(cls)
+        panels = (cols + 127) // 128
+        self._store = torch.empty(panels * rows * 68, dtype=torch.uint8, device=device)
+        self.shape, self.device = (rows, cols), device
+        self.codes_ptr = self._store.data_ptr()
+        self.scales_ptr = self.codes_ptr + panels * rows * 64
+        return self
+
+    def _parts(self):
+        if not isinstance(self._store, tuple):
+            rows, panels = self.shape[0], (self.shape[1] + 127) // 128
+            cut = panels * rows * 64
+            self._store = (self._store[:cut].view(panels, rows, 64), self._store[cut:].view(panels, rows, 4))
+        return self._store
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self):
+        return self._parts()[0]
+
+    @property
+    def scales(self):
+        return self._parts()[1]
 
     @property
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return (self.shape[1] + 127) // 128 * self.shape[0] * 68
 
     def __repr__(self):
         return f"Mx4Table({self.shape[0]} x {self.shape[1]}, {self.nbytes} bytes, {self.device})"
@@ -248,17 +281,14 @@ def mx4_quantize(x):
     if x.dim() != 2 or x.size(1) == 0:
         raise ValueError(f"mx4_quantize: expected [rows, cols] with cols > 0, got {tuple(x.shape)}")
     _type_of(x, "mx4_quantize")
-    _same_device("mx4_quantize", x)
+    _on_current_device("mx4_quantize", x.device)
     rows, cols = x.shape
     if cols > 2 ** 24 or rows >= 2 ** 31:
         raise ValueError("mx4_quantize: at most 2^24 columns and 2^31 - 1 rows")
     x = _rows(x.detach())
-    panels = (cols + 127) // 128
-    codes = torch.empty(panels, rows, 64, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(panels, rows, 4, dtype=torch.uint8, device=x.device)
-    L.call("bkg_mx4_quantize", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, codes.data_ptr(), scales.data_ptr(),
-           L.stream())
-    return Mx4Table(codes, scales, (rows, cols))
+    table = Mx4Table._empty(rows, cols, x.device)
+    L.call("bkg_mx4_quantize", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, table.codes_ptr, table.scales_ptr, L.stream())
+    return table
 
 
 def mx4_dequantize(table, dtype=torch.float32):
@@ -267,10 +297,10 @@ def mx4_dequantize(table, dtype=torch.float32):
         raise TypeError("mx4_dequantize: expected an Mx4Table")
     if dtype not in _TYPE:
         raise TypeError(f"mx4_dequantize: float32, bfloat16 or float16, got {dtype}")
-    _same_device("mx4_dequantize", table.codes, table.scales)
+    _on_current_device("mx4_dequantize", table.device)
     rows, cols = table.shape
     out = torch.empty(rows, cols, dtype=dtype, device=table.device)
-    L.call("bkg_mx4_dequantize", table.codes.data_ptr(), table.scales.data_ptr(), rows, cols, out.data_ptr(), _TYPE[dtype], cols,
+    L.call("bkg_mx4_dequantize", table.codes_ptr, table.scales_ptr, rows, cols, out.data_ptr(), _TYPE[dtype], cols,
            L.stream())
     return out
 
@@ -293,14 +323,13 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     if out_dtype not in _TYPE:
         raise TypeError(f"mx4_linear: out_dtype float32, bfloat16 or float16, got {out_dtype}")
     if packed:
-        _same_device("mx4_linear", x.codes, table.codes, bias)
+        _on_current_device("mx4_linear", table.device, x, bias)
         m = x.shape[0]
         out = torch.empty(m, n, dtype=out_dtype, device=table.device)
-        L.call("bkg_mx4_matmul", x.codes.data_ptr(), x.scales.data_ptr(), m, table.codes.data_ptr(), table.scales.data_ptr(), n,
-               cols, L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.stream())
+        L.call("bkg_mx4_matmul", x.codes_ptr, x.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.stream())
         return out
     xt = _type_of(x, "mx4_linear")
-    _same_device("mx4_linear", x, table.codes, bias)
+    _on_current_device("mx4_linear", x.device, table, bias)
     if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
     lead = x.shape[:-1]
@@ -309,6 +338,6 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     out = torch.empty(lead + (n,), dtype=out_dtype, device=x.device)
     ws_bytes = L.lib().bkg_mx4_linear_workspace_bytes(m, cols)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    L.call("bkg_mx4_linear", x2.data_ptr(), xt, x2.stride(0), m, table.codes.data_ptr(), table.scales.data_ptr(), n, cols,
+    L.call("bkg_mx4_linear", x2.data_ptr(), xt, x2.stride(0), m, table.codes_ptr, table.scales_ptr, n, cols,
            L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
     return out
