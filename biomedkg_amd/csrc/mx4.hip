@@ -159,9 +159,9 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(mx_i32x4 a, mx_i32x4 b, mx_f32x16 c
 
 // Tiled product.  Four waves (2 x 2) compute a block of 64 MT x 64 NT outputs, (32 MT) x (32 NT) per wave.  Panels travel
 // through a ring of S LDS slots by LDS-DMA: a stage is the block's rows of one panel of A and of B (64 contiguous bytes a
-// row: a wave-instruction copies 16 whole rows) and their dwords of scales.  Slot c' of row r holds piece c' ^ ((r / 2) & 3)
-// (the swizzle is applied to the DMA's source address): the b128 fragment reads of 8 neighbouring rows then fall on
-// different banks.  One raw barrier per stage, placed between its two halves: behind it every wave has both halves of stage
+// row: a wave-instruction copies 16 whole rows) and their dwords of scales.  Slot c' of row r holds piece c' ^ ((r / 4) & 3)
+// (the swizzle is applied to the DMA's source address): the b128 fragment reads of 16 neighbouring rows then fall on all 64
+// banks once.  One raw barrier per stage, placed between its two halves: behind it every wave has both halves of stage
 // t in registers, so slot t is refilled with stage t + S, and the first fragments of stage t + 1 are read while the second
 // half of stage t multiplies.  The ring is retired by counted vmcnt waits: the loop issues nothing but DMAs.
 //
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   int64_t src[CH], ssrc[CH / 4];
 #pragma unroll
   for (int j = 0; j < CH; ++j)
-    src[j] = min(r0 + ((wave & 1) * CH + j) * 16 + (lane >> 2), rows - 1) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
+    src[j] = min(r0 + ((wave & 1) * CH + j) * 16 + (lane >> 2), rows - 1) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
 #pragma unroll
   for (int j = 0; j < CH / 4; ++j) ssrc[j] = min(r0 + ((wave & 1) * (CH / 4) + j) * 64 + lane, rows - 1);
   auto copy = [&](int stage, int slot, int j) {              // copy j of this wave's DMAS of a stage
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   const int wm = (wave & 1) * 32 * MT, wn = (wave >> 1) * 32 * NT;
   struct Frags { mx_i32x4 a[MT], b[NT]; };
   struct Scales { uint32_t a[MT], b[NT]; };
-  const int swz = (l31 >> 1) & 3;
+  const int swz = (l31 >> 2) & 3;
   auto read = [&](int slot, int h, Frags& f, int i) {        // fragment i of the MT + NT
     const unsigned char* base = lds + slot * STAGE + l31 * 64 + (((2 * h + half) ^ swz) * 16);
     if (i < MT) f.a[i] = *reinterpret_cast<const mx_i32x4*>(base + (wm + 32 * i) * 64);
@@ -367,7 +367,7 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
       for (int j = 0; j < 2; ++j) {
         const int64_t r = min(m0 + (wave * 2 + j) * 16 + (lane >> 2), a.m - 1);
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(a.ca + (st * a.m + r) * 64 + ((lane & 3) ^ ((lane >> 3) & 3)) * 16),
+            (const __attribute__((address_space(1))) void*)(a.ca + (st * a.m + r) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16),
             (__attribute__((address_space(3))) void*)(base + st * 8192 + (wave * 2 + j) * 1024), 16, 0, 0);
       }
     const int st = STEPS == 2 ? wave >> 1 : 0;
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           fa[i][h] = *reinterpret_cast<const mx_i32x4*>(base + st * 8192 + (wm + 32 * i + l31) * 64 +
-                                                        (((2 * h + half) ^ ((l31 >> 1) & 3)) * 16));
+                                                        (((2 * h + half) ^ ((l31 >> 2) & 3)) * 16));
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(256) void mx4_few_kernel(const Mx4Args a, const Mx4
       }
       const Mx4Piece q = mx4_piece(f);
       const int st = piece >> 4, w = piece & 15;                            // word w of the row's 16: 16-byte piece w / 4, swizzled
-      *reinterpret_cast<uint32_t*>(lds + st * 2048 + row * 64 + (((w >> 2) ^ ((row >> 1) & 3)) * 16) + (w & 3) * 4) = q.codes;
+      *reinterpret_cast<uint32_t*>(lds + st * 2048 + row * 64 + (((w >> 2) ^ ((row >> 2) & 3)) * 16) + (w & 3) * 4) = q.codes;
       if (w == 0) xs[st * 32 + row] = q.scales;
     }
     __syncthreads();
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256) void mx4_few_kernel(const Mx4Args a, const Mx4
       xa = *reinterpret_cast<const uint32_t*>(lds + a.steps * 2048 + st * 128 + l31 * 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        va[h] = *reinterpret_cast<const mx_i32x4*>(lds + st * 2048 + l31 * 64 + (((2 * h + half) ^ ((l31 >> 1) & 3)) * 16));
+        va[h] = *reinterpret_cast<const mx_i32x4*>(lds + st * 2048 + l31 * 64 + (((2 * h + half) ^ ((l31 >> 2) & 3)) * 16));
     }
     acc = mx_mfma<0>(va[0], vb[at][0], acc, xa >> (8 * half), xb[at] >> (8 * half));
     acc = mx_mfma<1>(va[1], vb[at][1], acc, xa >> (8 * half), xb[at] >> (8 * half));
