@@ -143,7 +143,7 @@ struct Mx4Args {
   const unsigned char* ca; const uint32_t* sa; int64_t m;
   const unsigned char* cb; const uint32_t* sb; int64_t n;
   int steps;                                     // panels of 128 columns
-  int m_tiles, n_tiles, band;
+  int m_tiles, n_tiles, band;                    // band: rows of tiles walked together / row tiles a streaming block walks
   const float* bias;
   void* out; int64_t ldo;
   int wide;                                      // the rows of `out` take aligned 16-byte stores
@@ -176,8 +176,8 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, half = lane >> 5;
 
-  // tile order: each XCD takes a contiguous part of the list; the list runs through 8 tiles of rows at a time, so the tiles
-  // in flight on one XCD share their panels in its L2
+  // tile order: each XCD takes a contiguous part of the list; the list runs through `band` tiles of rows at a time, so the
+  // tiles in flight on one XCD share their panels in its L2
   const int64_t total = (int64_t)a.m_tiles * a.n_tiles, per = (total + BKG_XCDS - 1) / BKG_XCDS;
   const int64_t t = (int64_t)(blockIdx.x % BKG_XCDS) * per + blockIdx.x / BKG_XCDS;
   if (blockIdx.x / BKG_XCDS >= per || t >= total) return;
@@ -574,6 +574,9 @@ static void mx4_launch(Mx4Args a, hipStream_t s) {
   (void)set;
   a.m_tiles = (int)((a.m + 64 * MT - 1) / (64 * MT));
   a.n_tiles = (int)((a.n + 64 * NT - 1) / (64 * NT));
+  // rows of tiles walked together: 8 share panels best; 2 where the output's rows are long, so that what is written at one time
+  // is a few whole rows (1021 x 130000 x 768: 127 us with 2, 152 with 8; 8192 x 8192 x 512: 43 and 40)
+  a.band = a.n >= (1 << 16) ? 2 : 8;
   const int64_t total = (int64_t)a.m_tiles * a.n_tiles;
   const unsigned grid = (unsigned)((total + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS);
   hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, S>), dim3(grid), dim3(256), LDS, s, a);
@@ -676,8 +679,11 @@ static void mx4_product(const Mx4Args& a, hipStream_t s) {
   if (a.m <= 32) mx4_few_launch<T, true>(a, Mx4X{}, s);
   else if (a.steps == 1) mx4_stream_launch<T, 1>(a, s);
   else if (a.steps == 2) mx4_stream_launch<T, 2>(a, s);
-  // 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128
+  // 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128:
+  // four slots a block (two blocks on a CU) where tiles are few, two slots (four blocks: one stores while others multiply)
+  // from 1024 tiles on (8192 x 8192 x 512: 40 us with two slots, 54 with four)
   else if ((a.m + 255) / 256 * ((a.n + 255) / 256) >= 192 && a.steps >= 8) mx4_launch<T, 4, 4, 4>(a, s);
+  else if ((a.m + 127) / 128 * ((a.n + 127) / 128) >= 1024) mx4_launch<T, 2, 2, 2>(a, s);
   else mx4_launch<T, 2, 2, 4>(a, s);
 }
 
@@ -687,7 +693,7 @@ extern "C" int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t
   if (m == 0 || n == 0) return 0;
   BKG_ARG(a_codes && a_scales && (uintptr_t)a_codes % 16 == 0 && (uintptr_t)a_scales % 4 == 0, "bkg_mx4_matmul: null or misaligned buffer");
   const Mx4Args a{(const unsigned char*)a_codes, (const uint32_t*)a_scales, m, (const unsigned char*)b_codes,
-                  (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 8, bias, out, ldo,
+                  (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0, bias, out, ldo,
                   access_bytes(out, 0, ldo * type_bytes(type)) == 16};
   BKG_BY_TYPE(type, mx4_product<T>(a, (hipStream_t)stream));
   return check_launch("bkg_mx4_matmul");
@@ -711,7 +717,7 @@ extern "C" int bkg_mx4_linear(const void* x, int32_t x_type, int64_t ldx, int64_
     if (const int rc = bkg_mx4_quantize(x, x_type, ldx, m, cols, codes, scales, stream)) return rc;
     return bkg_mx4_matmul(codes, scales, m, b_codes, b_scales, n, cols, bias, out, type, ldo, stream);
   }
-  const Mx4Args a{nullptr, nullptr, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 8,
+  const Mx4Args a{nullptr, nullptr, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0,
                   bias, out, ldo, 0};
   BKG_BY_TYPE(type, (mx4_few_launch<T, false>(a, Mx4X{x, x_type, ldx, (int)cols}, (hipStream_t)stream)));
   return check_launch("bkg_mx4_linear");

@@ -45,6 +45,7 @@ class KGEModule(LightningModule):
         self.valid_metrics = metrics.clone(prefix="val_")
         self.test_metrics = metrics.clone(prefix="test_")
         self._fix_edge_id = None
+        self._teacher = None
 
     def fusion_fn(self, x) -> torch.Tensor:
         """reference kge_module.py:77-84."""
@@ -114,6 +115,8 @@ class KGEModule(LightningModule):
         loss, pos_pred, neg_pred, inverse = ops.kge_bce_loss(z, dec.rel_emb, batch.edge_index, batch.edge_type, neg_edge_index,
                                                              neg_edge_type, dec.kind, reg=1e-2,      # BCE + 1e-2 (mean z^2 + mean rel^2)
                                                              lazy_scores=True)
+        if self._teacher is not None and batch.edge_index.size(1) > 0:
+            loss = loss + self._distillation_term(batch, z)
         # (detached: must not keep the step's autograd graph alive; the positives' scores may still be in the order of the
         # scorer's sorted frame: ``_last_scores`` puts them in the batch's order when somebody reads them)
         self._scores_of_last_step = (z.detach(), pos_pred, neg_pred, inverse)
@@ -135,6 +138,55 @@ class KGEModule(LightningModule):
             self._scores_of_last_step = (z, pos_pred, neg_pred, None)
         return z, pos_pred, neg_pred
 
+
+    # ------------------------------------------------------------------ entity prediction (no counterpart in the reference)
+    def set_teacher(self, teacher, k=10, temperature=1.0, weight=1.0, queries=128):
+        """Distil from ``teacher`` (another :class:`KGEModule` over the same nodes and relations, any width): every training
+        step adds ``weight`` times the distillation loss of ``queries`` random edges of its batch, each predicting its tail and its
+        head out of ALL entities of the batch, against the teacher's ``k`` best entities (:func:`ops.topk_distill_loss`).
+        ``None`` switches it off.  The teacher is frozen and is no part of this module's parameters or state."""
+        if teacher is None:
+            self._teacher = None
+            return
+        for m, who in ((self, "student"), (teacher, "teacher")):
+            if not hasattr(m.model.decoder, "entity_logits"):
+                raise NotImplementedError(f"distillation over entities is implemented for DistMult decoders (the {who}'s is "
+                                          f"{type(m.model.decoder).__name__})")
+        if not (k >= 1 and temperature > 0 and queries >= 1):
+            raise ValueError("set_teacher: k and queries must be at least 1, the temperature positive")
+        teacher.eval().requires_grad_(False)
+        self._teacher = (teacher, int(k), float(temperature), float(weight), int(queries))     # (a tuple: not a submodule)
+
+    @property
+    def has_teacher(self):
+        return self._teacher is not None
+
+    def distillation_loss(self, z, anchor, relation, teacher_ids, teacher_logits, temperature=1.0):
+        """Mean over the queries ``(anchor, relation)`` of the distillation loss against a teacher's best entities
+        ``teacher_ids / teacher_logits [B, K]`` (id -1: no entry); gradients flow into ``z`` and the relation rows."""
+        from . import ops
+        return ops.topk_distill_loss(self.model.decoder.entity_logits(z, anchor, relation), teacher_ids, teacher_logits,
+                                     temperature)
+
+    @torch.no_grad()
+    def top_entities(self, z, anchor, relation, k, table=None):
+        """The ``k`` best entities of each query and their scores, ``([B, k] int64, [B, k] fp32)``.  ``table``:
+        ``ops.mx4_quantize(z)``, made once per set of embeddings -- the queries are then scored against the 4-bit table (an
+        eighth of the bytes of ``z``; its rounding moves scores by a few percent)."""
+        best = torch.topk(self.model.decoder.entity_logits(z, anchor, relation, table=table), min(int(k), z.size(0)), dim=1)
+        return best.indices, best.values
+
+    def _distillation_term(self, batch, z):
+        teacher, k, temperature, weight, queries = self._teacher
+        e = torch.randint(0, batch.edge_index.size(1), (queries,), device=z.device)
+        relation = batch.edge_type[e].repeat(2)
+        anchor = batch.edge_index[:, e].reshape(-1)                  # heads (their tails are asked for), then tails
+        with torch.no_grad():
+            if next(teacher.parameters()).device != z.device:
+                teacher.to(z.device)
+            zt = teacher(batch.x, batch.edge_index, batch.edge_type)
+            ids, logits = teacher.top_entities(zt, anchor, relation, k)
+        return weight * self.distillation_loss(z, anchor, relation, ids, logits, temperature)
 
     def training_step(self, batch, batch_idx=None):
         if getattr(self.model.decoder, "kind", None) is not None:

@@ -45,6 +45,16 @@ class DistMult(Decoder):
     def forward(self, z, edge_index, edge_type):
         return ops.kge_score(z, self.rel_emb, edge_index, edge_type, ops.KGE_DISTMULT)
 
+    def entity_logits(self, z, anchor, relation, table=None):
+        """Scores of the queries ``(anchor, relation)`` against EVERY entity, ``[B, N]`` fp32: ``(z[anchor] * rel_emb[relation])
+        . z[j]`` (DistMult is symmetric: the anchor is the head of a tail query or the tail of a head query).  Differentiable in
+        ``z`` and ``rel_emb``; with ``table`` (``ops.mx4_quantize(z)``) the product runs against the packed table, for inference.
+        No counterpart in the reference, whose decoder scores given triplets only (``biomedkg/model/decoder.py:45-49``)."""
+        q = ops.embedding(z, anchor) * ops.embedding(self.rel_emb, relation)
+        if table is not None:
+            return ops.mx4_linear(q, table, out_dtype=torch.float32)
+        return ops.linear(q, z)
+
 
 class ComplEx(Decoder):
     """Unsupported: the reference's ComplEx assigns a Parameter before ``Module.__init__`` and raises

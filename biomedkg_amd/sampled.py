@@ -158,6 +158,9 @@ class SaintGraphedKge:
         L.require_cuda(x, edge_index, edge_type)
         if getattr(module.model.decoder, "kind", None) is None:
             raise ValueError("the padded step is built on the fused DistMult / TransE loss")
+        if getattr(module, "has_teacher", False):
+            raise ValueError("the padded step holds the reference's loss alone: no distillation from a teacher "
+                             "(KGEModule.set_teacher(None), or the eager training_step)")
         self.module, self.clip, self.graphs_on = module, clip, graphs
         self.neg_ratio = int(module.neg_ratio) if module.neg_ratio else 1
         dev = x.device

@@ -122,9 +122,10 @@ class Trainer:
     def _try_graph(self, model, loader, opt):
         """Whole-graph loaders hand out the SAME batch every step: capture the step once into a hipGraph and replay it
         (biomedkg_amd/graphs.py) when the module's step has no host-side draws (GRACE); otherwise stay eager.  Off with
-        BKG_HIPGRAPH=0, for multi-rank runs (the gradient all-reduce is not part of the capture) and under fast_dev_run."""
+        BKG_HIPGRAPH=0, for multi-rank runs (the gradient all-reduce is not part of the capture), under fast_dev_run and while
+        a KGE module distils from a teacher (the captured steps hold the reference's loss alone)."""
         batch = getattr(loader, "batch", None)
-        if (self.world > 1 or self.fast_dev_run or os.environ.get("BKG_HIPGRAPH", "1") == "0"
+        if (getattr(model, "has_teacher", False) or self.world > 1 or self.fast_dev_run or os.environ.get("BKG_HIPGRAPH", "1") == "0"
                 or self.device.type != "cuda"):
             return None
         from .samplers import SaintBatchLoader

@@ -29,6 +29,10 @@ def build(cfg, config_name):
         model = KGEModule(**cfg.model, num_relation=data_module.data.num_edge_types, neg_ratio=cfg.neg_ratio,
                           node_init_method=cfg.data.node_init_method)
     model.edge_mapping = data_module.edge_map_index
+    teacher = cfg.get("teacher_path") or ""
+    if teacher:      # distil from a trained checkpoint: its best entities per query (teacher_k, teacher_temperature, teacher_weight)
+        model.set_teacher(KGEModule.load_from_checkpoint(teacher), k=cfg.get("teacher_k") or 10,
+                          temperature=cfg.get("teacher_temperature") or 1.0, weight=cfg.get("teacher_weight") or 1.0)
     return data_module, model
 
 
