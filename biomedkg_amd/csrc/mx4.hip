@@ -346,12 +346,18 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
   unsigned char* const ring = lds;
   float* const stage = reinterpret_cast<float*>(lds + 2 * SLOT);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, half = lane >> 5;
-  // block -> (a part of A's tiles, a tile of B): the XCDs take contiguous runs of B's tiles
-  const int per_xcd = (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS, local = blockIdx.x / BKG_XCDS % per_xcd;
-  const int64_t bt = (int64_t)(blockIdx.x % BKG_XCDS) * per_xcd + local;
-  if (bt >= a.n_tiles) return;
-  const int64_t t0 = (int64_t)(blockIdx.x / BKG_XCDS / per_xcd) * a.band, t1 = min(t0 + a.band, (int64_t)a.m_tiles);
-  if (t0 >= t1) return;
+  // block -> (a part of A's tiles, a tile of B): the XCDs take contiguous runs of B's tiles; few tiles go around
+  int64_t bt, part;
+  if (a.n_tiles >= 8 * BKG_XCDS) {
+    const int per_xcd = (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS;
+    bt = (int64_t)(blockIdx.x % BKG_XCDS) * per_xcd + blockIdx.x / BKG_XCDS % per_xcd;
+    part = blockIdx.x / BKG_XCDS / per_xcd;
+  } else {
+    bt = blockIdx.x % a.n_tiles;
+    part = blockIdx.x / a.n_tiles;
+  }
+  const int64_t t0 = part * a.band, t1 = min(t0 + a.band, (int64_t)a.m_tiles);
+  if (bt >= a.n_tiles || t0 >= t1) return;
   const int64_t n0 = bt * 128;
   const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
 
@@ -650,6 +656,12 @@ template <typename T, bool PACKED>
 static void mx4_few_launch(const Mx4Args& a, const Mx4X& x, hipStream_t s) {
   const int64_t tiles = (a.n + 31) / 32;
   const size_t lds = PACKED ? 0 : (size_t)a.steps * (2048 + 128);
+  if (!PACKED) {                                             // (up to 64 panels: more than a kernel gets unasked)
+    static const bool set =
+        hipFuncSetAttribute((const void*)mx4_few_kernel<T, PACKED, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 2176) == hipSuccess &&
+        hipFuncSetAttribute((const void*)mx4_few_kernel<T, PACKED, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 2176) == hipSuccess;
+    (void)set;
+  }
   // a wave per tile keeps the chip busy from 2048 tiles on; below that, and with panels to share, the waves of a block
   if (tiles >= 2048 || a.steps < 4)
     hipLaunchKernelGGL((mx4_few_kernel<T, PACKED, false>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), lds, s, a, x);
@@ -664,7 +676,8 @@ static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
   // parts of A's tiles: so many that two blocks per CU are there
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(a.m_tiles, 512 / a.n_tiles));
   a.band = (int)((a.m_tiles + parts - 1) / parts);
-  const int64_t blocks = (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS * ((a.m_tiles + a.band - 1) / a.band);
+  const int64_t blocks = (int64_t)((a.m_tiles + a.band - 1) / a.band) *
+                         (a.n_tiles >= 8 * BKG_XCDS ? (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS : a.n_tiles);
   static const bool set = hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS>,   // (more than a kernel gets unasked)
                                               hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess;
   (void)set;

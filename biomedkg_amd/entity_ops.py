@@ -5,8 +5,6 @@ re-exported by :mod:`biomedkg_amd.ops`; like everything there they need HIP tens
 """
 from __future__ import annotations
 
-import math
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -197,8 +195,8 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, redu
     if reduction not in ("batchmean", "sum", "none"):
         raise ValueError(f"topk_distill_loss: reduction {reduction!r} (batchmean, sum or none)")
     temp = float(temperature)
-    if not (temp > 0.0 and math.isfinite(temp)):
-        raise ValueError(f"topk_distill_loss: the temperature must be positive and finite, got {temperature}")
+    if not 1e-18 <= temp <= 1e18:
+        raise ValueError(f"topk_distill_loss: the temperature must lie between 1e-18 and 1e18, got {temperature}")
     rows, v = logits.shape
     k = teacher_ids.size(1)
     if not 1 <= k <= 1024:

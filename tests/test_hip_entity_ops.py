@@ -510,7 +510,8 @@ def check_linear(x, w, bias, out_dtype, got=None):
                                    (130, 257, 256), (64, 1000, 768), (300, 70, 1000), (257, 513, 384), (5, 5000, 256),
                                    (129, 128, 2048), (4099, 4100, 1100), (3, 70000, 1025), (33, 5000, 128),
                                    (700, 3000, 100), (200, 1024, 256), (1000, 2049, 250), (8200, 200, 256), (20, 40, 5000),
-                                   (32, 65600, 300), (1, 1, 8192), (2, 600, 4000)])
+                                   (32, 65600, 300), (1, 1, 8192), (2, 600, 4000), (40000, 130, 200),
+                                   (700, 8200, 256)])
 @pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                        (torch.float16, torch.float32), (torch.bfloat16, torch.float16)])
 def test_mx4_linear(m, n, k, dtype, out):
@@ -678,7 +679,7 @@ def test_entity_ops_refuse_bad_calls():
         ops.embedding(w, ids, padding_idx=4)
     with pytest.raises(L.HipLibraryError):
         ops.embedding(w, ids.cpu())
-    for temp in (0.0, -1.0, math.inf, math.nan):
+    for temp in (0.0, -1.0, math.inf, math.nan, 1e-30, 1e30):
         with pytest.raises(ValueError):
             ops.topk_distill_loss(w, tid, tl, temp)
     with pytest.raises(ValueError):
