@@ -2,6 +2,10 @@
 triplets, ``biomedkg/kge_module.py:109-132``): the scaled lookup of table rows with its gradient by sorted ids, the
 distillation loss over the entity logits, and the microscaled 4-bit table a model is served from.  Public names are
 re-exported by :mod:`biomedkg_amd.ops`; like everything there they need HIP tensors and launch on torch's current stream.
+
+All of them can be captured into a graph, backward passes included.  As for every operator under autograd, no eager graph over
+the same leaf tensors may be alive then (a kept loss of a warm-up step): its accumulation nodes belong to the stream they were
+made on, and the capture would be joined with it.
 """
 from __future__ import annotations
 

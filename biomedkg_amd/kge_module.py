@@ -152,8 +152,13 @@ class KGEModule(LightningModule):
             if not hasattr(m.model.decoder, "entity_logits"):
                 raise NotImplementedError(f"distillation over entities is implemented for DistMult decoders (the {who}'s is "
                                           f"{type(m.model.decoder).__name__})")
-        if not (k >= 1 and temperature > 0 and queries >= 1):
-            raise ValueError("set_teacher: k and queries must be at least 1, the temperature positive")
+        if not (1 <= k <= 1024 and 1e-18 <= temperature <= 1e18 and queries >= 1):
+            raise ValueError("set_teacher: k between 1 and 1024, the temperature between 1e-18 and 1e18, at least one query")
+        if teacher is self:
+            raise ValueError("set_teacher: a module is not its own teacher (it would be frozen)")
+        if teacher.model.decoder.rel_emb.size(0) != self.model.decoder.rel_emb.size(0):
+            raise ValueError(f"set_teacher: the teacher knows {teacher.model.decoder.rel_emb.size(0)} relations, the student "
+                             f"{self.model.decoder.rel_emb.size(0)}")
         teacher.eval().requires_grad_(False)
         self._teacher = (teacher, int(k), float(temperature), float(weight), int(queries))     # (a tuple: not a submodule)
 

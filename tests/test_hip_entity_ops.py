@@ -624,6 +624,114 @@ def test_entity_ops_in_a_graph():
         assert float((got[1] - wx.grad).abs().max()) <= 1e-5 * float(wx.grad.abs().max())
 
 
+@pytest.mark.gpu
+def test_entity_ops_in_two_graphs_at_once():
+    """two captured steps replayed side by side on two streams: nothing of one lies in the other's memory"""
+    def make(seed):
+        gen = torch.Generator().manual_seed(seed)
+        w = (0.2 * torch.randn(900, 64, generator=gen)).cuda()
+        many = torch.randint(0, 900, (20000,), generator=gen).cuda()
+        g = torch.randn(20000, 64, generator=gen).cuda()
+        x, tid, tl = make_distill(30, 9000, 6, torch.bfloat16, seed)
+
+        def work():
+            wm, xm = w.detach().requires_grad_(), x.detach().requires_grad_()
+            out = ops.embedding(wm, many, 3.0)
+            out.backward(g)
+            loss = ops.topk_distill_loss(xm, tid, tl, 2.0)
+            loss.backward()
+            return out.detach(), wm.grad, loss.detach(), xm.grad, ops.mx4_linear(w[:50], ops.mx4_quantize(w))
+        return work
+
+    works, graphs, outs, wants = [make(51), make(52)], [], [], []
+    for work in works:
+        wants.append([o.clone() for o in work()])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(work())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for out in outs:
+            for o in out:
+                o.zero_()
+        for s, graph in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        again = works[0]()
+        torch.cuda.synchronize()
+        for got, want in list(zip(outs, wants)) + [(again, wants[0])]:
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_embedding_beyond_32_bits():
+    v, d = 4500000, 512                                      # 2.3e9 values, 4.6 GB
+    w = torch.empty(v, d, dtype=torch.bfloat16, device="cuda").normal_()
+    ids = torch.tensor([v - 1, 0, v - 2, v - 1, 4194303, 4194304, 4194305, v, -1, v - 1], device="cuda")
+    g = torch.randn(10, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    out, dw = run_embedding(w, ids, 1.0, None, g)
+    assert torch.equal(out[[7, 8]], torch.zeros(2, d, dtype=torch.bfloat16, device="cuda"))
+    live = ids[[0, 1, 2, 4, 5, 6]]
+    assert torch.equal(out[[0, 1, 2, 4, 5, 6]], w[live]) and torch.equal(out[3], out[0]) and torch.equal(out[9], out[0])
+    small = torch.tensor([0, 1, 2, 0, 3, 4, 5, 9, 9, 0])     # the same with the live rows side by side
+    want, mag, cnt = plain_embedding_grad(g, small, 6, 1.0, None)
+    h, t = half_step(torch.bfloat16)
+    check(dw[live], want, want.abs() * h + (cnt[:, None] + 4) * U * mag * (1 + h) + t)
+    dw[live] = 0
+    assert not bool(dw.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,v", [(1100, 2000003), (3, 800000001)])
+def test_distill_beyond_32_bits(rows, v):
+    x = torch.empty(rows, v, dtype=torch.bfloat16, device="cuda").normal_()
+    gen = torch.Generator().manual_seed(2)
+    ids, tl = torch.randint(0, v, (rows, 5), generator=gen).cuda(), torch.randn(rows, 5, generator=gen).cuda()
+    ids[-1, 0] = v - 1
+    xx = x.requires_grad_()
+    loss = ops.topk_distill_loss(xx, ids, tl, 1.0, reduction="sum")
+    loss.backward()
+    losses = ops.topk_distill_loss(x.detach(), ids, tl, 1.0, reduction="none")
+    row = x.detach()[-1].double()                            # the last row, in 64 bits on the device
+    lp = row - torch.logsumexp(row, 0)
+    lq = torch.log_softmax(tl[-1].double(), 0)
+    want = float((lq.exp() * (lq - lp[ids[-1]])).sum())
+    span = float(row.max() - row.min())
+    err = U * (3 * span + v / 256 + 42)                      # (distill_bounds; up to v / 256 terms in a thread's chain)
+    assert abs(float(losses[-1]) - want) <= err * (4 + 2 * span + 2 * math.log(v + 1))
+    p = lp.exp()
+    pq = p.clone()
+    p.index_add_(0, ids[-1], -lq.exp())
+    pq.index_add_(0, ids[-1], lq.exp())
+    h, t = half_step(torch.bfloat16)
+    over = (xx.grad[-1].double() - p).abs() - (p.abs() * (h + 4 * U) + 2 * err * pq * (1 + h) + t)
+    assert float(over.max()) <= 0
+
+
+@pytest.mark.gpu
+def test_mx4_beyond_32_bits():
+    n, k = 34000001, 200                                     # 4.4 GB of codes, outputs beyond 2^31 values
+    w = torch.empty(n, k, dtype=torch.bfloat16, device="cuda").normal_()
+    table = ops.mx4_quantize(w)
+    tail = w[-300:].clone()
+    del w
+    want = ops.mx4_quantize(tail)
+    assert torch.equal(table.codes[:, -300:], want.codes) and torch.equal(table.scales[:, -300:], want.scales)
+    x = torch.randn(70, k, generator=torch.Generator().manual_seed(3)).cuda()
+    for m in (2, 70):
+        got = ops.mx4_linear(x[:m], table, out_dtype=torch.bfloat16)
+        check_linear(x[:m], tail, None, torch.bfloat16, got[:, -300:])
+        del got
+    values = ops.mx4_dequantize(table, torch.bfloat16)
+    assert torch.equal(values[-300:], ops.mx4_dequantize(want, torch.bfloat16))
+
+
 # ----------------------------------------------------------------------------- refusals (no GPU needed)
 def test_entity_ops_refuse_cpu_tensors():
     w = torch.randn(4, 8)

@@ -138,6 +138,19 @@ def test_teacher_of_another_width_and_refusals():
         SaintGraphedKge(student, b.x, b.edge_index, b.edge_type, 8, 4, None)
 
 
+def test_set_teacher_refuses():
+    student = module()
+    for bad in (dict(k=0), dict(k=1025), dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=1e-30),
+                dict(queries=0)):
+        with pytest.raises(ValueError):
+            student.set_teacher(module(), **bad)
+    with pytest.raises(ValueError):
+        student.set_teacher(student)
+    with pytest.raises(ValueError):
+        student.set_teacher(module(relations=4))
+    assert not student.has_teacher and all(p.requires_grad for p in student.parameters())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("sampler", ["full", "device"])
 def test_train_kge_distils_from_a_checkpoint(tmp_path, sampler):
