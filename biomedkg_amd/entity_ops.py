@@ -81,9 +81,9 @@ def _embedding_backward(ctx, g):
     g = _rows(g if g.dim() == 2 else g.reshape(n, d))
     dw = g.new_empty((v, d))
     ws_bytes = L.lib().bkg_embed_grad_workspace_bytes(n, d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device) if ws_bytes else None
     L.call("bkg_embed_grad", g.data_ptr(), _TYPE[g.dtype], g.stride(0), d, ids.data_ptr(), ids.dtype == torch.int32, n, v,
-           ctx.pad, ctx.scale, dw.data_ptr(), ws.data_ptr(), ws_bytes, L.stream())
+           ctx.pad, ctx.scale, dw.data_ptr(), L.ptr(ws), ws_bytes, L.stream())
     return dw, None, None, None
 
 

@@ -105,8 +105,26 @@ def test_embedding_gradient_of_long_runs(runs, shuffle):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v,d,n", [(1, 5, 2048), (16, 64, 2047), (17, 1024, 1500), (5000, 768, 2048), (300, 7, 1), (40, 2000, 31),
+                                   (2, 1030, 2), (9000, 1, 700), (70000, 24, 2049)])
+def test_embedding_gradient_of_short_lists(v, d, n, dtype):
+    """one hub takes a third of the ids; some lie outside the table"""
+    gen = torch.Generator().manual_seed(v + d + n)
+    w = torch.randn(v, d, generator=gen).to(dtype).cuda()
+    ids = torch.randint(-1, v + 1, (n,), generator=gen)
+    ids[torch.rand(n, generator=gen) < 0.34] = v // 2
+    for pad in (None, v // 2):
+        g = torch.randn(n, d, generator=gen).to(dtype).cuda()
+        out, dw = run_embedding(w, ids.cuda(), -0.5, pad, g)
+        check_embedding(w, ids, -0.5, pad, g, out, dw)
+        again = run_embedding(w, ids.cuda(), -0.5, pad, g)[1]
+        assert torch.equal(dw, again)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("v", [2, 511, 512, 513, 130000, 262143, 262144, 3000000])
-@pytest.mark.parametrize("n", [8192, 8193, 12288, 50001])
+@pytest.mark.parametrize("n", [2048, 2049, 8192, 8193, 12288, 50001])
 def test_embedding_gradient_over_many_rows(v, n):
     """one, two and three passes of the sort, tables with and without a spare bit above the last row"""
     gen = torch.Generator().manual_seed(v + n)
