@@ -418,7 +418,7 @@ static int kd_parts(int64_t rows, int64_t v, int e) {
 static int kd_check(const char* who, const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t v, int32_t k, int32_t t_type,
                     float temp) {
   BKG_ARG(x && type >= 0 && type <= 2 && t_type >= 0 && t_type <= 2, "bkg_distill: null logits or unknown type");
-  BKG_ARG(rows > 0 && v > 0 && v < (1ll << 30) && ldx >= 0 && rows < (1ll << 24), "bkg_distill: rows in (0, 2^24), columns in (0, 2^30)");
+  BKG_ARG(rows > 0 && v > 0 && v < (1ll << 30) && ldx >= 0 && rows < (1ll << 22), "bkg_distill: rows in (0, 2^22), columns in (0, 2^30)");
   BKG_ARG(k > 0 && k <= KD_MAX_K, "bkg_distill: between 1 and 1024 teacher entries per row");
   BKG_ARG(temp >= 1e-18f && temp <= 1e18f, "bkg_distill: the temperature must lie between 1e-18 and 1e18");
   BKG_ARG((uintptr_t)x % type_bytes(type) == 0, "bkg_distill: misaligned logits");

@@ -603,7 +603,12 @@ template <typename T, int VEC>
 static void embed_rows_launch(const void* w, int64_t ldw, int64_t n_rows, int64_t d, const void* ids, int ids_i32, int64_t n,
                               float scale, void* out, int64_t ldo, hipStream_t s) {
   const int lpr = lanes_log2(d, VEC);
-  const int64_t per_block = (256 >> lpr) * EMBED_UNROLL;
+  const int64_t per_block = (256 >> lpr) * EMBED_UNROLL, most = per_block << 23;     // (a launch has below 2^32 threads)
+  if (n > most) {
+    embed_rows_launch<T, VEC>(w, ldw, n_rows, d, ids, ids_i32, most, scale, out, ldo, s);
+    return embed_rows_launch<T, VEC>(w, ldw, n_rows, d, (const char*)ids + most * (ids_i32 ? 4 : 8), ids_i32, n - most, scale,
+                                     (T*)out + most * ldo, ldo, s);
+  }
   const dim3 grid((unsigned)((n + per_block - 1) / per_block), (unsigned)ceil_div(d, (int64_t)VEC << lpr));
   if (sizeof(T) * VEC == 16 && n * d * (int64_t)sizeof(T) > STREAM_BYTES)
     hipLaunchKernelGGL((embed_rows_kernel<T, VEC, sizeof(T) * VEC == 16>), grid, dim3(256), 0, s, (const T*)w, ldw, n_rows, (int)d,
@@ -710,7 +715,7 @@ extern "C" int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t 
     return check_launch("bkg_embed_grad");
   }
   const int64_t total = n_rows * d * e, n16 = total / 16;
-  BKG_ARG(n16 / 256 < (1ll << 31) - 1, "bkg_embed_grad: table too large for one launch");
+  BKG_ARG(n16 + n < (1ll << 32) - (1 << 20), "bkg_embed_grad: gradient too large for one launch (64 GB)");
   BKG_ARG(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= bkg_embed_grad_workspace_bytes(n, d),
           "bkg_embed_grad: workspace below bkg_embed_grad_workspace_bytes or not 256-byte aligned");
   unsigned char* ws = (unsigned char*)workspace;

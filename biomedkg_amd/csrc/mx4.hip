@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
 // two such products (h = 0, 1): lane half `half` takes the panel's 16-byte piece 2 h + half and byte 2 h + half of its dword
 // of scales.
 // 32 staged result rows of a wave (PITCH floats apart, 16-byte aligned), W columns, as 16-byte stores: LPR lanes a row.
-template <typename T, int W, int PITCH, bool GUARD>
+template <typename T, int W, int PITCH, bool GUARD, bool STREAM>
 __device__ __forceinline__ void mx_store_rows(const float* mine, const float* bias, T* dst, int64_t ldo, int64_t rows_left, int lane) {
   constexpr int VE = 16 / sizeof(T), LPR = W / VE, RPI = 64 / LPR, N = 32 / RPI;
   const int col = (lane % LPR) * VE, row0 = lane / LPR;
@@ -135,7 +135,10 @@ __device__ __forceinline__ void mx_store_rows(const float* mine, const float* bi
     Pack<T, VE> o;
 #pragma unroll
     for (int e = 0; e < VE; ++e) o.v[e] = (T)(v[r][e / 4][e % 4] + bias[e]);
-    if (!GUARD || r * RPI + row0 < rows_left) store16(dst + (r * RPI + row0) * ldo + col, o);
+    if (!GUARD || r * RPI + row0 < rows_left) {
+      if constexpr (STREAM) stream16(dst + (r * RPI + row0) * ldo + col, o);
+      else store16(dst + (r * RPI + row0) * ldo + col, o);
+    }
   }
 }
 
@@ -147,7 +150,19 @@ struct Mx4Args {
   const float* bias;
   void* out; int64_t ldo;
   int wide;                                      // the rows of `out` take aligned 16-byte stores
+  int classes, stream;                           // see mx_class; the result is written past the caches
 };
+
+// Rows of the output whose starts lie at different places of a 128-byte line would be written with two partial lines for every
+// tile's piece.  So a tile takes rows of ONE class r % classes -- `classes` rows further on the start lies at the same place of
+// a line again -- and begins `shift` columns early, where a line does: its pieces are whole lines (1021 x 130000 x 256 in
+// bf16, rows of 2031 lines and 32 bytes: 66 us, without classes 80).
+struct MxClass { int64_t row, rows; int shift; };  // its first row, how many it has, columns a tile begins early
+template <typename T>
+__device__ __forceinline__ MxClass mx_class(const Mx4Args& a, int q) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(static_cast<T*>(a.out) + q * a.ldo);
+  return MxClass{q, (a.m - q + a.classes - 1) / a.classes, a.wide ? (int)(at % 128 / sizeof(T)) : 0};
+}
 
 __device__ __forceinline__ mx_i32x8 mx_operand(mx_i32x4 v) {
   return mx_i32x8{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
@@ -318,7 +333,8 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
     // (a wave's LDS operations complete in order and the area is its own: no barrier)
     const int64_t mr = m0 + wm + 32 * i;
     if (wide) {
-      mx_store_rows<T, WN, PITCH, true>(mine, bias, out + mr * a.ldo + nw, a.ldo, a.m - mr, lane);
+      if (a.stream) mx_store_rows<T, WN, PITCH, true, true>(mine, bias, out + mr * a.ldo + nw, a.ldo, a.m - mr, lane);
+      else mx_store_rows<T, WN, PITCH, true, false>(mine, bias, out + mr * a.ldo + nw, a.ldo, a.m - mr, lane);
     } else {                                                   // the last columns, or rows that are not 16-byte aligned
       const int rows_here = (int)min((int64_t)32, a.m - mr);
       for (int row = 0; row < rows_here; ++row)
@@ -329,64 +345,69 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   }
 }
 
-// Narrow inner dimension (one or two panels: an entity table of up to 256 columns), many outputs: the call is the writing of
-// its outputs.  A block keeps its 128 rows of B in registers (32 at two panels) and walks A's 128-row tiles: tile t + 1
-// travels into the other of two LDS slots while tile t multiplies and its results leave, so loads, products and stores
-// overlap within a block too, and only A moves, out of the L2.  All blocks walk the rows of the output from the top, next to
-// each other: what is written at one time is a band of whole rows, not a column of it -- whole DRAM pages, as far as they go
-// (1021 x 130000 x 256 in bf16: 72 us walking B's tiles past A).
+// Inner dimension of up to six panels (an entity table of up to 768 columns): the call is the writing of its outputs, or close
+// to it.  A block keeps its rows of B in registers (a wave 128 of them, 64 from three panels on) and walks A's 32-row tiles:
+// tile t + 1 travels into the other of two LDS slots while tile t multiplies and its results leave, so loads, products and
+// stores overlap within a block too, and only A moves, out of the L2.  All blocks walk the rows of the output from the top,
+// next to each other: what is written at one time is a band of whole rows, not a column of it -- whole DRAM pages, as far as
+// they go, and few of them (1021 x 130000 x 256 in bf16, packed operands, outputs in turn: 66 us, 265 MB at 4.0 TB/s; with
+// tiles of 128 rows 85; 4096 x 32768 54 us, 5 TB/s, where a fill of that size takes 40).
 //
 // (Dynamic LDS: reading a static array that LDS-DMAs write makes hipcc wait for every copy in flight.)
-constexpr int MS_PITCH = 64 + 4;                           // floats of a staged result row
-constexpr int ms_lds(int steps) { return 2 * steps * (128 * 64 + 128 * 4) + 4 * 32 * MS_PITCH * 4; }
-template <typename T, int STEPS>
+constexpr int MS_ROWS = 32, MS_PITCH = 64 + 4, MS_STEPS = 6;                      // pitch: floats of a staged result row
+constexpr int ms_frags(int steps) { return steps <= 2 ? 4 : 2; }                  // fragments of 32 columns of B that a wave keeps
+constexpr int ms_cols(int steps) { return 4 * 32 * ms_frags(steps); }
+constexpr int ms_slot(int steps) { return steps * MS_ROWS * 64 + (steps + 1) / 2 * 256; }
+constexpr int ms_lds(int steps) { return 2 * ms_slot(steps) + 4 * 32 * MS_PITCH * 4; }
+template <typename T, int STEPS, bool STREAM>
 __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
-  constexpr int SLOT = STEPS * (128 * 64 + 128 * 4), PITCH = MS_PITCH;
+  constexpr int SLOT = ms_slot(STEPS), PITCH = MS_PITCH, NF = ms_frags(STEPS), NP = NF / 2;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   unsigned char* const ring = lds;
   float* const stage = reinterpret_cast<float*>(lds + 2 * SLOT);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, half = lane >> 5;
-  // block -> (a part of A's tiles, a tile of B): the XCDs take contiguous runs of B's tiles; few tiles go around
+  // block -> (a part of A's tiles, a tile of B, a class of rows, next to each other): the XCDs take contiguous runs of B's
+  // tiles; few tiles go around
+  const int64_t n_tiles = (int64_t)a.n_tiles * a.classes;
   int64_t bt, part;
-  if (a.n_tiles >= 8 * BKG_XCDS) {
-    const int per_xcd = (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS;
+  if (n_tiles >= 8 * BKG_XCDS) {
+    const int64_t per_xcd = (n_tiles + BKG_XCDS - 1) / BKG_XCDS;
     bt = (int64_t)(blockIdx.x % BKG_XCDS) * per_xcd + blockIdx.x / BKG_XCDS % per_xcd;
     part = blockIdx.x / BKG_XCDS / per_xcd;
   } else {
-    bt = blockIdx.x % a.n_tiles;
-    part = blockIdx.x / a.n_tiles;
+    bt = blockIdx.x % n_tiles;
+    part = blockIdx.x / n_tiles;
   }
   const int64_t t0 = part * a.band, t1 = min(t0 + a.band, (int64_t)a.m_tiles);
-  if (bt >= a.n_tiles || t0 >= t1) return;
-  const int64_t n0 = bt * 128;
-  const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+  if (bt >= n_tiles || t0 >= t1) return;
+  const MxClass cl = mx_class<T>(a, (int)(bt % a.classes));
+  const int64_t nw = bt / a.classes * ms_cols(STEPS) - cl.shift + wave * 32 * NF;       // the wave's first column
 
-  // copies of a tile: per panel 8 chunks of 16 rows (two a wave) and two of 64 scales (waves 0 and 1: panel 0's, 2 and 3:
-  // panel 1's; with one panel waves 2 and 3 copy it a second time: every wave issues the same number)
-  constexpr int DMAS = 2 * STEPS + 1;
+  // copies of a tile, dealt out to the waves: per panel 2 chunks of 16 rows, and the scales of 2 panels at a time side by side
   auto copy_tile = [&](int64_t tile, int slot) {
-    const int64_t m0 = min(tile, (int64_t)a.m_tiles - 1) * 128;
+    const int64_t m0 = min(tile, (int64_t)a.m_tiles - 1) * MS_ROWS;
     unsigned char* base = ring + slot * SLOT;
 #pragma unroll
-    for (int st = 0; st < STEPS; ++st)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int64_t r = min(m0 + (wave * 2 + j) * 16 + (lane >> 2), a.m - 1);
+    for (int u = 0; u < (2 * STEPS + (STEPS + 1) / 2 + 3) / 4; ++u) {
+      const int i = u * 4 + wave;
+      if (i < 2 * STEPS) {
+        const int64_t r = cl.row + min(m0 + (i & 1) * 16 + (lane >> 2), cl.rows - 1) * a.classes;
         __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(a.ca + (st * a.m + r) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16),
-            (__attribute__((address_space(3))) void*)(base + st * 8192 + (wave * 2 + j) * 1024), 16, 0, 0);
+            (const __attribute__((address_space(1))) void*)(a.ca + ((i >> 1) * a.m + r) * 64 + ((lane & 3) ^ ((lane >> 4) & 3)) * 16),
+            (__attribute__((address_space(3))) void*)(base + i * 1024), 16, 0, 0);
+      } else if (i < 2 * STEPS + (STEPS + 1) / 2) {
+        const int64_t r = cl.row + min(m0 + l31, cl.rows - 1) * a.classes, st = min(2 * (i - 2 * STEPS) + half, STEPS - 1);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.sa + st * a.m + r),
+                                         (__attribute__((address_space(3))) void*)(base + STEPS * 2048 + (i - 2 * STEPS) * 256), 4, 0, 0);
       }
-    const int st = STEPS == 2 ? wave >> 1 : 0;
-    const int64_t r = min(m0 + (wave & 1) * 64 + lane, a.m - 1);
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.sa + st * a.m + r),
-                                     (__attribute__((address_space(3))) void*)(base + STEPS * 8192 + st * 512 + (wave & 1) * 256), 4, 0, 0);
+    }
   };
 
-  mx_i32x4 fb[2][STEPS][2];
-  uint32_t xb[2][STEPS];
+  mx_i32x4 fb[NF][STEPS][2];
+  uint32_t xb[NF][STEPS];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t r = min(n0 + wn + 32 * j + l31, a.n - 1);
+  for (int j = 0; j < NF; ++j) {
+    const int64_t r = max((int64_t)0, min(nw + 32 * j + l31, a.n - 1));
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
       xb[j][st] = a.sb[st * a.n + r] >> (8 * half);
@@ -395,25 +416,35 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
         fb[j][st][h] = *reinterpret_cast<const mx_i32x4*>(a.cb + (st * a.n + r) * 64 + (2 * h + half) * 16);
     }
   }
-  constexpr int VE = 16 / sizeof(T), LPR = 64 / VE, RPI = 64 / LPR, STORES = 2 * 32 / RPI;
-  const int64_t nw = n0 + wn;
-  const bool cols_full = a.wide && nw + 64 <= a.n;
-  const int col = cols_full ? (lane % LPR) * VE : lane;
-  float bias[VE];
+  // the results leave in NP pieces of 64 columns
+  constexpr int VE = 16 / sizeof(T), LPR = 64 / VE, RPI = 64 / LPR, STORES = NP * 32 / RPI;
+  bool full[NP], all_full = true;
+  int col[NP];
+  float bias[NP][VE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) bias[e] = a.bias ? a.bias[min(nw + (cols_full ? col + e : col), a.n - 1)] : 0.f;
+  for (int p = 0; p < NP; ++p) {
+    const int64_t np = nw + 64 * p;
+    full[p] = a.wide && np >= 0 && np + 64 <= a.n;
+    all_full = all_full && full[p];
+    col[p] = full[p] ? (lane % LPR) * VE : lane;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) bias[p][e] = a.bias ? a.bias[max((int64_t)0, min(np + (full[p] ? col[p] + e : col[p]), a.n - 1))] : 0.f;
+  }
   copy_tile(t0, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < NF; ++j)
 #pragma unroll
     for (int st = 0; st < STEPS; ++st)
-      asm volatile("" : "+v"(fb[i][st][0]), "+v"(fb[i][st][1]), "+v"(xb[i][st]));
+      asm volatile("" : "+v"(fb[j][st][0]), "+v"(fb[j][st][1]), "+v"(xb[j][st]));
 #pragma unroll
-  for (int e = 0; e < VE; ++e) asm volatile("" : "+v"(bias[e]));
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int e = 0; e < VE; ++e) asm volatile("" : "+v"(bias[p][e]));
 
   float* mine = stage + wave * 32 * PITCH;
-  T* out = static_cast<T*>(a.out);
+  T* out = static_cast<T*>(a.out) + cl.row * a.ldo;
+  const int64_t ldo = a.ldo * a.classes;
   bool stores_known = false;                               // the last tile's STORES are behind the current tile's copies
   int slot = 0;
   for (int64_t t = t0; t < t1; ++t) {
@@ -423,55 +454,47 @@ __global__ __launch_bounds__(256, 2) void mx4_stream_kernel(const Mx4Args a) {
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();                          // everyone's have, and everyone is done with the other slot
     asm volatile("" ::: "memory");
-    const int64_t mw = t * 128 + wm;
-    const bool wide = cols_full && mw + 64 <= a.m;
+    const int64_t mr = t * MS_ROWS;
     copy_tile(t + 1, slot ^ 1);                            // (past the range: valid memory, never read)
     const unsigned char* base = ring + slot * SLOT;
-    mx_f32x16 acc[2][2];
+    mx_f32x16 acc[NF];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < NF; ++j)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+      for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
-      uint32_t xa[2];
-      mx_i32x4 fa[2][2];
+      const uint32_t xa = *reinterpret_cast<const uint32_t*>(base + STEPS * 2048 + st * 128 + l31 * 4) >> (8 * half);
+      mx_i32x4 fa[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        xa[i] = *reinterpret_cast<const uint32_t*>(base + STEPS * 8192 + st * 512 + (wm + 32 * i + l31) * 4) >> (8 * half);
+      for (int h = 0; h < 2; ++h)
+        fa[h] = *reinterpret_cast<const mx_i32x4*>(base + st * 2048 + l31 * 64 + (((2 * h + half) ^ ((l31 >> 2) & 3)) * 16));
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          fa[i][h] = *reinterpret_cast<const mx_i32x4*>(base + st * 8192 + (wm + 32 * i + l31) * 64 +
-                                                        (((2 * h + half) ^ ((l31 >> 2) & 3)) * 16));
+      for (int j = 0; j < NF; ++j) {
+        acc[j] = mx_mfma<0>(fa[0], fb[j][st][0], acc[j], xa, xb[j][st]);
+        acc[j] = mx_mfma<1>(fa[1], fb[j][st][1], acc[j], xa, xb[j][st]);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          acc[i][j] = mx_mfma<0>(fa[i][0], fb[j][st][0], acc[i][j], xa[i], xb[j][st]);
-          acc[i][j] = mx_mfma<1>(fa[i][1], fb[j][st][1], acc[i][j], xa[i], xb[j][st]);
-        }
     }
+    const bool rows_full = mr + MS_ROWS <= cl.rows;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int p = 0; p < NP; ++p) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mine[(8 * (r >> 2) + 4 * half + (r & 3)) * PITCH + 32 * j + l31] = acc[i][j][r];
-      const int64_t mr = mw + 32 * i;
-      if (wide) {
-        mx_store_rows<T, 64, PITCH, false>(mine, bias, out + mr * a.ldo + nw, a.ldo, 32, lane);
-      } else if (cols_full) {
-        mx_store_rows<T, 64, PITCH, true>(mine, bias, out + mr * a.ldo + nw, a.ldo, a.m - mr, lane);
+        for (int r = 0; r < 16; ++r) mine[(8 * (r >> 2) + 4 * half + (r & 3)) * PITCH + 32 * j + l31] = acc[2 * p + j][r];
+      const int64_t np = nw + 64 * p;
+      if (full[p] && rows_full) {
+        mx_store_rows<T, 64, PITCH, false, STREAM>(mine, bias[p], out + mr * ldo + np, ldo, MS_ROWS, lane);
+      } else if (full[p]) {
+        mx_store_rows<T, 64, PITCH, true, STREAM>(mine, bias[p], out + mr * ldo + np, ldo, cl.rows - mr, lane);
       } else {
-        const int rows_here = (int)min((int64_t)32, a.m - mr);
+        const int rows_here = (int)min((int64_t)MS_ROWS, cl.rows - mr);
+        const int64_t c = np + col[p];
         for (int row = 0; row < rows_here; ++row)
-          if (nw + col < a.n) out[(mr + row) * a.ldo + nw + col] = (T)(mine[row * PITCH + col] + bias[0]);
+          if (c >= 0 && c < a.n) out[(mr + row) * ldo + c] = (T)(mine[row * PITCH + col[p]] + bias[p][0]);
       }
     }
-    stores_known = wide;
+    stores_known = all_full && rows_full;
     slot ^= 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the copies past the range
@@ -572,6 +595,14 @@ __global__ __launch_bounds__(256) void mx4_few_kernel(const Mx4Args a, const Mx4
   }
 }
 
+// Whole lines of a result beyond STREAM_BYTES leave past the caches; a smaller one is found there by whoever reads it next (a
+// 1536 x 130000 product in bf16 and the maximum of its rows: 189 us so, 215 through the caches; 768 rows: 96 and 76).
+template <typename T>
+static bool mx4_past_caches(const Mx4Args& a) {
+  const int64_t row = a.ldo * (int64_t)sizeof(T);
+  return a.wide && row * a.classes % 128 == 0 && a.m * row > STREAM_BYTES;
+}
+
 template <typename T, int MT, int NT, int S>
 static void mx4_launch(Mx4Args a, hipStream_t s) {
   constexpr int LDS = S * (64 * (MT + NT) * 64 + 64 * (MT + NT) * 4);
@@ -580,6 +611,7 @@ static void mx4_launch(Mx4Args a, hipStream_t s) {
   (void)set;
   a.m_tiles = (int)((a.m + 64 * MT - 1) / (64 * MT));
   a.n_tiles = (int)((a.n + 64 * NT - 1) / (64 * NT));
+  a.stream = mx4_past_caches<T>(a);
   // rows of tiles walked together: 8 share panels best; 2 where the output's rows are long, so that what is written at one time
   // is a few whole rows (1021 x 130000 x 768: 127 us with 2, 152 with 8; 8192 x 8192 x 512: 43 and 40)
   a.band = a.n >= (1 << 16) ? 2 : 8;
@@ -608,7 +640,7 @@ extern "C" int bkg_mx4_quantize(const void* x, int32_t type, int64_t ldx, int64_
           "bkg_mx4_quantize: null or misaligned buffer");
   const int pieces = (int)(mx4_steps(cols) * 16);
   const int64_t blocks = (rows * pieces + 255) / 256;
-  BKG_ARG(blocks < (1ll << 31), "bkg_mx4_quantize: table too large for one launch");
+  BKG_ARG(blocks < (1ll << 24), "bkg_mx4_quantize: table too large for one launch");
   const bool al = access_bytes(x, 0, ldx * type_bytes(type)) == 16;
   hipStream_t s = (hipStream_t)stream;
 #define BKG_MX4_Q(AL)                                                                                                       \
@@ -628,7 +660,7 @@ extern "C" int bkg_mx4_dequantize(const void* codes, const void* scales, int64_t
           "bkg_mx4_dequantize: null or misaligned buffer");
   const int pieces = (int)(mx4_steps(cols) * 16);
   const int64_t blocks = (rows * pieces + 255) / 256;
-  BKG_ARG(blocks < (1ll << 31), "bkg_mx4_dequantize: table too large for one launch");
+  BKG_ARG(blocks < (1ll << 24), "bkg_mx4_dequantize: table too large for one launch");
   const bool al = access_bytes(out, 0, ldo * type_bytes(type)) == 16;
   hipStream_t s = (hipStream_t)stream;
 #define BKG_MX4_D(AL)                                                                                                       \
@@ -648,7 +680,7 @@ static int mx4_check_product(int64_t m, int64_t n, int64_t cols, const void* b_c
   BKG_ARG((uintptr_t)b_codes % 16 == 0 && (uintptr_t)b_scales % 4 == 0 && (uintptr_t)out % type_bytes(type) == 0 &&
               (uintptr_t)bias % 4 == 0,
           "bkg_mx4 product: misaligned buffer");
-  BKG_ARG((m + 127) / 128 * ((n + 127) / 128) < (1ll << 31) - 64, "bkg_mx4 product: too many tiles for one launch");
+  BKG_ARG((m <= 32 ? 1 : (m + 127) / 128 + 8) * ((n + 127) / 128 + 1) < (1ll << 24) - 1024, "bkg_mx4 product: too many tiles for one launch");
   return 0;
 }
 
@@ -669,19 +701,38 @@ static void mx4_few_launch(const Mx4Args& a, const Mx4X& x, hipStream_t s) {
     hipLaunchKernelGGL((mx4_few_kernel<T, PACKED, true>), dim3((unsigned)tiles), dim3(256), lds, s, a, x);
 }
 
-template <typename T, int STEPS>
-static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
-  a.m_tiles = (int)((a.m + 127) / 128);
-  a.n_tiles = (int)((a.n + 127) / 128);
-  // parts of A's tiles: so many that two blocks per CU are there
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(a.m_tiles, 512 / a.n_tiles));
-  a.band = (int)((a.m_tiles + parts - 1) / parts);
-  const int64_t blocks = (int64_t)((a.m_tiles + a.band - 1) / a.band) *
-                         (a.n_tiles >= 8 * BKG_XCDS ? (a.n_tiles + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS : a.n_tiles);
-  static const bool set = hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS>,   // (more than a kernel gets unasked)
+template <typename T, int STEPS, bool STREAM>
+static void mx4_stream_launch_as(const Mx4Args& a, unsigned blocks, hipStream_t s) {
+  static const bool set = hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS, STREAM>,
                                               hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess;
   (void)set;
-  hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS>), dim3((unsigned)blocks), dim3(256), ms_lds(STEPS), s, a);
+  hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS, STREAM>), dim3(blocks), dim3(256), ms_lds(STEPS), s, a);
+}
+template <typename T, int STEPS>
+static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
+  // classes of rows (mx_class) where rows are long and every class fills a tile.  Blocks next to each other write the lines that
+  // short rows share at about the same time: 130000 x 1000 in bf16, 256 inner columns, 93 us without classes and 110 with; in
+  // fp32 162 and 132; 32768 x 4008 in bf16 96 and 62.
+  constexpr int64_t LONG_ROW = 4000;                         // bytes
+  const int64_t row = a.ldo * (int64_t)sizeof(T);
+  if (a.wide && row >= LONG_ROW) {
+    while (row * a.classes % 128) a.classes <<= 1;
+    if (a.m < (int64_t)MS_ROWS * a.classes) a.classes = 1;
+  }
+  int64_t early = 0;                                         // columns that tiles begin early, at most
+  for (int q = 0; q < a.classes && a.wide; ++q)
+    early = std::max<int64_t>(early, (int64_t)((uintptr_t)(static_cast<T*>(a.out) + q * a.ldo) % 128 / sizeof(T)));
+  a.stream = mx4_past_caches<T>(a);
+  a.m_tiles = (int)(((a.m + a.classes - 1) / a.classes + MS_ROWS - 1) / MS_ROWS);
+  a.n_tiles = (int)((a.n + early + ms_cols(STEPS) - 1) / ms_cols(STEPS));
+  const int64_t n_tiles = (int64_t)a.n_tiles * a.classes;
+  // parts of A's tiles: so many that two blocks per CU are there
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(a.m_tiles, 512 / n_tiles));
+  a.band = (int)((a.m_tiles + parts - 1) / parts);
+  const int64_t blocks = (int64_t)((a.m_tiles + a.band - 1) / a.band) *
+                         (n_tiles >= 8 * BKG_XCDS ? (n_tiles + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS : n_tiles);
+  if (a.stream) mx4_stream_launch_as<T, STEPS, true>(a, (unsigned)blocks, s);
+  else mx4_stream_launch_as<T, STEPS, false>(a, (unsigned)blocks, s);
 }
 
 // rows of x that a product packs within its one launch: at most 32, and few enough values that every block packs them anew
@@ -690,9 +741,15 @@ static bool mx4_packs_itself(int64_t m, int64_t cols) { return m <= 32 && m * mx
 template <typename T>
 static void mx4_product(const Mx4Args& a, hipStream_t s) {
   if (a.m <= 32) mx4_few_launch<T, true>(a, Mx4X{}, s);
+  // up to six panels: B in registers (1021 x 130000 x 768 in bf16 157 us with 128 x 128 tiles, 124 so; 8192 x 8192 x 768 68 and
+  // 46; 4096 x 4096 x 768 17.4 and 16.5; 130000 x 256 x 768 37 and 29); each class of rows loads it anew.
   else if (a.steps == 1) mx4_stream_launch<T, 1>(a, s);
   else if (a.steps == 2) mx4_stream_launch<T, 2>(a, s);
-  // 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128:
+  else if (a.steps == 3) mx4_stream_launch<T, 3>(a, s);
+  else if (a.steps == 4) mx4_stream_launch<T, 4>(a, s);
+  else if (a.steps == 5) mx4_stream_launch<T, 5>(a, s);
+  else if (a.steps == 6) mx4_stream_launch<T, 6>(a, s);
+  // More: 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128:
   // four slots a block (two blocks on a CU) where tiles are few, two slots (four blocks: one stores while others multiply)
   // from 1024 tiles on (8192 x 8192 x 512: 40 us with two slots, 54 with four)
   else if ((a.m + 255) / 256 * ((a.n + 255) / 256) >= 192 && a.steps >= 8) mx4_launch<T, 4, 4, 4>(a, s);
@@ -707,7 +764,7 @@ extern "C" int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t
   BKG_ARG(a_codes && a_scales && (uintptr_t)a_codes % 16 == 0 && (uintptr_t)a_scales % 4 == 0, "bkg_mx4_matmul: null or misaligned buffer");
   const Mx4Args a{(const unsigned char*)a_codes, (const uint32_t*)a_scales, m, (const unsigned char*)b_codes,
                   (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0, bias, out, ldo,
-                  access_bytes(out, 0, ldo * type_bytes(type)) == 16};
+                  access_bytes(out, 0, ldo * type_bytes(type)) == 16, 1, 0};
   BKG_BY_TYPE(type, mx4_product<T>(a, (hipStream_t)stream));
   return check_launch("bkg_mx4_matmul");
 }
@@ -731,7 +788,7 @@ extern "C" int bkg_mx4_linear(const void* x, int32_t x_type, int64_t ldx, int64_
     return bkg_mx4_matmul(codes, scales, m, b_codes, b_scales, n, cols, bias, out, type, ldo, stream);
   }
   const Mx4Args a{nullptr, nullptr, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0,
-                  bias, out, ldo, 0};
+                  bias, out, ldo, 0, 1, 0};
   BKG_BY_TYPE(type, (mx4_few_launch<T, false>(a, Mx4X{x, x_type, ldx, (int)cols}, (hipStream_t)stream)));
   return check_launch("bkg_mx4_linear");
 }

@@ -205,8 +205,8 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, redu
     k = teacher_ids.size(1)
     if not 1 <= k <= 1024:
         raise ValueError(f"topk_distill_loss: between 1 and 1024 teacher entries per row, got {k}")
-    if v == 0 or v >= 2 ** 30 or rows >= 2 ** 24:
-        raise ValueError("topk_distill_loss: between 1 and 2^30 - 1 columns, below 2^24 rows")
+    if v == 0 or v >= 2 ** 30 or rows >= 2 ** 22:
+        raise ValueError("topk_distill_loss: between 1 and 2^30 - 1 columns, below 2^22 rows")
     if teacher_logits.requires_grad:
         raise ValueError("topk_distill_loss: the teacher's logits are constants (detach them)")
     if rows == 0:

@@ -529,7 +529,8 @@ def check_linear(x, w, bias, out_dtype, got=None):
                                    (129, 128, 2048), (4099, 4100, 1100), (3, 70000, 1025), (33, 5000, 128),
                                    (700, 3000, 100), (200, 1024, 256), (1000, 2049, 250), (8200, 200, 256), (20, 40, 5000),
                                    (32, 65600, 300), (1, 1, 8192), (2, 600, 4000), (40000, 130, 200),
-                                   (700, 8200, 256)])
+                                   (700, 8200, 256), (1100, 1000, 200), (600, 1040, 500), (300, 544, 100), (2100, 1000, 700),
+                                   (4200, 5000, 1100)])
 @pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                        (torch.float16, torch.float32), (torch.bfloat16, torch.float16)])
 def test_mx4_linear(m, n, k, dtype, out):
@@ -538,6 +539,54 @@ def test_mx4_linear(m, n, k, dtype, out):
     w = (torch.randn(n, k, generator=gen) / math.sqrt(k)).to(dtype).cuda()
     bias = torch.randn(n, generator=gen).cuda() if (m + n) % 2 else None
     check_linear(x, w, bias, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,out", [(1100, 130000, 200, torch.float32), (1300, 130008, 400, torch.bfloat16),
+                                       (600, 240016, 100, torch.float16), (9000, 20000, 1100, torch.bfloat16)])
+def test_mx4_linear_of_huge_results(m, n, k, out):
+    """results beyond the caches, rows of every alignment; the product of the held values in 64 bits on the device"""
+    gen = torch.Generator().manual_seed(m + n)
+    x = (torch.randn(m, k, generator=gen) * torch.exp(torch.randn(m, 1, generator=gen))).cuda()
+    w = torch.randn(n, k, generator=gen).cuda()
+    bias = torch.randn(n, generator=gen).cuda()
+    table = ops.mx4_quantize(w)
+    store = torch.full((m + 2, n), 7.0, dtype=out, device="cuda")
+    got = ops.mx4_linear(x, table, bias=bias, out_dtype=out)
+    h, t = half_step(out)
+    xv, wv = ops.mx4_dequantize(ops.mx4_quantize(x)).double(), ops.mx4_dequantize(table).double()
+    for lo in range(0, m, 500):
+        want = xv[lo:lo + 500] @ wv.t() + bias.double()
+        mag = xv[lo:lo + 500].abs() @ wv.abs().t() + bias.double().abs()
+        over = (got[lo:lo + 500].double() - want).abs() - (want.abs() * h + (k + 4) * U * mag * (1 + h) + t)
+        assert float(over.max()) <= 0
+    # through the C entry into the middle of a buffer: nothing beside the rows is written
+    a = ops.mx4_quantize(x)
+    L.call("bkg_mx4_matmul", a.codes_ptr, a.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, k, bias.data_ptr(),
+           store[1].data_ptr(), ops_type(out), n, L.stream())
+    assert torch.equal(store[1:-1], got) and bool((store[[0, -1]] == 7).all())
+
+
+def ops_type(dtype):
+    return TYPES.index(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [200, 700])
+@pytest.mark.parametrize("start,ldo", [(0, 1000), (8, 1008), (24, 1024), (3, 1001), (56, 1016)])
+def test_mx4_matmul_into_a_view(k, start, ldo):
+    """rows of an output with any start and pitch: only the product's places are written"""
+    m, n = 1200, 950
+    gen = torch.Generator().manual_seed(k + start)
+    a, b = ops.mx4_quantize(torch.randn(m, k, generator=gen).cuda()), ops.mx4_quantize(torch.randn(n, k, generator=gen).cuda())
+    want = ops.mx4_linear(a, b, out_dtype=torch.bfloat16)
+    store = torch.full((m * ldo + start + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+    L.call("bkg_mx4_matmul", a.codes_ptr, a.scales_ptr, m, b.codes_ptr, b.scales_ptr, n, k, None, store.data_ptr() + 2 * start, 1,
+           ldo, L.stream())
+    view = store[start:start + m * ldo].view(m, ldo)
+    assert torch.equal(view[:, :n], want)                    # (whatever the tiles, the sums run over the panels in order)
+    view[:, :n] = 7
+    assert bool((store == 7).all())
 
 
 @pytest.mark.gpu
