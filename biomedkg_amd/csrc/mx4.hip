@@ -180,8 +180,10 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(mx_i32x4 a, mx_i32x4 b, mx_f32x16 c
 // t in registers, so slot t is refilled with stage t + S, and the first fragments of stage t + 1 are read while the second
 // half of stage t multiplies.  The ring is retired by counted vmcnt waits: the loop issues nothing but DMAs.
 //
-// The result goes through LDS once (32 rows of a wave at a time) so that rows leave in runs of 16-byte stores: for the
-// narrow inner dimensions of an entity table (256 columns: two panels) writing the outputs is what the call costs.
+// The result goes through LDS once (32 rows of a wave at a time) so that rows leave in runs of 16-byte stores.
+//
+// Bound by power at 256 x 256: a product of random values runs at 1.66 GHz with the matrix units 55 % busy, one of zeros takes
+// two thirds of its time; without copies and LDS reads the products alone would take three quarters.
 template <typename T, int MT, int NT, int S>
 __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(const Mx4Args a) {
   constexpr int BM = 64 * MT, BN = 64 * NT;
@@ -612,9 +614,9 @@ static void mx4_launch(Mx4Args a, hipStream_t s) {
   a.m_tiles = (int)((a.m + 64 * MT - 1) / (64 * MT));
   a.n_tiles = (int)((a.n + 64 * NT - 1) / (64 * NT));
   a.stream = mx4_past_caches<T>(a);
-  // rows of tiles walked together: 8 share panels best; 2 where the output's rows are long, so that what is written at one time
-  // is a few whole rows (1021 x 130000 x 768: 127 us with 2, 152 with 8; 8192 x 8192 x 512: 43 and 40)
-  a.band = a.n >= (1 << 16) ? 2 : 8;
+  // rows of tiles walked together: enough to share panels, few enough that what is written at one time is a few whole rows
+  // (8192 x 16384 x 1024 in bf16: 133 us with 4 or 2, 155 with 8; 8192 x 8192 x 2048: 104 with 4, 108 with 2, 114 with 8)
+  a.band = 4;
   const int64_t total = (int64_t)a.m_tiles * a.n_tiles;
   const unsigned grid = (unsigned)((total + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS);
   hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, S>), dim3(grid), dim3(256), LDS, s, a);
@@ -749,12 +751,11 @@ static void mx4_product(const Mx4Args& a, hipStream_t s) {
   else if (a.steps == 4) mx4_stream_launch<T, 4>(a, s);
   else if (a.steps == 5) mx4_stream_launch<T, 5>(a, s);
   else if (a.steps == 6) mx4_stream_launch<T, 6>(a, s);
-  // More: 256 x 256 tiles where they fill the chip and the inner dimension pays for a block that has a CU to itself; else 128 x 128:
-  // four slots a block (two blocks on a CU) where tiles are few, two slots (four blocks: one stores while others multiply)
-  // from 1024 tiles on (8192 x 8192 x 512: 40 us with two slots, 54 with four)
-  else if ((a.m + 255) / 256 * ((a.n + 255) / 256) >= 192 && a.steps >= 8) mx4_launch<T, 4, 4, 4>(a, s);
-  else if ((a.m + 127) / 128 * ((a.n + 127) / 128) >= 1024) mx4_launch<T, 2, 2, 2>(a, s);
-  else mx4_launch<T, 2, 2, 4>(a, s);
+  // More: 256 x 256 tiles, a block with a CU to itself, where they fill the chip and the inner dimension is long (8192 x 8192 x
+  // 8192 in bf16: 271 us, 4 PFLOP/s, against 316 with 128 x 128; 4096 x 4096 x 4096 42 and 46; x 2048 31 and 31); else 128 x 128,
+  // four blocks on a CU: one stores while others multiply (5000 x 6000 x 1024: 34 us, 256 x 256 44; 2048 x 2048 x 8192 39 and 52).
+  else if ((a.m + 255) / 256 * ((a.n + 255) / 256) >= 192 && a.steps >= 16) mx4_launch<T, 4, 4, 4>(a, s);
+  else mx4_launch<T, 2, 2, 2>(a, s);
 }
 
 extern "C" int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t m, const void* b_codes, const void* b_scales,

@@ -530,7 +530,7 @@ def check_linear(x, w, bias, out_dtype, got=None):
                                    (700, 3000, 100), (200, 1024, 256), (1000, 2049, 250), (8200, 200, 256), (20, 40, 5000),
                                    (32, 65600, 300), (1, 1, 8192), (2, 600, 4000), (40000, 130, 200),
                                    (700, 8200, 256), (1100, 1000, 200), (600, 1040, 500), (300, 544, 100), (2100, 1000, 700),
-                                   (4200, 5000, 1100)])
+                                   (4200, 5000, 1100), (3600, 3500, 2000), (500, 700, 8200)])
 @pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                        (torch.float16, torch.float32), (torch.bfloat16, torch.float16)])
 def test_mx4_linear(m, n, k, dtype, out):
