@@ -324,18 +324,19 @@ __global__ __launch_bounds__(N) void kd_row_kernel(const KdArgs a) {
   if (a.d) kd_write_grad<T, N>(a, xr, static_cast<T*>(a.d) + row * a.ldd, sp, done.rw, a.coef, id_lds, t_lds);
 }
 
-// scale * the sum of the rows' losses, in a fixed order (one block)
-template <int N>
-__device__ __forceinline__ void kd_sum(const float* __restrict__ losses, int64_t n, float scale, float* red, float* __restrict__ out) {
+// scale * the sum of the rows' losses, in a fixed order (one block).  FRESH: written by other blocks of this launch, past the L2
+template <int N, bool FRESH>
+__device__ __forceinline__ void kd_sum(const float* losses, int64_t n, float scale, float* red, float* __restrict__ out) {
   float s = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += N) s += losses[i];
+  for (int64_t i = threadIdx.x; i < n; i += N)
+    s += FRESH ? __hip_atomic_load(losses + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : losses[i];
   s = kd_block_sum(s, red);
   if (threadIdx.x == 0) out[0] = scale * s;
 }
 __global__ __launch_bounds__(1024) void kd_sum_kernel(const float* __restrict__ losses, int64_t n, float scale,
                                                       float* __restrict__ out) {
   __shared__ float red[16];
-  kd_sum<1024>(losses, n, scale, red, out);
+  kd_sum<1024, false>(losses, n, scale, red, out);
 }
 
 // ---- few rows: a.parts blocks share one.  First the parts' statistics ...
@@ -370,21 +371,21 @@ __global__ __launch_bounds__(KD_THREADS) void kd_join_kernel(const KdArgs a) {
   if (p == 0) {
     const float loss = kd_loss(a, xr, id_lds, t_lds, m, s, tm, ts, red);
     if (threadIdx.x == 0) {
-      a.losses[row] = off ? 0.f : loss;
+      __hip_atomic_store(a.losses + row, off ? 0.f : loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       a.rows[row] = rw;
     }
   }
-  if (p == 0 && a.loss) {                        // (which block is the last does not change the sum's order)
+  // Which block is the last does not change the sum's order.  A row's loss goes past the L2 by itself and is waited for: a fence
+  // for the device would write back all that the XCD's L2 holds of the gradients (128 x 130000 in fp32: this launch took 63 us with it, 30 without).
+  if (p == 0 && a.loss) {
     __shared__ bool last;
     if (threadIdx.x == 0) {
-      __threadfence();
-      last = atomicAdd(a.done, 1u) == (unsigned)a.n_rows - 1;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      last = __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)a.n_rows - 1;
+      asm volatile("" ::: "memory");
     }
     __syncthreads();
-    if (last) {
-      __threadfence();
-      kd_sum<KD_THREADS>(a.losses, a.n_rows, a.sum_scale, red, a.loss);
-    }
+    if (last) kd_sum<KD_THREADS, true>(a.losses, a.n_rows, a.sum_scale, red, a.loss);
   }
   if (a.d) {
     const KdSpan<T> sp(xr, a.v, p, a.parts);

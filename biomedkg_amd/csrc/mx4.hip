@@ -528,7 +528,8 @@ __global__ __launch_bounds__(256) void mx4_few_kernel(const Mx4Args a, const Mx4
   if constexpr (!PACKED) {
     const int pieces = a.steps * 16;
     uint32_t* xs = reinterpret_cast<uint32_t*>(lds + a.steps * 2048);
-    for (int p = threadIdx.x; p < 32 * pieces; p += 256) {                  // (32 * pieces is a multiple of 256)
+    // (whole waves, at most 32 rows; what lies in the rows behind them ends in output rows that are not there)
+    for (int p = threadIdx.x; p < (((int)a.m * pieces + 63) & ~63); p += 256) {
       const int row = p / pieces, piece = p - row * pieces, c = piece * 8;
       float f[8];
 #pragma unroll
