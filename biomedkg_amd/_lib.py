@@ -211,19 +211,24 @@ def sref(struct):
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def stream():
     """Raw handle of torch's CURRENT stream on the current device (every launch of the library goes there)."""
     if _raw_stream is not None:          # ~0.3 us instead of ~2 us for the Stream object: it is paid on every launch
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_get_device())
     return torch.cuda.current_stream().cuda_stream
 
 
 def call(name, *args):
     rc = getattr(lib(), name)(*args)
     if rc != 0:
-        raise HipLibraryError(f"{name} failed ({rc}): {lib().bkg_last_error().decode()}")
+        failed(name, rc)
+
+
+def failed(name, rc):
+    raise HipLibraryError(f"{name} failed ({rc}): {lib().bkg_last_error().decode()}")
 
 
 def require_cuda(*tensors):

@@ -15,6 +15,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib as L
 
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ID_I32 = {torch.int64: False, torch.int32: True}
 
 
 def _type_of(t, what):
@@ -30,64 +31,80 @@ def _rows(t):
 
 
 def _ids(t, what):
-    if t.dtype not in (torch.int64, torch.int32):
+    if t.dtype not in _ID_I32:
         raise TypeError(f"{what}: expected int64 or int32, got {t.dtype}")
 
 
 def _on_current_device(what, dev, *others):
     """Everything on one device, the current one: the library launches on its current stream."""
-    if dev.type != "cuda":
-        raise L.HipLibraryError(f"{what}: biomedkg_amd runs on MI355X only: got tensors on {dev} (there is no CPU fallback)")
+    ok = dev.type == "cuda" and dev.index == L._get_device()
     for t in others:
-        if t is not None and t.device != dev:
-            if t.device.type != "cuda":
-                raise L.HipLibraryError(f"{what}: biomedkg_amd runs on MI355X only: got a tensor on {t.device}")
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"{what}: tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()} "
-                         "(use torch.cuda.device)")
+        ok = ok and (t is None or t.device == dev)
+    if not ok:
+        _refuse_devices(what, dev, others)
+
+
+def _refuse_devices(what, dev, others):
+    for d in (dev, *(t.device for t in others if t is not None)):
+        if d.type != "cuda":
+            raise L.HipLibraryError(f"{what}: biomedkg_amd runs on MI355X only: got a tensor on {d} (there is no CPU fallback)")
+        if d != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {d}")
+    raise ValueError(f"{what}: tensors on {dev}, but the current device is cuda:{L._get_device()} (use torch.cuda.device)")
 
 
 # ----------------------------------------------------------------------------- embedding
 def _embed_rows(weight, ids, scale):
-    w = _rows(weight)
-    if not ids.is_contiguous():
-        ids = ids.contiguous()
+    w = weight if weight.is_contiguous() else _rows(weight)
     v, d = w.shape
     out = w.new_empty(ids.shape + (d,))
-    L.call("bkg_embed_rows", w.data_ptr(), _TYPE[w.dtype], w.stride(0), v, d, ids.data_ptr(), ids.dtype == torch.int32,
-           ids.numel(), scale, out.data_ptr(), d, L.stream())
-    return out, ids
+    rc = L.lib().bkg_embed_rows(w.data_ptr(), _TYPE[w.dtype], w.stride(0), v, d, ids.data_ptr(), _ID_I32[ids.dtype], ids.numel(),
+                                scale, out.data_ptr(), d, L.stream())
+    if rc:
+        L.failed("bkg_embed_rows", rc)
+    return out
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, pad):
-        out, ids = _embed_rows(weight, ids, scale)
+        out = _embed_rows(weight, ids, scale)
         ctx.save_for_backward(ids)
-        ctx.scale, ctx.pad, ctx.shape = scale, pad, weight.shape
+        v, d = weight.shape
+        n = ids.numel()
+        lib = L.lib()
+        # (what the backward's call takes beside tensors, made here: autograd's thread starts with cold caches, every lookup there
+        # counts twice.  Addresses are taken there: hooks may have moved what was saved)
+        ctx.call = (lib.bkg_embed_grad, _TYPE[weight.dtype], v, d, n, lib.bkg_embed_grad_workspace_bytes(n, d),
+                    _ID_I32[ids.dtype], pad, scale)
         return out
 
     @staticmethod
     def backward(ctx, g):
-        # (the plain path is once_differentiable's without its wrapping: gradients are recorded only under create_graph)
-        return (_embedding_backward_once if torch.is_grad_enabled() else _embedding_backward)(ctx, g)
+        if torch.is_grad_enabled():      # (the plain path is once_differentiable's without its wrapping)
+            return _embedding_backward_once(ctx, g)
+        (ids,) = ctx.saved_tensors
+        grad, code, v, d, n, ws_bytes, ids_i32, pad, scale = ctx.call
+        if g.dim() != 2 or g.stride() != (d, 1):
+            g = _rows(g.reshape(n, d))
+        dw = g.new_empty((v, d))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device) if ws_bytes else None
+        rc = grad(g.data_ptr(), code, g.stride(0), d, ids.data_ptr(), ids_i32, n, v, pad, scale, dw.data_ptr(),
+                  ws.data_ptr() if ws_bytes else None, ws_bytes, L.stream())
+        if rc:
+            L.failed("bkg_embed_grad", rc)
+        return dw, None, None, None
 
 
-def _embedding_backward(ctx, g):
-    (ids,) = ctx.saved_tensors
-    v, d = ctx.shape
-    n = ids.numel()
-    g = _rows(g if g.dim() == 2 else g.reshape(n, d))
-    dw = g.new_empty((v, d))
-    ws_bytes = L.lib().bkg_embed_grad_workspace_bytes(n, d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=g.device) if ws_bytes else None
-    L.call("bkg_embed_grad", g.data_ptr(), _TYPE[g.dtype], g.stride(0), d, ids.data_ptr(), ids.dtype == torch.int32, n, v,
-           ctx.pad, ctx.scale, dw.data_ptr(), L.ptr(ws), ws_bytes, L.stream())
-    return dw, None, None, None
+_embedding_backward_once = once_differentiable(lambda ctx, g: _Embedding.backward(ctx, g))
 
 
-_embedding_backward_once = once_differentiable(_embedding_backward)
+def _check_embedding(weight, ids):
+    if weight.dim() != 2:
+        raise ValueError(f"embedding: expected a [V, d] table, got {tuple(weight.shape)}")
+    _type_of(weight, "embedding")
+    _ids(ids, "embedding ids")
+    _on_current_device("embedding", weight.device, ids)
 
 
 def embedding(weight, ids, scale=1.0, padding_idx=None):
@@ -98,11 +115,7 @@ def embedding(weight, ids, scale=1.0, padding_idx=None):
 
     The gradient is dense ``[V, d]`` in ``weight``'s type: ids sorted (stable), every row summed in fp32 in the order of its
     positions, rounded once -- bitwise repeatable, no atomics (csrc/embed.hip)."""
-    if weight.dim() != 2:
-        raise ValueError(f"embedding: expected a [V, d] table, got {tuple(weight.shape)}")
-    _type_of(weight, "embedding")
-    _ids(ids, "embedding ids")
-    _on_current_device("embedding", weight.device, ids)
+    _check_embedding(weight, ids)
     v, d = weight.shape
     if v >= 2 ** 31 or ids.numel() >= 2 ** 31 or d > 2 ** 20:
         raise ValueError("embedding: at most 2^31 - 1 rows and ids, 2^20 columns")
@@ -112,24 +125,29 @@ def embedding(weight, ids, scale=1.0, padding_idx=None):
         if not -v <= padding_idx < v:
             raise ValueError(f"embedding: padding_idx {padding_idx} outside the table's {v} rows")
         pad = int(padding_idx) % v
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(weight, ids, scale, pad)
-    return _embed_rows(weight, ids, scale)[0]
+    return _embed_rows(weight, ids, scale)
 
 
 # ----------------------------------------------------------------------------- distillation
 def _distill_forward(x, ids, t, temp, sum_scale, want_sum, d=None):
     rows, v = x.shape
     dev, xt = x.device, _TYPE[x.dtype]
+    lib = L.lib()
     # one buffer: the row statistics (kept for the backward), the rows' losses, the launches' scratch
-    n_ws = L.lib().bkg_distill_workspace_floats(rows, v, xt)
+    n_ws = lib.bkg_distill_workspace_floats(rows, v, xt)
     stats = torch.empty(4 * rows + (rows if want_sum else 0) + n_ws, dtype=torch.float32, device=dev)
     out = torch.empty(() if want_sum else (rows,), dtype=torch.float32, device=dev)
-    base = stats.data_ptr()
-    losses = base + 16 * rows if want_sum else out.data_ptr()
-    L.call("bkg_distill_forward", x.data_ptr(), xt, x.stride(0), rows, v, ids.data_ptr(), ids.dtype == torch.int32, ids.stride(0),
-           t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), temp, sum_scale, base + (20 if want_sum else 16) * rows, base,
-           losses, out.data_ptr() if want_sum else None, L.ptr(d), v, L.stream())
+    base, to = stats.data_ptr(), out.data_ptr()
+    losses, scratch = (base + 16 * rows, base + 20 * rows) if want_sum else (to, base + 16 * rows)
+    rc = lib.bkg_distill_forward(x.data_ptr(), xt, x.stride(0), rows, v, ids.data_ptr(), _ID_I32[ids.dtype], ids.stride(0),
+                                 t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), temp, sum_scale, scratch, base, losses,
+                                 to if want_sum else None, None if d is None else d.data_ptr(), v, L.stream())
+    if rc:
+        L.failed("bkg_distill_forward", rc)
     return out, stats
 
 
@@ -146,33 +164,34 @@ class _TopkDistill(torch.autograd.Function):
             d = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         out, stats = _distill_forward(x, ids, t, temp, sum_scale, want_sum, d)
         ctx.save_for_backward(x, ids, t, stats)
-        ctx.made, ctx.temp, ctx.coef, ctx.g_step = d, temp, temp * sum_scale, int(not want_sum)
+        ctx.made = d
+        # (as for the lookup: what the backward's call takes beside tensors, made here)
+        ctx.call = (L.lib().bkg_distill_backward, _TYPE[x.dtype], _ID_I32[ids.dtype], _TYPE[t.dtype], ids.size(1), temp,
+                    int(not want_sum), temp * sum_scale)
         return out
 
     @staticmethod
     def backward(ctx, g):
-        if not torch.is_grad_enabled():
-            return _distill_backward(ctx, g)
-        # (the gradient depends on the logits too: a second derivative is refused even where g itself records none)
-        return _distill_backward_once(ctx, g if g.requires_grad else g.detach().requires_grad_())
+        if torch.is_grad_enabled():
+            # (the gradient depends on the logits too: a second derivative is refused even where g itself records none)
+            return _distill_backward_once(ctx, g if g.requires_grad else g.detach().requires_grad_())
+        x, ids, t, stats = ctx.saved_tensors
+        d, ctx.made = ctx.made, None
+        grad, xt, ids_i32, tt, k, temp, g_step, coef = ctx.call
+        rows, v = x.shape
+        kept = d is not None and not torch.cuda.is_current_stream_capturing()
+        if not kept:
+            d = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.to(torch.float32).contiguous()
+        rc = grad(x.data_ptr(), xt, x.stride(0), rows, v, ids.data_ptr(), ids_i32, ids.stride(0), t.data_ptr(), tt, t.stride(0),
+                  k, temp, stats.data_ptr(), g.data_ptr(), g_step, coef, kept, d.data_ptr(), v, L.stream())
+        if rc:
+            L.failed("bkg_distill_backward", rc)
+        return d, None, None, None, None, None
 
 
-def _distill_backward(ctx, g):
-    x, ids, t, stats = ctx.saved_tensors
-    rows, v = x.shape
-    d, ctx.made = ctx.made, None
-    kept = d is not None and not torch.cuda.is_current_stream_capturing()
-    if not kept:
-        d = torch.empty(rows, v, dtype=x.dtype, device=x.device)
-    if g.dtype != torch.float32 or not g.is_contiguous():
-        g = g.to(torch.float32).contiguous()
-    L.call("bkg_distill_backward", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, v, ids.data_ptr(), ids.dtype == torch.int32,
-           ids.stride(0), t.data_ptr(), _TYPE[t.dtype], t.stride(0), ids.size(1), ctx.temp, stats.data_ptr(), g.data_ptr(),
-           ctx.g_step, ctx.coef, kept, d.data_ptr(), v, L.stream())
-    return d, None, None, None, None, None
-
-
-_distill_backward_once = once_differentiable(_distill_backward)
+_distill_backward_once = once_differentiable(lambda ctx, g: _TopkDistill.backward(ctx, g))
 
 
 def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, reduction="batchmean"):

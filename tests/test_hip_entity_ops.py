@@ -8,6 +8,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from biomedkg_amd import _lib as L
 from biomedkg_amd import ops
@@ -689,6 +690,41 @@ def test_entity_ops_in_a_graph():
         assert torch.equal(got[0], loss.detach()) and torch.equal(got[2], wm.grad) and torch.equal(got[3], y)
         # (the logits' own product splits its inner dimension with atomics in the backward: not bit-equal)
         assert float((got[1] - wx.grad).abs().max()) <= 1e-5 * float(wx.grad.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_gradients_from_tensors_that_hooks_moved(reduction):
+    """saved tensors that went to the host and back, and a recomputed step: the same gradients, whatever lies where they were"""
+    x, tid, tl = make_distill(9, 5000, 6, torch.bfloat16, 61)
+    x, tid, tl = x[:, :4991], tid.clamp(max=4990)[:, ::2], tl[:, ::2]
+    w = torch.randn(400, 40, generator=torch.Generator().manual_seed(62)).cuda()
+    where = torch.randint(0, 400, (2, 3000), generator=torch.Generator().manual_seed(63)).cuda().t()
+    g = torch.randn(3000, 2, 40, generator=torch.Generator().manual_seed(64)).cuda()
+    up = torch.rand(9, generator=torch.Generator().manual_seed(65)).cuda()
+
+    def step(how):
+        xx, ww = x.detach().clone().requires_grad_(), w.detach().requires_grad_()
+
+        def both(a, b):
+            loss = ops.topk_distill_loss(a * 2, tid.clone(), tl.clone(), 2.0, reduction=reduction)
+            return (loss * up).sum(), ops.embedding(b * 2, where.clone(), 0.5)
+        if how == "host":
+            with torch.autograd.graph.save_on_cpu():
+                loss, out = both(xx, ww)
+        elif how == "again":
+            loss, out = torch.utils.checkpoint.checkpoint(both, xx, ww, use_reentrant=False)
+        else:
+            loss, out = both(xx, ww)
+        junk = [torch.full((n,), 7, dtype=torch.int64, device="cuda") for n in (27, 54, 3000, 6000, 6000, 22460)]
+        torch.autograd.backward([loss, out], [torch.ones_like(loss), g])
+        del junk
+        return loss.detach(), out.detach(), xx.grad, ww.grad
+
+    want = step("plain")
+    for how in ("host", "again"):
+        for a, b in zip(step(how), want):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.gpu
