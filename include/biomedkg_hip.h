@@ -654,7 +654,7 @@ int bkg_embed_rows(const void* w, int32_t type, int64_t ldw, int64_t n_rows, int
                    int64_t n, float scale, void* out, int64_t ldo, void* stream);
 int64_t bkg_embed_grad_workspace_bytes(int64_t n, int64_t d);
 /* dw [n_rows, d] (contiguous, 16-byte aligned; every row is written) = scale * sum of g's rows by id, fp32 sums in position
- * order; ids outside [0, n_rows) and pad (-1: none) add nothing.  workspace: 256-byte aligned. */
+ * order; ids outside [0, n_rows) and pad (-1: none) add nothing.  workspace: 256-byte aligned (n <= 2048: none). */
 int bkg_embed_grad(const void* g, int32_t type, int64_t ldg, int64_t d, const void* ids, int32_t ids_i32, int64_t n,
                    int64_t n_rows, int64_t pad, float scale, void* dw, void* workspace, int64_t workspace_bytes, void* stream);
 /* Distillation from a teacher's k best entries per row (csrc/distill.hip has the formulas).  losses [rows] = the rows' losses,

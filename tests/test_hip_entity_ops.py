@@ -791,6 +791,25 @@ def test_embedding_beyond_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [40, 3000])
+def test_embedding_of_as_many_rows_as_there_may_be(n):
+    v = 2 ** 31 - 1
+    w = torch.zeros(v, 1, dtype=torch.bfloat16, device="cuda")
+    live = torch.tensor([0, 1, 2097151, 2097152, 2 ** 30, 2 ** 30 + 1, v - 2, v - 1], device="cuda")
+    w[live, 0] = torch.arange(1, 9, device="cuda").bfloat16()
+    which = torch.randint(0, 9, (n,), generator=torch.Generator().manual_seed(n)).cuda()
+    ids = torch.cat([live, live.new_tensor([v])])[which]                  # (the last: outside)
+    g = torch.ones(n, 1, dtype=torch.bfloat16, device="cuda")
+    out, dw = run_embedding(w, ids, 2.0, None, g)
+    assert torch.equal(out[:, 0], torch.where(which < 8, 2.0 * (which + 1), 0.0).bfloat16())
+    assert torch.equal(dw[live, 0], (2.0 * torch.bincount(which, minlength=9)[:8]).bfloat16())
+    dw[live] = 0
+    assert not bool(dw.any())
+    with pytest.raises(ValueError):
+        ops.embedding(w.new_empty(1, 1).expand(v + 1, 1), ids)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,v", [(1100, 2000003), (3, 800000001)])
 def test_distill_beyond_32_bits(rows, v):
     x = torch.empty(rows, v, dtype=torch.bfloat16, device="cuda").normal_()
@@ -890,6 +909,9 @@ def test_entity_ops_refuse_bad_calls():
         ops.embedding(w, ids, padding_idx=4)
     with pytest.raises(L.HipLibraryError):
         ops.embedding(w, ids.cpu())
+    many = torch.zeros(2 ** 22, 1, device="cuda")
+    with pytest.raises(ValueError):
+        ops.topk_distill_loss(many, many.long(), many)
     for temp in (0.0, -1.0, math.inf, math.nan, 1e-30, 1e30):
         with pytest.raises(ValueError):
             ops.topk_distill_loss(w, tid, tl, temp)
