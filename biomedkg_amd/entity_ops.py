@@ -306,9 +306,12 @@ def mx4_quantize(x):
     rows, cols = x.shape
     if cols > 2 ** 24 or rows >= 2 ** 31:
         raise ValueError("mx4_quantize: at most 2^24 columns and 2^31 - 1 rows")
-    x = _rows(x.detach())
+    if not x.is_contiguous():
+        x = _rows(x.detach())
     table = Mx4Table._empty(rows, cols, x.device)
-    L.call("bkg_mx4_quantize", x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, table.codes_ptr, table.scales_ptr, L.stream())
+    rc = L.lib().bkg_mx4_quantize(x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, table.codes_ptr, table.scales_ptr, L.stream())
+    if rc:
+        L.failed("bkg_mx4_quantize", rc)
     return table
 
 
@@ -321,8 +324,9 @@ def mx4_dequantize(table, dtype=torch.float32):
     _on_current_device("mx4_dequantize", table.device)
     rows, cols = table.shape
     out = torch.empty(rows, cols, dtype=dtype, device=table.device)
-    L.call("bkg_mx4_dequantize", table.codes_ptr, table.scales_ptr, rows, cols, out.data_ptr(), _TYPE[dtype], cols,
-           L.stream())
+    rc = L.lib().bkg_mx4_dequantize(table.codes_ptr, table.scales_ptr, rows, cols, out.data_ptr(), _TYPE[dtype], cols, L.stream())
+    if rc:
+        L.failed("bkg_mx4_dequantize", rc)
     return out
 
 
@@ -347,18 +351,23 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
         _on_current_device("mx4_linear", table.device, x, bias)
         m = x.shape[0]
         out = torch.empty(m, n, dtype=out_dtype, device=table.device)
-        L.call("bkg_mx4_matmul", x.codes_ptr, x.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.stream())
+        L.call("bkg_mx4_matmul", x.codes_ptr, x.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
+               out.data_ptr(), _TYPE[out_dtype], n, L.stream())
         return out
     xt = _type_of(x, "mx4_linear")
     _on_current_device("mx4_linear", x.device, table, bias)
     if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
-    lead = x.shape[:-1]
-    x2 = _rows(x if x.dim() == 2 else x.reshape(-1, cols))
+    lib = L.lib()
+    x2 = x if x.dim() == 2 else x.reshape(-1, cols)
+    if not x2.is_contiguous():
+        x2 = _rows(x2)
     m = x2.size(0)
-    out = torch.empty(lead + (n,), dtype=out_dtype, device=x.device)
-    ws_bytes = L.lib().bkg_mx4_linear_workspace_bytes(m, cols)
+    out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
+    ws_bytes = lib.bkg_mx4_linear_workspace_bytes(m, cols)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    L.call("bkg_mx4_linear", x2.data_ptr(), xt, x2.stride(0), m, table.codes_ptr, table.scales_ptr, n, cols,
-           L.ptr(bias), out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
+    rc = lib.bkg_mx4_linear(x2.data_ptr(), xt, x2.stride(0), m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
+                            out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
+    if rc:
+        L.failed("bkg_mx4_linear", rc)
     return out
