@@ -44,28 +44,6 @@ static inline int check_launch(const char* what) {
     }                                                                                            \
   } while (0)
 
-// Memory an embedding gradient clears beside its sort.
-struct EmbedZero {
-  uint4* p; int64_t n16;                          // whole 16-byte words
-  unsigned char* tail; int n_tail;                // < 16 bytes behind them
-  uint32_t *pad_keys, *pad_perm; int n_pad;       // the words behind the sorted entries (null: none; <= 256 of them)
-};
-__device__ __forceinline__ void embed_zero(int64_t i, const EmbedZero& z) {
-  if (z.pad_keys && i < z.n_pad) { z.pad_keys[i] = 0xFFFFFFFFu; z.pad_perm[i] = 0u; }
-  if (i < z.n16) z.p[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (i < z.n_tail) z.tail[i] = 0;
-}
-// The sort key of an embedding lookup's id: the id, or n_rows for an entry whose gradient goes nowhere (those come last).
-__device__ __forceinline__ uint32_t embed_key(const void* __restrict__ ids, int ids_i32, int64_t i, int64_t n_rows, int64_t pad) {
-  const int64_t v = ids_i32 ? (int64_t)static_cast<const int32_t*>(ids)[i] : static_cast<const int64_t*>(ids)[i];
-  return (v < 0 || v >= n_rows || v == pad) ? (uint32_t)n_rows : (uint32_t)v;
-}
-// Stable ascending sort of up to EMBED_SMALL_SORT such keys with their positions, in one launch whose other blocks clear
-// `zero` (graph.hip).
-constexpr int64_t EMBED_SMALL_SORT = 8192;
-int embed_small_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, int bits, uint32_t* sorted_keys,
-                     uint32_t* perm, const EmbedZero& zero, hipStream_t s);
-
 static inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Deterministic mode (bkg_set_deterministic_workspace): the split-K weight-gradient products write one [M, N] slab per

@@ -26,6 +26,23 @@ __device__ __forceinline__ int64_t embed_id(const void* __restrict__ ids, int id
   return ids_i32 ? (int64_t)static_cast<const int32_t*>(ids)[i] : static_cast<const int64_t*>(ids)[i];
 }
 
+// Memory the gradient clears beside its sort.
+struct EmbedZero {
+  uint4* p; int64_t n16;                           // whole 16-byte words
+  unsigned char* tail; int n_tail;                 // < 16 bytes behind them
+  uint32_t *pad_keys, *pad_perm; int n_pad;        // the words behind the sorted entries
+};
+__device__ __forceinline__ void embed_zero(int64_t i, const EmbedZero& z) {
+  if (i < z.n_pad) { z.pad_keys[i] = 0xFFFFFFFFu; z.pad_perm[i] = 0u; }
+  if (i < z.n16) z.p[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (i < z.n_tail) z.tail[i] = 0;
+}
+// The sort key of an id: the id, or n_rows for an entry whose gradient goes nowhere (those come last).
+__device__ __forceinline__ uint32_t embed_key(const void* __restrict__ ids, int ids_i32, int64_t i, int64_t n_rows, int64_t pad) {
+  const int64_t v = embed_id(ids, ids_i32, i);
+  return (v < 0 || v >= n_rows || v == pad) ? (uint32_t)n_rows : (uint32_t)v;
+}
+
 constexpr int EMBED_UNROLL = 4;
 
 // A lane group of 2^lpr_log2 lanes copies a row's VEC-wide columns of tile blockIdx.y; UNROLL rows in flight per group.
@@ -249,7 +266,7 @@ __global__ __launch_bounds__(512) void embed_grad_finish_kernel(const EmbedGradA
 // ---- up to EF_IDS ids: one launch.  A block owns some rows of the table and a tile of its columns: it looks through ALL ids,
 // keeps those of its rows (in LDS, a word each: the row above the position), clears the rows meanwhile, sorts what it kept -- a
 // few words, unless there is a hub -- and sums: its lane groups take equal parts of the sorted entries, and a run that crosses
-// such parts is joined from partial rows in LDS, in order.  No scratch memory, no other launch.  Against the four launches
+// such parts is joined from partial rows in LDS, in order.  No scratch memory, no other launch.  Against the three launches
 // below, on the chip: 13.0 us to 22.0 for 2048 ids of 5000 rows, 768 in fp32 (1021 ids: 11.2), 14.4 to 26.2 for 2048 ids of
 // 130000 rows, 256 in bf16; all ids equal, the worst case: 24.5 to 28.2 and 30.3 to 29.4.  Tiles of 32 lanes (512 bytes of a
 // row) spread a hub over more CUs than 64 (36.9 us), and clear whole pieces of rows better than 16 (uniform ids 14.9).
@@ -418,6 +435,82 @@ __global__ __launch_bounds__(EF_THREADS) void embed_grad_few_kernel(const EmbedF
   }
 }
 
+// ---- up to ES_SMALL ids: one workgroup sorts in LDS, in stable passes over SS_BITS-bit digits -- its waves take neighbouring
+// entries 64 at a time, lanes with equal digits find each other by ballots -- while the blocks behind it clear the gradient.
+// (Positions behind n carry all-ones keys: they start last and stay last.)  Whole gradient of 8192 ids of 130000 rows, 256 in bf16: 33 us,
+// 48 with the device library's block sort; with the launches of longer lists below 42.
+constexpr int ES_SMALL = 8192, SS_THREADS = 1024, SS_WAVES = SS_THREADS / 64, SS_BITS = 6, SS_DIGITS = 1 << SS_BITS;
+static_assert(SS_WAVES * SS_DIGITS == SS_THREADS, "a thread per counter");
+template <int ITEMS>
+__global__ __launch_bounds__(SS_THREADS) void embed_small_sort_kernel(const void* __restrict__ ids, int ids_i32, int n, int64_t n_rows,
+                                                                      int64_t pad, int bits, uint32_t* __restrict__ sorted_keys,
+                                                                      uint32_t* __restrict__ perm, const EmbedZero zero) {
+  __shared__ uint32_t key_lds[SS_THREADS * ITEMS];
+  __shared__ uint16_t val_lds[SS_THREADS * ITEMS];
+  __shared__ uint32_t seen[SS_WAVES][SS_DIGITS], wave_sums[SS_WAVES];
+  if (blockIdx.x > 0) {
+    embed_zero((int64_t)(blockIdx.x - 1) * SS_THREADS + threadIdx.x, zero);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = wave * 64 * ITEMS + lane;
+  uint32_t key[ITEMS], place[ITEMS];
+  uint16_t val[ITEMS];
+#pragma unroll
+  for (int u = 0; u < ITEMS; ++u) {
+    const int i = i0 + u * 64;
+    key[u] = i < n ? embed_key(ids, ids_i32, i, n_rows, pad) : 0xFFFFFFFFu;
+    val[u] = (uint16_t)i;
+  }
+  for (int shift = 0; shift < bits; shift += SS_BITS) {
+    (&seen[0][0])[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const uint32_t digit = (key[u] >> shift) & (SS_DIGITS - 1);
+      uint64_t peers = ~0ull;
+#pragma unroll
+      for (int b = 0; b < SS_BITS; ++b) {
+        const uint64_t set = __ballot((digit >> b) & 1u);
+        peers &= ((digit >> b) & 1u) ? set : ~set;
+      }
+      const uint32_t first = seen[wave][digit], ahead = __popcll(peers & ((1ull << lane) - 1));     // (a wave's LDS operations
+      place[u] = first + ahead;                                                                     // complete in order)
+      asm volatile("" ::: "memory");
+      if (ahead == 0) seen[wave][digit] = first + __popcll(peers);
+      asm volatile("" ::: "memory");
+    }
+    __syncthreads();
+    // where each (digit, wave)'s entries go: exclusive prefix sums over the counters, a thread each
+    const uint32_t count = seen[threadIdx.x % SS_WAVES][threadIdx.x / SS_WAVES];
+    uint32_t at = count;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t up = __shfl_up((int)at, o, 64);
+      if (lane >= o) at += up;
+    }
+    if (lane == 63) wave_sums[wave] = at;
+    __syncthreads();
+    at -= count;
+    for (int w = 0; w < wave; ++w) at += wave_sums[w];
+    seen[threadIdx.x % SS_WAVES][threadIdx.x / SS_WAVES] = at;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const uint32_t to = seen[wave][(key[u] >> shift) & (SS_DIGITS - 1)] + place[u];
+      key_lds[to] = key[u];
+      val_lds[to] = val[u];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) { key[u] = key_lds[i0 + u * 64]; val[u] = val_lds[i0 + u * 64]; }
+  }
+#pragma unroll
+  for (int u = 0; u < ITEMS; ++u) {
+    const int i = i0 + u * 64;
+    if (i < n) { sorted_keys[i] = key[u]; perm[i] = val[u]; }
+  }
+}
+
 // ---- the sort of longer id lists: stable radix passes over ES_BITS-bit digits, (key, position) pairs.  A block counts its
 // ES_TILE entries' digits (the first pass makes the keys from the ids); a block per digit turns the counts into offsets; the
 // third launch ranks the tile's entries -- its waves take 64 neighbouring entries at a time, lanes with equal digits find
@@ -563,7 +656,7 @@ static int64_t round256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 static int es_blocks(int64_t n) { return (int)((n + ES_TILE - 1) / ES_TILE); }
 // two more pairs of arrays to pass through, the counts and the totals
 static int64_t embed_sort_bytes(int64_t n) {
-  return n <= EMBED_SMALL_SORT ? 0 : 2 * round256(4 * n) + round256(4 * (int64_t)ES_DIGITS * (es_blocks(n) + 1));
+  return n <= ES_SMALL ? 0 : 2 * round256(4 * n) + round256(4 * (int64_t)ES_DIGITS * (es_blocks(n) + 1));
 }
 
 // Stable ascending sort of the ids' keys with their positions; `zero` is cleared beside it.
@@ -571,7 +664,16 @@ static int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, i
                       unsigned char* ws, const EmbedZero& zero, hipStream_t s) {
   int bits = 1;
   while (bits < 32 && (1ull << bits) <= (uint64_t)n_rows) ++bits;      // (keys go up to n_rows itself)
-  if (n <= EMBED_SMALL_SORT) return embed_small_sort(ids, ids_i32, n, n_rows, pad, bits, keys, perm, zero, s);
+  if (n <= ES_SMALL) {
+    const unsigned blocks = (unsigned)(1 + (zero.n16 + SS_THREADS) / SS_THREADS);
+    if (n <= ES_SMALL / 2)
+      hipLaunchKernelGGL(embed_small_sort_kernel<4>, dim3(blocks), dim3(SS_THREADS), 0, s, ids, ids_i32, (int)n, n_rows, pad, bits,
+                         keys, perm, zero);
+    else
+      hipLaunchKernelGGL(embed_small_sort_kernel<8>, dim3(blocks), dim3(SS_THREADS), 0, s, ids, ids_i32, (int)n, n_rows, pad, bits,
+                         keys, perm, zero);
+    return check_launch("bkg_embed_grad: sort");
+  }
   uint32_t* other_keys = (uint32_t*)ws;
   uint32_t* other_perm = (uint32_t*)(ws + round256(4 * n));
   uint32_t* counts = (uint32_t*)(ws + 2 * round256(4 * n));

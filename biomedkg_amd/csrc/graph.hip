@@ -114,36 +114,6 @@ __global__ void role_incidence_keys_kernel(const int64_t* __restrict__ head, con
   vals[i] = oth | ((uint32_t)rel[t] << 24);
 }
 
-// small_sort_kernel for the ids of an embedding lookup (csrc/embed.hip): up to 1024 * IPT ids in one launch (positions behind n carry all-ones keys); the blocks
-// behind the first clear the gradient the sort is for
-template <int IPT>
-__global__ __launch_bounds__(1024) void embed_small_sort_kernel(const void* __restrict__ ids, int ids_i32, int n, int64_t n_rows,
-                                                                int64_t pad, int bits, uint32_t* __restrict__ sorted_keys,
-                                                                uint32_t* __restrict__ perm, const EmbedZero zero) {
-  using sort_t = rocprim::block_radix_sort<uint32_t, 1024, IPT, uint32_t>;
-  __shared__ typename sort_t::storage_type storage;
-  if (blockIdx.x > 0) {
-    embed_zero((int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, zero);
-    return;
-  }
-  uint32_t keys[IPT], vals[IPT];
-#pragma unroll
-  for (int i = 0; i < IPT; ++i) {
-    const int idx = threadIdx.x * IPT + i;
-    keys[i] = idx < n ? embed_key(ids, ids_i32, idx, n_rows, pad) : 0xFFFFFFFFu;
-    vals[i] = (uint32_t)idx;
-  }
-  sort_t().sort(keys, vals, storage, 0, bits);
-#pragma unroll
-  for (int i = 0; i < IPT; ++i) {
-    const int idx = threadIdx.x * IPT + i;
-    if (idx < n) {
-      sorted_keys[idx] = keys[i];
-      perm[idx] = vals[i];
-    }
-  }
-}
-
 __global__ void lower_bound_kernel(const uint32_t* __restrict__ sorted, int64_t n, int64_t n_q, uint32_t stride,
                                    int32_t* __restrict__ out) {
   int64_t s = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -447,25 +417,6 @@ static int sort_edges_impl(const int64_t* lo, const int64_t* hi, int64_t n_lo, i
     hipLaunchKernelGGL(lower_bound_kernel, grid1(n_q), dim3(256), 0, s, sorted_keys, n, n_q, stride, rowptr);
   return check_launch("bkg_sort_edges");
 }
-
-namespace bkg {
-int embed_small_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, int64_t pad, int bits, uint32_t* sorted_keys,
-                     uint32_t* perm, const EmbedZero& zero, hipStream_t s) {
-  static_assert(EMBED_SMALL_SORT == SMALL_SORT_MAX, "one launch up to the one-workgroup sort's size");
-  // (a position behind n must stay behind every real key in the sorted bits: its low bits are all ones, and a real key
-  // that has them too comes before it because the sort is stable)
-  const unsigned blocks = (unsigned)(1 + (zero.n16 + 1024) / 1024);
-#define BKG_EMBED_SORT_LAUNCH(IPT)                                                                                         \
-  hipLaunchKernelGGL(embed_small_sort_kernel<IPT>, dim3(blocks), dim3(1024), 0, s, ids, ids_i32, (int)n, n_rows, pad, bits, \
-                     sorted_keys, perm, zero)
-  if (n <= 1024) BKG_EMBED_SORT_LAUNCH(1);
-  else if (n <= 2048) BKG_EMBED_SORT_LAUNCH(2);
-  else if (n <= 4096) BKG_EMBED_SORT_LAUNCH(4);
-  else BKG_EMBED_SORT_LAUNCH(8);
-#undef BKG_EMBED_SORT_LAUNCH
-  return check_launch("bkg_embed_grad: sort and clear");
-}
-}  // namespace bkg
 
 extern "C" int bkg_sort_edges(const int64_t* lo, const int64_t* hi, int64_t n_lo, int64_t n_hi, int64_t n,
                               uint32_t* keys_tmp, uint32_t* iota_tmp, uint32_t* sorted_keys, uint32_t* perm,
