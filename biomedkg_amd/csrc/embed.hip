@@ -518,6 +518,9 @@ __global__ __launch_bounds__(SS_THREADS) void embed_small_sort_kernel(const void
 // A million ids below 130001 take two passes: 68 us, the clearing of the 66 MB gradient in bf16 included.
 constexpr int ES_BITS = 9, ES_DIGITS = 1 << ES_BITS, ES_THREADS = 1024, ES_WAVES = ES_THREADS / 64, ES_ITEMS = 2;
 constexpr int ES_TILE = ES_THREADS * ES_ITEMS;     // (100003 ids: whole gradient of 8 columns 37 us, 43 with 4 items; 4M: 273, 260)
+// Up to so many blocks, each adds up the counts of all by itself, without the launch between (whole gradient of 8 columns: 30000
+// ids 30 us, 32 with it; 131072 ids 43 and 45; 500000 ids 97 and 81).
+constexpr int ES_FEW_BLOCKS = 64;
 static_assert(ES_THREADS >= ES_DIGITS, "a thread per digit computes where the digit begins");
 
 struct EmbedSort {
@@ -526,8 +529,8 @@ struct EmbedSort {
   uint32_t *key_out, *val_out;
   int64_t n;
   int n_blocks, shift;
-  uint32_t* counts;                                    // [ES_DIGITS][n_blocks]
-  uint32_t* totals;                                    // [ES_DIGITS]
+  uint32_t* counts;                                    // [ES_DIGITS][n_blocks]; few blocks: [n_blocks][ES_DIGITS]
+  uint32_t* totals;                                    // [ES_DIGITS] (null: few blocks)
 };
 __device__ __forceinline__ uint32_t es_key(const EmbedSort& a, int64_t i) {
   return a.ids ? embed_key(a.ids, a.ids_i32, i, a.n_rows, a.pad) : a.key_in[i];
@@ -553,7 +556,8 @@ __global__ __launch_bounds__(ES_THREADS) void embed_count_kernel(const EmbedSort
   for (int r = 0; r < ES_ITEMS; ++r)
     if (i0 + r * ES_THREADS + threadIdx.x < a.n) atomicAdd(&count[(k[r] >> a.shift) & (ES_DIGITS - 1)], 1u);
   __syncthreads();
-  for (int d = threadIdx.x; d < ES_DIGITS; d += ES_THREADS) a.counts[(int64_t)d * a.n_blocks + blockIdx.x] = count[d];
+  for (int d = threadIdx.x; d < ES_DIGITS; d += ES_THREADS)
+    a.counts[a.totals ? (int64_t)d * a.n_blocks + blockIdx.x : (int64_t)blockIdx.x * ES_DIGITS + d] = count[d];
 }
 
 // block d: the counts of digit d become their exclusive prefix sums over the blocks; totals[d] their sum
@@ -602,7 +606,20 @@ __global__ __launch_bounds__(ES_THREADS) void embed_scatter_kernel(const EmbedSo
   // where each digit begins: the totals' exclusive prefix sums (threads 0 .. ES_DIGITS - 1), plus this block's offset
   uint32_t start = 0;
   {
-    const uint32_t v = threadIdx.x < ES_DIGITS ? a.totals[threadIdx.x] : 0u;
+    uint32_t v = 0u, before = 0u;                      // the digit's total; its entries in the blocks before this one
+    if (threadIdx.x < ES_DIGITS) {
+      if (a.totals) {
+        v = a.totals[threadIdx.x];
+        before = a.counts[(int64_t)threadIdx.x * a.n_blocks + blockIdx.x];
+      } else {
+#pragma unroll 8
+        for (int b = 0; b < a.n_blocks; ++b) {
+          const uint32_t c = a.counts[b * ES_DIGITS + threadIdx.x];
+          v += c;
+          before += b < (int)blockIdx.x ? c : 0u;
+        }
+      }
+    }
     uint32_t s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -612,8 +629,7 @@ __global__ __launch_bounds__(ES_THREADS) void embed_scatter_kernel(const EmbedSo
     if (lane == 63) wave_sums[wave] = s;
     __syncthreads();
     for (int w = 0; w < wave; ++w) start += wave_sums[w];
-    start += s - v;
-    if (threadIdx.x < ES_DIGITS) start += a.counts[(int64_t)threadIdx.x * a.n_blocks + blockIdx.x];
+    start += s - v + before;
   }
 #pragma unroll
   for (int r = 0; r < ES_ITEMS; ++r) {
@@ -679,6 +695,7 @@ static int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, i
   uint32_t* counts = (uint32_t*)(ws + 2 * round256(4 * n));
   EmbedSort a{ids, ids_i32, n_rows, pad, nullptr, nullptr, nullptr, nullptr, n, es_blocks(n), 0, counts,
               counts + (int64_t)ES_DIGITS * es_blocks(n)};
+  if (a.n_blocks <= ES_FEW_BLOCKS) a.totals = nullptr;
   const int passes = (bits + ES_BITS - 1) / ES_BITS;
   for (int p = 0; p < passes; ++p) {                                   // the last pass ends in keys / perm
     const bool to_result = (passes - 1 - p) % 2 == 0;
@@ -687,7 +704,7 @@ static int embed_sort(const void* ids, int ids_i32, int64_t n, int64_t n_rows, i
     a.shift = p * ES_BITS;
     const unsigned clear = p == 0 ? (unsigned)((zero.n16 + ES_THREADS) / ES_THREADS) : 0u;
     hipLaunchKernelGGL(embed_count_kernel, dim3(a.n_blocks + clear), dim3(ES_THREADS), 0, s, a, zero);
-    hipLaunchKernelGGL(embed_offsets_kernel, dim3(ES_DIGITS), dim3(256), 0, s, a.counts, a.n_blocks, a.totals);
+    if (a.totals) hipLaunchKernelGGL(embed_offsets_kernel, dim3(ES_DIGITS), dim3(256), 0, s, a.counts, a.n_blocks, a.totals);
     hipLaunchKernelGGL(embed_scatter_kernel, dim3(a.n_blocks), dim3(ES_THREADS), 0, s, a);
     a.ids = nullptr;
     a.key_in = a.key_out;

@@ -125,7 +125,7 @@ def test_embedding_gradient_of_short_lists(v, d, n, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("v", [2, 511, 512, 513, 130000, 262143, 262144, 3000000])
-@pytest.mark.parametrize("n", [2048, 2049, 4096, 4097, 8192, 8193, 12288, 50001])
+@pytest.mark.parametrize("n", [2048, 2049, 4096, 4097, 8192, 8193, 12288, 50001, 131072, 131073])
 def test_embedding_gradient_over_many_rows(v, n):
     """one, two and three passes of the sort, tables with and without a spare bit above the last row"""
     gen = torch.Generator().manual_seed(v + n)
