@@ -170,8 +170,9 @@ SIGNATURES = {
     "bkg_distill_backward": (I32, [P, I32, I64, I64, I64, P, I32, I64, P, I32, I64, I32, F32, P, P, I32, F32, I32, P, I64, P]),
     "bkg_mx4_quantize": (I32, [P, I32, I64, I64, I64, P, P, P]),
     "bkg_mx4_dequantize": (I32, [P, P, I64, I64, P, I32, I64, P]),
-    "bkg_mx4_matmul": (I32, [P, P, I64, P, P, I64, I64, P, P, I32, I64, P]),
-    "bkg_mx4_linear_workspace_bytes": (I64, [I64, I64]),
+    "bkg_mx4_matmul_workspace_bytes": (I64, [I64, I64, I64]),
+    "bkg_mx4_matmul": (I32, [P, P, I64, P, P, I64, I64, P, P, I32, I64, P, I64, P]),
+    "bkg_mx4_linear_workspace_bytes": (I64, [I64, I64, I64]),
     "bkg_mx4_linear": (I32, [P, I32, I64, I64, P, P, I64, I64, P, P, I32, I64, P, I64, P]),
 }
 

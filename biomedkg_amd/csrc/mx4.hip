@@ -151,6 +151,7 @@ struct Mx4Args {
   void* out; int64_t ldo;
   int wide;                                      // the rows of `out` take aligned 16-byte stores
   int classes, stream;                           // see mx_class; the result is written past the caches
+  int slices;                                    // (tiles) parts of the panels; more than one: fp32 sums [slice][m][ldo] in `out`
 };
 
 // Rows of the output whose starts lie at different places of a 128-byte line would be written with two partial lines for every
@@ -193,11 +194,13 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, half = lane >> 5;
 
-  // tile order: each XCD takes a contiguous part of the list; the list runs through `band` tiles of rows at a time, so the
-  // tiles in flight on one XCD share their panels in its L2
-  const int64_t total = (int64_t)a.m_tiles * a.n_tiles, per = (total + BKG_XCDS - 1) / BKG_XCDS;
-  const int64_t t = (int64_t)(blockIdx.x % BKG_XCDS) * per + blockIdx.x / BKG_XCDS;
-  if (blockIdx.x / BKG_XCDS >= per || t >= total) return;
+  // tile order: each XCD takes a contiguous part of the list (slice after slice of the panels); the list runs through `band`
+  // tiles of rows at a time, so the tiles in flight on one XCD share their panels in its L2
+  const int64_t tiles = (int64_t)a.m_tiles * a.n_tiles, total = tiles * a.slices, per = (total + BKG_XCDS - 1) / BKG_XCDS;
+  const int64_t ts = (int64_t)(blockIdx.x % BKG_XCDS) * per + blockIdx.x / BKG_XCDS;
+  if (blockIdx.x / BKG_XCDS >= per || ts >= total) return;
+  const int64_t slice = ts / tiles, t = ts - slice * tiles;
+  const int per_slice = (a.steps + a.slices - 1) / a.slices, k0 = (int)slice * per_slice, steps = min(per_slice, a.steps - k0);
   const int64_t in_band = a.band * (int64_t)a.n_tiles, band = t / in_band, at = t - band * in_band;
   const int band_m = (int)min((int64_t)a.band, a.m_tiles - band * a.band);
   const int64_t m0 = (band * a.band + at % band_m) * BM, n0 = at / band_m * BN;
@@ -215,7 +218,7 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
 #pragma unroll
   for (int j = 0; j < CH / 4; ++j) ssrc[j] = min(r0 + ((wave & 1) * (CH / 4) + j) * 64 + lane, rows - 1);
   auto copy = [&](int stage, int slot, int j) {              // copy j of this wave's DMAS of a stage
-    const int64_t k = min(stage, a.steps - 1);               // (past the end: valid memory, never read)
+    const int64_t k = min(k0 + stage, a.steps - 1);          // (past the end: valid memory, never used)
     unsigned char* base = lds + slot * STAGE;
     if (j < CH)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(codes + k * rows * 64 + src[j]),
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   read_scales(0, sn);
   pin(f0, sn);
   int slot = 0;
-  for (int st = 0; st < a.steps; ++st) {
+  for (int st = 0; st < steps; ++st) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) sc.a[i] = sn.a[i] >> (8 * half);
 #pragma unroll
@@ -314,7 +317,7 @@ __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(co
   constexpr int WN = 32 * NT, PITCH = WN + 4;                  // floats
   float* mine = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
   static_assert(4 * 32 * PITCH * 4 <= S * STAGE, "the results' staging area lies in the ring");
-  T* out = static_cast<T*>(a.out);
+  T* out = static_cast<T*>(a.out) + slice * a.m * a.ldo;
   constexpr int VE = 16 / sizeof(T), LPR = WN / VE;          // elements per store, lanes per row
   const int64_t nw = n0 + wn;                                  // the wave's first column
   const bool wide = a.wide && nw + WN <= a.n;
@@ -606,6 +609,20 @@ static bool mx4_past_caches(const Mx4Args& a) {
   return a.wide && row * a.classes % 128 == 0 && a.m * row > STREAM_BYTES;
 }
 
+// The slices' sums, added in order, with the bias: a thread per four columns of a row (ld: the sums' rows, a multiple of 4).
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__ sums, int slices, int64_t m, int64_t n, int64_t ld,
+                                                       const float* __restrict__ bias, T* __restrict__ out, int64_t ldo) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / (ld / 4), c = (at - row * (ld / 4)) * 4;
+  if (row >= m) return;
+  mx_f32x4 s = *reinterpret_cast<const mx_f32x4*>(sums + row * ld + c);
+#pragma unroll 4
+  for (int i = 1; i < slices; ++i) s += *reinterpret_cast<const mx_f32x4*>(sums + (i * m + row) * ld + c);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j < n) out[row * ldo + c + j] = (T)(s[j] + (bias ? bias[c + j] : 0.f));
+}
+
 template <typename T, int MT, int NT, int S>
 static void mx4_launch(Mx4Args a, hipStream_t s) {
   constexpr int LDS = S * (64 * (MT + NT) * 64 + 64 * (MT + NT) * 4);
@@ -618,7 +635,7 @@ static void mx4_launch(Mx4Args a, hipStream_t s) {
   // rows of tiles walked together: enough to share panels, few enough that what is written at one time is a few whole rows
   // (8192 x 16384 x 1024 in bf16: 133 us with 4 or 2, 155 with 8; 8192 x 8192 x 2048: 104 with 4, 108 with 2, 114 with 8)
   a.band = 4;
-  const int64_t total = (int64_t)a.m_tiles * a.n_tiles;
+  const int64_t total = (int64_t)a.m_tiles * a.n_tiles * a.slices;
   const unsigned grid = (unsigned)((total + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS);
   hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, S>), dim3(grid), dim3(256), LDS, s, a);
 }
@@ -741,8 +758,37 @@ static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
 // rows of x that a product packs within its one launch: at most 32, and few enough values that every block packs them anew
 static bool mx4_packs_itself(int64_t m, int64_t cols) { return m <= 32 && m * mx4_steps(cols) * MX_K <= 8192; }
 
+// Parts of a long inner dimension (32 panels or more) for a product of so few 128 x 128 tiles that most CUs would have none: as
+// many as fill them, eight panels or more each; a second launch adds their sums in order.  33 x 5000 x 8192 in bf16: 15 us, 36 in
+// one part; 8192 x 16 x 8192 20 and 39; 500 x 500 x 4096 15 and 19; 4096 x 64 x 4096 16 and 16.  1024 x 2048 x 2048 (128 tiles)
+// took 20 instead of 11.  1: not worth it, or another kernel's (see mx4_product).
+static int mx4_slices(int64_t m, int64_t n, int64_t cols) {
+  const int64_t tiles = (m + 127) / 128 * ((n + 127) / 128), steps = mx4_steps(cols);
+  if (m <= 32 || n <= 0 || steps < 32 || tiles > 64) return 1;
+  const int64_t want = std::min<int64_t>(256 / tiles, steps / 8), per = (steps + want - 1) / want;
+  return (int)((steps + per - 1) / per);                     // (every slice has a panel)
+}
+static int64_t mx4_sums_bytes(int64_t m, int64_t n, int64_t cols) {
+  const int slices = mx4_slices(m, n, cols);
+  return slices == 1 ? 0 : slices * m * ((n + 3) / 4 * 4) * 4;
+}
+
 template <typename T>
-static void mx4_product(const Mx4Args& a, hipStream_t s) {
+static void mx4_product(const Mx4Args& a, float* sums, int64_t cols, hipStream_t s) {
+  const int slices = mx4_slices(a.m, a.n, cols);
+  if (slices > 1) {
+    Mx4Args b = a;
+    b.bias = nullptr;
+    b.out = sums;
+    b.ldo = (a.n + 3) / 4 * 4;
+    b.wide = 1;                                              // (the workspace is 16-byte aligned)
+    b.slices = slices;
+    mx4_launch<float, 2, 2, 2>(b, s);
+    const int64_t threads = a.m * (b.ldo / 4);
+    hipLaunchKernelGGL((mx4_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, sums, slices, a.m, a.n, b.ldo,
+                       a.bias, (T*)a.out, a.ldo);
+    return;
+  }
   if (a.m <= 32) mx4_few_launch<T, true>(a, Mx4X{}, s);
   // up to six panels: B in registers (1021 x 130000 x 768 in bf16 157 us with 128 x 128 tiles, 124 so; 8192 x 8192 x 768 68 and
   // 46; 4096 x 4096 x 768 17.4 and 16.5; 130000 x 256 x 768 37 and 29); each class of rows loads it anew.
@@ -759,20 +805,30 @@ static void mx4_product(const Mx4Args& a, hipStream_t s) {
   else mx4_launch<T, 2, 2, 2>(a, s);
 }
 
+extern "C" int64_t bkg_mx4_matmul_workspace_bytes(int64_t m, int64_t n, int64_t cols) {
+  return m <= 0 || n <= 0 || cols <= 0 ? 0 : mx4_sums_bytes(m, n, cols);
+}
+
 extern "C" int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t m, const void* b_codes, const void* b_scales,
-                              int64_t n, int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* stream) {
+                              int64_t n, int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
   if (const int rc = mx4_check_product(m, n, cols, b_codes, b_scales, bias, out, type, ldo)) return rc;
   if (m == 0 || n == 0) return 0;
   BKG_ARG(a_codes && a_scales && (uintptr_t)a_codes % 16 == 0 && (uintptr_t)a_scales % 4 == 0, "bkg_mx4_matmul: null or misaligned buffer");
+  const int64_t need = mx4_sums_bytes(m, n, cols);
+  BKG_ARG(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
+          "bkg_mx4_matmul: workspace below bkg_mx4_matmul_workspace_bytes or misaligned");
   const Mx4Args a{(const unsigned char*)a_codes, (const uint32_t*)a_scales, m, (const unsigned char*)b_codes,
                   (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0, bias, out, ldo,
-                  access_bytes(out, 0, ldo * type_bytes(type)) == 16, 1, 0};
-  BKG_BY_TYPE(type, mx4_product<T>(a, (hipStream_t)stream));
+                  access_bytes(out, 0, ldo * type_bytes(type)) == 16, 1, 0, 1};
+  BKG_BY_TYPE(type, mx4_product<T>(a, (float*)workspace, cols, (hipStream_t)stream));
   return check_launch("bkg_mx4_matmul");
 }
 
-extern "C" int64_t bkg_mx4_linear_workspace_bytes(int64_t m, int64_t cols) {
-  return m <= 0 || cols <= 0 || mx4_packs_itself(m, cols) ? 0 : mx4_steps(cols) * m * 68;
+// the packed rows, then the slices' sums
+static int64_t mx4_packed_bytes(int64_t m, int64_t cols) { return (mx4_steps(cols) * m * 68 + 255) & ~(int64_t)255; }
+extern "C" int64_t bkg_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t cols) {
+  return m <= 0 || n <= 0 || cols <= 0 || mx4_packs_itself(m, cols) ? 0 : mx4_packed_bytes(m, cols) + mx4_sums_bytes(m, n, cols);
 }
 
 extern "C" int bkg_mx4_linear(const void* x, int32_t x_type, int64_t ldx, int64_t m, const void* b_codes, const void* b_scales,
@@ -782,15 +838,16 @@ extern "C" int bkg_mx4_linear(const void* x, int32_t x_type, int64_t ldx, int64_
   if (m == 0 || n == 0) return 0;
   BKG_ARG(x && x_type >= 0 && x_type <= 2 && (uintptr_t)x % type_bytes(x_type) == 0, "bkg_mx4_linear: null or misaligned x");
   if (!mx4_packs_itself(m, cols)) {
-    BKG_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= bkg_mx4_linear_workspace_bytes(m, cols),
+    BKG_ARG(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= bkg_mx4_linear_workspace_bytes(m, n, cols),
             "bkg_mx4_linear: workspace below bkg_mx4_linear_workspace_bytes or misaligned");
     unsigned char* codes = (unsigned char*)workspace;
     unsigned char* scales = codes + mx4_steps(cols) * m * 64;
     if (const int rc = bkg_mx4_quantize(x, x_type, ldx, m, cols, codes, scales, stream)) return rc;
-    return bkg_mx4_matmul(codes, scales, m, b_codes, b_scales, n, cols, bias, out, type, ldo, stream);
+    return bkg_mx4_matmul(codes, scales, m, b_codes, b_scales, n, cols, bias, out, type, ldo, codes + mx4_packed_bytes(m, cols),
+                          workspace_bytes - mx4_packed_bytes(m, cols), stream);
   }
   const Mx4Args a{nullptr, nullptr, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0,
-                  bias, out, ldo, 0, 1, 0};
+                  bias, out, ldo, 0, 1, 0, 1};
   BKG_BY_TYPE(type, (mx4_few_launch<T, false>(a, Mx4X{x, x_type, ldx, (int)cols}, (hipStream_t)stream)));
   return check_launch("bkg_mx4_linear");
 }

@@ -351,8 +351,10 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
         _on_current_device("mx4_linear", table.device, x, bias)
         m = x.shape[0]
         out = torch.empty(m, n, dtype=out_dtype, device=table.device)
+        ws_bytes = L.lib().bkg_mx4_matmul_workspace_bytes(m, n, cols)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=table.device) if ws_bytes else None
         L.call("bkg_mx4_matmul", x.codes_ptr, x.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
-               out.data_ptr(), _TYPE[out_dtype], n, L.stream())
+               out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
         return out
     xt = _type_of(x, "mx4_linear")
     _on_current_device("mx4_linear", x.device, table, bias)
@@ -364,7 +366,7 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
         x2 = _rows(x2)
     m = x2.size(0)
     out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
-    ws_bytes = lib.bkg_mx4_linear_workspace_bytes(m, cols)
+    ws_bytes = lib.bkg_mx4_linear_workspace_bytes(m, n, cols)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
     rc = lib.bkg_mx4_linear(x2.data_ptr(), xt, x2.stride(0), m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
                             out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())

@@ -676,11 +676,14 @@ int bkg_distill_backward(const void* x, int32_t type, int64_t ldx, int64_t rows,
 int bkg_mx4_quantize(const void* x, int32_t type, int64_t ldx, int64_t rows, int64_t cols, void* codes, void* scales, void* stream);
 int bkg_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int32_t type, int64_t ldo,
                        void* stream);
-/* out [m, n] = A B^T (+ bias [n]) over two packed tables of the same width, fp32 sums, one rounding into `type` */
+/* out [m, n] = A B^T (+ bias [n]) over two packed tables of the same width, fp32 sums, one rounding into `type`; workspace:
+ * 16-byte aligned (0 bytes but for small products of a long inner dimension) */
+int64_t bkg_mx4_matmul_workspace_bytes(int64_t m, int64_t n, int64_t cols);
 int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t m, const void* b_codes, const void* b_scales, int64_t n,
-                   int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* stream);
+                   int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                   void* stream);
 /* The same product with x [m, cols] (x_type) packed within the call; workspace: 16-byte aligned (0 bytes for a few rows). */
-int64_t bkg_mx4_linear_workspace_bytes(int64_t m, int64_t cols);
+int64_t bkg_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t cols);
 int bkg_mx4_linear(const void* x, int32_t x_type, int64_t ldx, int64_t m, const void* b_codes, const void* b_scales, int64_t n,
                    int64_t cols, const float* bias, void* out, int32_t type, int64_t ldo, void* workspace,
                    int64_t workspace_bytes, void* stream);

@@ -531,7 +531,9 @@ def check_linear(x, w, bias, out_dtype, got=None):
                                    (700, 3000, 100), (200, 1024, 256), (1000, 2049, 250), (8200, 200, 256), (20, 40, 5000),
                                    (32, 65600, 300), (1, 1, 8192), (2, 600, 4000), (40000, 130, 200),
                                    (700, 8200, 256), (1100, 1000, 200), (600, 1040, 500), (300, 544, 100), (2100, 1000, 700),
-                                   (4200, 5000, 1100), (3600, 3500, 2000), (500, 700, 8200)])
+                                   (4200, 5000, 1100), (3600, 3500, 2000), (500, 700, 8200), (33, 5000, 8192), (64, 30, 4000), (8000, 17, 1100),
+                                   (900, 1100, 1030), (40, 129, 1025), (8000, 17, 4097),
+                                   (100, 3, 8320), (1000, 1000, 4100)])
 @pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                        (torch.float16, torch.float32), (torch.bfloat16, torch.float16)])
 def test_mx4_linear(m, n, k, dtype, out):
@@ -564,7 +566,7 @@ def test_mx4_linear_of_huge_results(m, n, k, out):
     # through the C entry into the middle of a buffer: nothing beside the rows is written
     a = ops.mx4_quantize(x)
     L.call("bkg_mx4_matmul", a.codes_ptr, a.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, k, bias.data_ptr(),
-           store[1].data_ptr(), ops_type(out), n, L.stream())
+           store[1].data_ptr(), ops_type(out), n, None, 0, L.stream())
     assert torch.equal(store[1:-1], got) and bool((store[[0, -1]] == 7).all())
 
 
@@ -573,17 +575,22 @@ def ops_type(dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("k", [200, 700])
+@pytest.mark.parametrize("k", [200, 700, 1300, 4200])
 @pytest.mark.parametrize("start,ldo", [(0, 1000), (8, 1008), (24, 1024), (3, 1001), (56, 1016)])
 def test_mx4_matmul_into_a_view(k, start, ldo):
     """rows of an output with any start and pitch: only the product's places are written"""
-    m, n = 1200, 950
+    m, n = (1200, 950) if k < 4000 else (650, 950)
     gen = torch.Generator().manual_seed(k + start)
     a, b = ops.mx4_quantize(torch.randn(m, k, generator=gen).cuda()), ops.mx4_quantize(torch.randn(n, k, generator=gen).cuda())
     want = ops.mx4_linear(a, b, out_dtype=torch.bfloat16)
     store = torch.full((m * ldo + start + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(L.lib().bkg_mx4_matmul_workspace_bytes(m, n, k), dtype=torch.uint8, device="cuda")
     L.call("bkg_mx4_matmul", a.codes_ptr, a.scales_ptr, m, b.codes_ptr, b.scales_ptr, n, k, None, store.data_ptr() + 2 * start, 1,
-           ldo, L.stream())
+           ldo, L.ptr(ws), ws.numel(), L.stream())
+    if ws.numel():
+        with pytest.raises(L.HipLibraryError):
+            L.call("bkg_mx4_matmul", a.codes_ptr, a.scales_ptr, m, b.codes_ptr, b.scales_ptr, n, k, None,
+                   store.data_ptr() + 2 * start, 1, ldo, L.ptr(ws), ws.numel() - 1, L.stream())
     view = store[start:start + m * ldo].view(m, ldo)
     assert torch.equal(view[:, :n], want)                    # (whatever the tiles, the sums run over the panels in order)
     view[:, :n] = 7
