@@ -245,7 +245,7 @@ class Mx4Table:
     with zeros): ``codes`` uint8 ``[panels, rows, 64]`` (two columns a byte, the lower one in the low nibble) and ``scales``
     uint8 ``[panels, rows, 4]`` (the exponent of each 32 columns + 127; 255: the block held an infinity or NaN).  0.53 bytes a
     value."""
-    __slots__ = ("shape", "device", "codes_ptr", "scales_ptr", "_store")
+    __slots__ = ("shape", "_store")
 
     def __init__(self, codes, scales, shape):
         self.shape = tuple(shape)
@@ -258,26 +258,38 @@ class Mx4Table:
             raise ValueError(f"Mx4Table: codes on {codes.device}, scales on {scales.device}")
         if codes.data_ptr() % 16 or scales.data_ptr() % 4:
             raise ValueError("Mx4Table: codes must be 16-byte, scales 4-byte aligned")
-        self.device, self.codes_ptr, self.scales_ptr = codes.device, codes.data_ptr(), scales.data_ptr()
         self._store = (codes, scales)
 
     @classmethod
     def _empty(cls, rows, cols, device):
         """An unwritten table in one piece of memory: the codes, then the scales."""
         self = cls.__new__(cls)
-        panels = (cols + 127) // 128
-        self._store = torch.empty(panels * rows * 68, dtype=torch.uint8, device=device)
-        self.shape, self.device = (rows, cols), device
-        self.codes_ptr = self._store.data_ptr()
-        self.scales_ptr = self.codes_ptr + panels * rows * 64
+        self._store = torch.empty((cols + 127) // 128 * rows * 68, dtype=torch.uint8, device=device)
+        self.shape = (rows, cols)
         return self
 
+    def __reduce__(self):
+        """Copies and saved tables (``copy``, ``pickle``, ``torch.save``) are made from the memory and the shape."""
+        if self._store.__class__ is tuple:
+            return Mx4Table, (*self._store, self.shape)
+        return _table_in_one_piece, (self._store, self.shape)
+
     def _parts(self):
-        if not isinstance(self._store, tuple):
-            rows, panels = self.shape[0], (self.shape[1] + 127) // 128
-            cut = panels * rows * 64
-            self._store = (self._store[:cut].view(panels, rows, 64), self._store[cut:].view(panels, rows, 4))
-        return self._store
+        store = self._store
+        if store.__class__ is tuple:
+            return store
+        rows, panels = self.shape[0], (self.shape[1] + 127) // 128
+        cut = panels * rows * 64
+        return store[:cut].view(panels, rows, 64), store[cut:].view(panels, rows, 4)
+
+    def _addresses(self):
+        """Where the codes and the scales lie.  (Asked of the memory at every call: a number kept beside it would go along into
+        a copy, whose memory is another.)"""
+        store = self._store
+        if store.__class__ is tuple:
+            return store[0].data_ptr(), store[1].data_ptr()
+        base = store.data_ptr()
+        return base, base + (self.shape[1] + 127) // 128 * self.shape[0] * 64
 
     @property
     def codes(self):
@@ -288,11 +300,33 @@ class Mx4Table:
         return self._parts()[1]
 
     @property
+    def codes_ptr(self):
+        return self._addresses()[0]
+
+    @property
+    def scales_ptr(self):
+        return self._addresses()[1]
+
+    @property
+    def device(self):
+        return (self._store[0] if self._store.__class__ is tuple else self._store).device
+
+    @property
     def nbytes(self):
         return (self.shape[1] + 127) // 128 * self.shape[0] * 68
 
     def __repr__(self):
         return f"Mx4Table({self.shape[0]} x {self.shape[1]}, {self.nbytes} bytes, {self.device})"
+
+
+def _table_in_one_piece(store, shape):
+    rows, cols = shape
+    if store.dtype != torch.uint8 or store.shape != ((cols + 127) // 128 * rows * 68,) or not store.is_contiguous() \
+            or store.data_ptr() % 16:
+        raise ValueError(f"Mx4Table: no packed table of {tuple(shape)}")
+    self = Mx4Table.__new__(Mx4Table)
+    self.shape, self._store = (rows, cols), store
+    return self
 
 
 def mx4_quantize(x):
@@ -309,7 +343,8 @@ def mx4_quantize(x):
     if not x.is_contiguous():
         x = _rows(x.detach())
     table = Mx4Table._empty(rows, cols, x.device)
-    rc = L.lib().bkg_mx4_quantize(x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, table.codes_ptr, table.scales_ptr, L.stream())
+    codes, scales = table._addresses()
+    rc = L.lib().bkg_mx4_quantize(x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, codes, scales, L.stream())
     if rc:
         L.failed("bkg_mx4_quantize", rc)
     return table
@@ -324,7 +359,8 @@ def mx4_dequantize(table, dtype=torch.float32):
     _on_current_device("mx4_dequantize", table.device)
     rows, cols = table.shape
     out = torch.empty(rows, cols, dtype=dtype, device=table.device)
-    rc = L.lib().bkg_mx4_dequantize(table.codes_ptr, table.scales_ptr, rows, cols, out.data_ptr(), _TYPE[dtype], cols, L.stream())
+    codes, scales = table._addresses()
+    rc = L.lib().bkg_mx4_dequantize(codes, scales, rows, cols, out.data_ptr(), _TYPE[dtype], cols, L.stream())
     if rc:
         L.failed("bkg_mx4_dequantize", rc)
     return out
@@ -341,6 +377,7 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     n, cols = table.shape
     if bias is not None and (bias.shape != (n,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise ValueError(f"mx4_linear: bias must be contiguous fp32 [{n}]")
+    codes, scales = table._addresses()
     packed = isinstance(x, Mx4Table)
     if (x.shape[-1] if len(x.shape) else -1) != cols:
         raise ValueError(f"mx4_linear: x {tuple(x.shape)} against a table of {cols} columns")
@@ -353,7 +390,7 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
         out = torch.empty(m, n, dtype=out_dtype, device=table.device)
         ws_bytes = L.lib().bkg_mx4_matmul_workspace_bytes(m, n, cols)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=table.device) if ws_bytes else None
-        L.call("bkg_mx4_matmul", x.codes_ptr, x.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
+        L.call("bkg_mx4_matmul", *x._addresses(), m, codes, scales, n, cols, L.ptr(bias),
                out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
         return out
     xt = _type_of(x, "mx4_linear")
@@ -368,7 +405,7 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
     ws_bytes = lib.bkg_mx4_linear_workspace_bytes(m, n, cols)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    rc = lib.bkg_mx4_linear(x2.data_ptr(), xt, x2.stride(0), m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
+    rc = lib.bkg_mx4_linear(x2.data_ptr(), xt, x2.stride(0), m, codes, scales, n, cols, L.ptr(bias),
                             out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
     if rc:
         L.failed("bkg_mx4_linear", rc)
