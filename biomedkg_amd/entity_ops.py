@@ -10,6 +10,7 @@ made on, and the capture would be joined with it.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -51,6 +52,16 @@ def _refuse_devices(what, dev, others):
         if d != dev:
             raise ValueError(f"{what}: tensors on {dev} and {d}")
     raise ValueError(f"{what}: tensors on {dev}, but the current device is cuda:{L._get_device()} (use torch.cuda.device)")
+
+
+def _refuse_tangents(what, *tensors):
+    """Forward-mode derivatives are not implemented: an input that carries one is refused, whether or not a gradient is recorded
+    (an autograd function refuses it by itself, but a call that records nothing does not go through one)."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:        # (outside every dual_level no tensor carries one)
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 
 # ----------------------------------------------------------------------------- embedding
@@ -103,6 +114,7 @@ def _check_embedding(weight, ids):
     if weight.dim() != 2:
         raise ValueError(f"embedding: expected a [V, d] table, got {tuple(weight.shape)}")
     _type_of(weight, "embedding")
+    _refuse_tangents("embedding", weight)
     _ids(ids, "embedding ids")
     _on_current_device("embedding", weight.device, ids)
 
@@ -214,6 +226,7 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, redu
     _type_of(logits, "topk_distill_loss logits")
     _type_of(teacher_logits, "topk_distill_loss teacher logits")
     _ids(teacher_ids, "topk_distill_loss teacher ids")
+    _refuse_tangents("topk_distill_loss", logits, teacher_logits)
     _on_current_device("topk_distill_loss", logits.device, teacher_ids, teacher_logits)
     if reduction not in ("batchmean", "sum", "none"):
         raise ValueError(f"topk_distill_loss: reduction {reduction!r} (batchmean, sum or none)")
@@ -385,6 +398,7 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     if out_dtype not in _TYPE:
         raise TypeError(f"mx4_linear: out_dtype float32, bfloat16 or float16, got {out_dtype}")
     if packed:
+        _refuse_tangents("mx4_linear", bias)
         _on_current_device("mx4_linear", table.device, x, bias)
         m = x.shape[0]
         out = torch.empty(m, n, dtype=out_dtype, device=table.device)
@@ -394,6 +408,7 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
                out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
         return out
     xt = _type_of(x, "mx4_linear")
+    _refuse_tangents("mx4_linear", x, bias)
     _on_current_device("mx4_linear", x.device, table, bias)
     if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
