@@ -390,6 +390,9 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     n, cols = table.shape
     if bias is not None and (bias.shape != (n,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise ValueError(f"mx4_linear: bias must be contiguous fp32 [{n}]")
+    if torch.is_grad_enabled() and ((bias is not None and bias.requires_grad)
+                                    or (isinstance(x, torch.Tensor) and x.requires_grad)):
+        raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
     codes, scales = table._addresses()
     packed = isinstance(x, Mx4Table)
     if (x.shape[-1] if len(x.shape) else -1) != cols:
@@ -410,8 +413,6 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     xt = _type_of(x, "mx4_linear")
     _refuse_tangents("mx4_linear", x, bias)
     _on_current_device("mx4_linear", x.device, table, bias)
-    if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
-        raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
     lib = L.lib()
     x2 = x if x.dim() == 2 else x.reshape(-1, cols)
     if not x2.is_contiguous():

@@ -4,6 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
+from biomedkg_amd import _lib as L
 from biomedkg_amd import ops
 
 
@@ -60,3 +61,26 @@ def test_plain_tensors_inside_a_dual_level():
     want = ops.embedding(w, ids)
     with fwad.dual_level():
         assert torch.equal(ops.embedding(w, ids), want)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_product_refuses_a_bias_that_requires_a_gradient(packed):
+    x, table = torch.randn(3, 8), ops.Mx4Table(torch.zeros(1, 6, 64, dtype=torch.uint8), torch.zeros(1, 6, 4, dtype=torch.uint8), (6, 8))
+    if packed:
+        x = ops.Mx4Table(torch.zeros(1, 3, 64, dtype=torch.uint8), torch.zeros(1, 3, 4, dtype=torch.uint8), (3, 8))
+    bias = torch.zeros(6, requires_grad=True)
+    with pytest.raises(ValueError, match="without a gradient"):
+        ops.mx4_linear(x, table, bias=bias)
+    with torch.no_grad(), pytest.raises(L.HipLibraryError):      # (as far as the tensors' device)
+        ops.mx4_linear(x, table, bias=bias)
+
+
+@pytest.mark.gpu
+def test_packed_product_and_a_bias_that_requires_a_gradient():
+    gen = torch.Generator().manual_seed(3)
+    x, table = ops.mx4_quantize(torch.randn(3, 8, generator=gen).cuda()), ops.mx4_quantize(torch.randn(6, 8, generator=gen).cuda())
+    bias = torch.randn(6, generator=gen).cuda().requires_grad_()
+    with pytest.raises(ValueError):
+        ops.mx4_linear(x, table, bias=bias)
+    with torch.no_grad():
+        assert torch.equal(ops.mx4_linear(x, table, bias=bias), ops.mx4_linear(x, table, bias=bias.detach()))
