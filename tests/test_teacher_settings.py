@@ -1,0 +1,41 @@
+"""The settings of a distillation run reach ``KGEModule.set_teacher`` as they were given (``train_kge.py teacher_*=``)."""
+import os
+
+import pytest
+
+import train_kge
+from biomedkg_amd.config import compose
+
+CFG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "configs")
+DATA = ["data=synthetic", "data.num_nodes=300", "data.num_edges=2000", "data.embed_dim=16", "model.in_dim=16", "model.hidden_dim=16",
+        "model.out_dim=16", "neg_ratio=1"]
+
+
+@pytest.fixture(scope="module")
+def checkpoint(tmp_path_factory):
+    from biomedkg_amd.trainer import Trainer
+    _, teacher = train_kge.build(compose(CFG, "kge", DATA), "kge")
+    path = str(tmp_path_factory.mktemp("teacher") / "last.ckpt")
+    Trainer(max_epochs=1).save_checkpoint(teacher, path)
+    return path
+
+
+def built(checkpoint, *settings):
+    return train_kge.build(compose(CFG, "kge", DATA + [f"teacher_path={checkpoint}", *settings]), "kge")[1]._teacher
+
+
+def test_settings_as_given(checkpoint):
+    assert built(checkpoint)[1:4] == (10, 1.0, 1.0)
+    assert built(checkpoint, "teacher_k=null", "teacher_weight=null")[1:4] == (10, 1.0, 1.0)
+    assert built(checkpoint, "teacher_k=5", "teacher_temperature=2.0", "teacher_weight=0.5")[1:4] == (5, 2.0, 0.5)
+
+
+@pytest.mark.parametrize("zero", ["0", "0.0"])
+def test_a_weight_of_zero_is_zero(checkpoint, zero):
+    assert built(checkpoint, f"teacher_weight={zero}")[3] == 0.0
+
+
+@pytest.mark.parametrize("bad", ["teacher_k=0", "teacher_temperature=0", "teacher_temperature=0.0"])
+def test_zeros_that_mean_nothing_are_refused(checkpoint, bad):
+    with pytest.raises(ValueError):
+        built(checkpoint, bad)

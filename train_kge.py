@@ -31,8 +31,9 @@ def build(cfg, config_name):
     model.edge_mapping = data_module.edge_map_index
     teacher = cfg.get("teacher_path") or ""
     if teacher:      # distil from a trained checkpoint: its best entities per query (teacher_k, teacher_temperature, teacher_weight)
-        model.set_teacher(KGEModule.load_from_checkpoint(teacher), k=cfg.get("teacher_k") or 10,
-                          temperature=cfg.get("teacher_temperature") or 1.0, weight=cfg.get("teacher_weight") or 1.0)
+        given = {name: cfg.get("teacher_" + name) for name in ("k", "temperature", "weight")}
+        # (absent or null: set_teacher's default; a zero is a setting like any other)
+        model.set_teacher(KGEModule.load_from_checkpoint(teacher), **{n: v for n, v in given.items() if v is not None})
     return data_module, model
 
 
