@@ -154,6 +154,8 @@ class KGEModule(LightningModule):
                                           f"{type(m.model.decoder).__name__})")
         if not (1 <= k <= 1024 and 1e-18 <= temperature <= 1e18 and queries >= 1):
             raise ValueError("set_teacher: k between 1 and 1024, the temperature between 1e-18 and 1e18, at least one query")
+        if not 0.0 <= weight < float("inf"):
+            raise ValueError(f"set_teacher: the weight must be finite and not negative, got {weight}")
         if teacher is self:
             raise ValueError("set_teacher: a module is not its own teacher (it would be frozen)")
         if teacher.model.decoder.rel_emb.size(0) != self.model.decoder.rel_emb.size(0):

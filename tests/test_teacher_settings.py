@@ -5,6 +5,7 @@ import pytest
 
 import train_kge
 from biomedkg_amd.config import compose
+from biomedkg_amd.kge_module import KGEModule
 
 CFG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "configs")
 DATA = ["data=synthetic", "data.num_nodes=300", "data.num_edges=2000", "data.embed_dim=16", "model.in_dim=16", "model.hidden_dim=16",
@@ -39,3 +40,15 @@ def test_a_weight_of_zero_is_zero(checkpoint, zero):
 def test_zeros_that_mean_nothing_are_refused(checkpoint, bad):
     with pytest.raises(ValueError):
         built(checkpoint, bad)
+
+
+@pytest.mark.parametrize("weight", [float("nan"), float("inf"), float("-inf"), -1.0])
+def test_weights_that_are_no_weights_are_refused(weight):
+    def module():
+        return KGEModule("rgcn", "dismult", 8, 8, 8, 2, 5, 2, "cosine", 1e-3, 0.2, "none", 2, "random")
+    student = module()
+    with pytest.raises(ValueError, match="weight"):
+        student.set_teacher(module(), weight=weight)
+    assert not student.has_teacher
+    student.set_teacher(module(), weight=0)
+    assert student.has_teacher
