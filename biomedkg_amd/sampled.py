@@ -158,9 +158,7 @@ class SaintGraphedKge:
         L.require_cuda(x, edge_index, edge_type)
         if getattr(module.model.decoder, "kind", None) is None:
             raise ValueError("the padded step is built on the fused DistMult / TransE loss")
-        if getattr(module, "has_teacher", False):
-            raise ValueError("the padded step holds the reference's loss alone: no distillation from a teacher "
-                             "(KGEModule.set_teacher(None), or the eager training_step)")
+        self._refuse_teacher(module)
         self.module, self.clip, self.graphs_on = module, clip, graphs
         self.neg_ratio = int(module.neg_ratio) if module.neg_ratio else 1
         dev = x.device
@@ -192,6 +190,12 @@ class SaintGraphedKge:
         self.copied = torch.cuda.Event()
         self.branches = True
         self._pinned = []
+
+    @staticmethod
+    def _refuse_teacher(module):
+        if getattr(module, "has_teacher", False):
+            raise ValueError("the padded step holds the reference's loss alone: no distillation from a teacher "
+                             "(KGEModule.set_teacher(None), or the eager training_step)")
 
     def close(self):
         """Wait for everything this loop has in flight (the sampler runs a batch ahead on its own stream): its buffers
@@ -303,6 +307,7 @@ class SaintGraphedKge:
         return choose_bucket(self.buckets, self.neg_ratio, n_b, e_b, e_free)
 
     def step(self):
+        self._refuse_teacher(self.module)                                  # (one may have come since the loop was made)
         trainer = self.module.__dict__.pop("trainer", None)                # .log() inside a step would sync
         L.call("bkg_set_rng_epoch", L.ptr(self.epoch))
         outer = torch.cuda.current_stream()

@@ -2,6 +2,7 @@
 import os
 
 import pytest
+import torch
 
 import train_kge
 from biomedkg_amd.config import compose
@@ -52,3 +53,33 @@ def test_weights_that_are_no_weights_are_refused(weight):
     assert not student.has_teacher
     student.set_teacher(module(), weight=0)
     assert student.has_teacher
+
+
+def _module(dim=8):
+    return KGEModule("rgcn", "dismult", dim, dim, dim, 2, 5, 2, "cosine", 1e-3, 0.2, "none", 1, "random")
+
+
+def test_a_teacher_that_comes_after_the_padded_loop_is_refused():
+    from biomedkg_amd.sampled import SaintGraphedKge
+    loop = SaintGraphedKge.__new__(SaintGraphedKge)
+    loop.module = _module()
+    loop.module.set_teacher(_module())
+    with pytest.raises(ValueError, match="teacher"):
+        loop.step()
+
+
+@pytest.mark.gpu
+def test_padded_loop_around_a_teacher():
+    from biomedkg_amd.sampled import SaintGraphedKge
+    gen = torch.Generator().manual_seed(1)
+    student = _module(32).cuda().train()
+    loop = SaintGraphedKge(student, torch.randn(300, 32, generator=gen).cuda(), torch.randint(0, 300, (2, 2500), generator=gen).cuda(),
+                           torch.randint(0, 5, (2500,), generator=gen).cuda(), 8, 4, None)
+    assert bool(torch.isfinite(loop.step()))
+    student.set_teacher(_module(32))
+    with pytest.raises(ValueError, match="teacher"):
+        loop.step()
+    student.set_teacher(None)
+    assert bool(torch.isfinite(loop.step()))
+    torch.cuda.synchronize()
+    loop.close()
