@@ -168,20 +168,30 @@ __device__ __forceinline__ void kd_teacher_softmax(int k, float c, const int* __
   if (!any) ts = 0.f;
 }
 
+// L = T sum_j q_j ((t_j - tm) - (x_j - m)) + T^2 (ln s - ln ts).  The sum runs over 2^-12 of the differences: logits masked with
+// the type's lowest value are finite, and so is a loss over several of them, but not the sum of up to 1024 such differences, nor a
+// difference divided by T < 1.  (Powers of two: the same digits.)
+constexpr float KD_SMALL = 1.f / 4096, KD_LARGE = 4096.f;
+__device__ __forceinline__ float kd_gap(float t, float tm, float x, float m) {
+  return (t * KD_SMALL - tm * KD_SMALL) - (x * KD_SMALL - m * KD_SMALL);
+}
+__device__ __forceinline__ float kd_loss_of(float temp, float gap, float s, float ts) {
+  const float ln_s = KD_LN2 * __builtin_amdgcn_logf(s), ln_ts = KD_LN2 * __builtin_amdgcn_logf(ts);
+  return temp * KD_LARGE * gap + temp * temp * (ln_s - ln_ts);
+}
+
 // The row's loss from its statistics, in every thread (t_lds still holds t).
 template <typename T>
 __device__ __forceinline__ float kd_loss(const KdArgs& a, const T* __restrict__ xr, const int* __restrict__ id_lds,
                                          const float* __restrict__ t_lds, float m, float s, float tm, float ts, float* red) {
-  const float ln_s = KD_LN2 * __builtin_amdgcn_logf(s), ln_ts = KD_LN2 * __builtin_amdgcn_logf(ts), inv_ts = 1.f / ts;
-  const float inv_t = a.c * KD_LN2;
-  float loss = 0.f;
+  const float inv_ts = 1.f / ts;
+  float gap = 0.f;
   for (int j = threadIdx.x; j < a.te.k; j += blockDim.x) {
     if (id_lds[j] < 0) continue;
     const float q = kd_exp2((t_lds[j] - tm) * a.c) * inv_ts;
-    const float ln_q = (t_lds[j] - tm) * inv_t - ln_ts, ln_p = (widen(xr[id_lds[j]]) - m) * inv_t - ln_s;
-    if (!(q == 0.f)) loss += q * (ln_q - ln_p);
+    if (!(q == 0.f)) gap += q * kd_gap(t_lds[j], tm, widen(xr[id_lds[j]]), m);
   }
-  return a.temp * a.temp * kd_block_sum(loss, red);
+  return kd_loss_of(a.temp, kd_block_sum(gap, red), s, ts);
 }
 
 // The teacher's columns of a row's gradient (the block's part of them) are written again, whole, once the others are there.
@@ -270,13 +280,13 @@ __device__ __forceinline__ KdDone kd_finish_row(const KdArgs& a, float m, float 
     kd_join(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
     tm = fmaxf(tm, __shfl_xor(tm, o, 64));
   }
-  // the teacher's sum and the loss: sum q (ln q - ln p) = sum e ((t - tm) - (x - m)) / (T sum e) - ln sum e + ln s
+  // the teacher's sum and the loss: q = e / sum e
   float ts = 0.f, gap = 0.f;
 #pragma unroll
   for (int x = 0; x < KD_E; ++x) {
     te.e[x] = te.id[x] >= 0 ? kd_exp2((te.tv[x] - tm) * c) : 0.f;
     ts += te.e[x];
-    if (!(te.e[x] == 0.f)) gap += te.e[x] * ((te.tv[x] - tm) - (te.xt[x] - m));
+    if (!(te.e[x] == 0.f)) gap += te.e[x] * kd_gap(te.tv[x], tm, te.xt[x], m);
   }
   ts = wave_sum(ts); gap = wave_sum(gap);
   __syncthreads();
@@ -286,8 +296,7 @@ __device__ __forceinline__ KdDone kd_finish_row(const KdArgs& a, float m, float 
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1) { ts += __shfl_xor(ts, o, 64); gap += __shfl_xor(gap, o, 64); }
   const bool off = !any || (m == -INFINITY && s == 0.f);
-  const float ln_s = KD_LN2 * __builtin_amdgcn_logf(s), ln_ts = KD_LN2 * __builtin_amdgcn_logf(ts);
-  const float loss = off ? 0.f : a.temp * a.temp * (gap * (c * KD_LN2) / ts - ln_ts + ln_s);
+  const float loss = off ? 0.f : kd_loss_of(a.temp, gap / ts, s, ts);
   return KdDone{KdRow{m, off ? 0.f : s, tm, off ? 0.f : ts}, loss};
 }
 
