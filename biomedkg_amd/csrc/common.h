@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/biomedkg_hip.h"
 
 #define BKG_WAVE 64
@@ -19,6 +21,23 @@ static inline int check_launch(const char* what) {
     set_error(what, e);
     return (int)e;
   }
+  return 0;
+}
+
+// Dynamic LDS beyond the 64 KB that a kernel gets unasked: granted per device, so it is asked for on every device that a launch
+// goes to (`granted`: a bit per device, one word per kernel), and again where asking failed.
+static inline int grant_lds(const void* kernel, int bytes, std::atomic<uint64_t>& granted, const char* who) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == hipSuccess && (granted.load(std::memory_order_relaxed) & bit)) return 0;
+  if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();                     // (reported here, not by the next launch)
+    set_error(who, e);
+    return (int)e;
+  }
+  granted.fetch_or(bit, std::memory_order_relaxed);
   return 0;
 }
 

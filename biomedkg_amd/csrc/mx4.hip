@@ -9,6 +9,7 @@
 //
 // Dividing by s only moves the exponent, so quantisation has one rounding and is the same whatever the input's type.
 #include <algorithm>
+#include <atomic>
 
 #include "rowtypes.h"
 
@@ -623,12 +624,12 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__
     if (c + j < n) out[row * ldo + c + j] = (T)(s[j] + (bias ? bias[c + j] : 0.f));
 }
 
+static const char* const MX_LDS = "bkg_mx4 product: dynamic LDS";
 template <typename T, int MT, int NT, int S>
-static void mx4_launch(Mx4Args a, hipStream_t s) {
+static int mx4_launch(Mx4Args a, hipStream_t s) {
   constexpr int LDS = S * (64 * (MT + NT) * 64 + 64 * (MT + NT) * 4);
-  static const bool set = hipFuncSetAttribute((const void*)mx4_tile_kernel<T, MT, NT, S>,
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, LDS) == hipSuccess;
-  (void)set;
+  static std::atomic<uint64_t> granted{0};
+  if (const int rc = grant_lds((const void*)mx4_tile_kernel<T, MT, NT, S>, LDS, granted, MX_LDS)) return rc;
   a.m_tiles = (int)((a.m + 64 * MT - 1) / (64 * MT));
   a.n_tiles = (int)((a.n + 64 * NT - 1) / (64 * NT));
   a.stream = mx4_past_caches<T>(a);
@@ -638,6 +639,7 @@ static void mx4_launch(Mx4Args a, hipStream_t s) {
   const int64_t total = (int64_t)a.m_tiles * a.n_tiles * a.slices;
   const unsigned grid = (unsigned)((total + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS);
   hipLaunchKernelGGL((mx4_tile_kernel<T, MT, NT, S>), dim3(grid), dim3(256), LDS, s, a);
+  return 0;
 }
 
 }  // namespace bkg
@@ -704,32 +706,33 @@ static int mx4_check_product(int64_t m, int64_t n, int64_t cols, const void* b_c
   return 0;
 }
 
-template <typename T, bool PACKED>
-static void mx4_few_launch(const Mx4Args& a, const Mx4X& x, hipStream_t s) {
-  const int64_t tiles = (a.n + 31) / 32;
+template <typename T, bool PACKED, bool KSPLIT>
+static int mx4_few_launch_as(const Mx4Args& a, const Mx4X& x, unsigned blocks, hipStream_t s) {
   const size_t lds = PACKED ? 0 : (size_t)a.steps * (2048 + 128);
   if (!PACKED) {                                             // (up to 64 panels: more than a kernel gets unasked)
-    static const bool set =
-        hipFuncSetAttribute((const void*)mx4_few_kernel<T, PACKED, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 2176) == hipSuccess &&
-        hipFuncSetAttribute((const void*)mx4_few_kernel<T, PACKED, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 64 * 2176) == hipSuccess;
-    (void)set;
+    static std::atomic<uint64_t> granted{0};
+    if (const int rc = grant_lds((const void*)mx4_few_kernel<T, PACKED, KSPLIT>, 64 * 2176, granted, MX_LDS)) return rc;
   }
+  hipLaunchKernelGGL((mx4_few_kernel<T, PACKED, KSPLIT>), dim3(blocks), dim3(256), lds, s, a, x);
+  return 0;
+}
+template <typename T, bool PACKED>
+static int mx4_few_launch(const Mx4Args& a, const Mx4X& x, hipStream_t s) {
+  const int64_t tiles = (a.n + 31) / 32;
   // a wave per tile keeps the chip busy from 2048 tiles on; below that, and with panels to share, the waves of a block
-  if (tiles >= 2048 || a.steps < 4)
-    hipLaunchKernelGGL((mx4_few_kernel<T, PACKED, false>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), lds, s, a, x);
-  else
-    hipLaunchKernelGGL((mx4_few_kernel<T, PACKED, true>), dim3((unsigned)tiles), dim3(256), lds, s, a, x);
+  if (tiles >= 2048 || a.steps < 4) return mx4_few_launch_as<T, PACKED, false>(a, x, (unsigned)((tiles + 3) / 4), s);
+  return mx4_few_launch_as<T, PACKED, true>(a, x, (unsigned)tiles, s);
 }
 
 template <typename T, int STEPS, bool STREAM>
-static void mx4_stream_launch_as(const Mx4Args& a, unsigned blocks, hipStream_t s) {
-  static const bool set = hipFuncSetAttribute((const void*)mx4_stream_kernel<T, STEPS, STREAM>,
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, ms_lds(STEPS)) == hipSuccess;
-  (void)set;
+static int mx4_stream_launch_as(const Mx4Args& a, unsigned blocks, hipStream_t s) {
+  static std::atomic<uint64_t> granted{0};
+  if (const int rc = grant_lds((const void*)mx4_stream_kernel<T, STEPS, STREAM>, ms_lds(STEPS), granted, MX_LDS)) return rc;
   hipLaunchKernelGGL((mx4_stream_kernel<T, STEPS, STREAM>), dim3(blocks), dim3(256), ms_lds(STEPS), s, a);
+  return 0;
 }
 template <typename T, int STEPS>
-static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
+static int mx4_stream_launch(Mx4Args a, hipStream_t s) {
   // classes of rows (mx_class) where rows are long and every class fills a tile.  Blocks next to each other write the lines that
   // short rows share at about the same time: 130000 x 1000 in bf16, 256 inner columns, 93 us without classes and 110 with; in
   // fp32 162 and 132; 32768 x 4008 in bf16 96 and 62.
@@ -751,8 +754,8 @@ static void mx4_stream_launch(Mx4Args a, hipStream_t s) {
   a.band = (int)((a.m_tiles + parts - 1) / parts);
   const int64_t blocks = (int64_t)((a.m_tiles + a.band - 1) / a.band) *
                          (n_tiles >= 8 * BKG_XCDS ? (n_tiles + BKG_XCDS - 1) / BKG_XCDS * BKG_XCDS : n_tiles);
-  if (a.stream) mx4_stream_launch_as<T, STEPS, true>(a, (unsigned)blocks, s);
-  else mx4_stream_launch_as<T, STEPS, false>(a, (unsigned)blocks, s);
+  return a.stream ? mx4_stream_launch_as<T, STEPS, true>(a, (unsigned)blocks, s)
+                  : mx4_stream_launch_as<T, STEPS, false>(a, (unsigned)blocks, s);
 }
 
 // rows of x that a product packs within its one launch: at most 32, and few enough values that every block packs them anew
@@ -774,7 +777,7 @@ static int64_t mx4_sums_bytes(int64_t m, int64_t n, int64_t cols) {
 }
 
 template <typename T>
-static void mx4_product(const Mx4Args& a, float* sums, int64_t cols, hipStream_t s) {
+static int mx4_product(const Mx4Args& a, float* sums, int64_t cols, hipStream_t s) {
   const int slices = mx4_slices(a.m, a.n, cols);
   if (slices > 1) {
     Mx4Args b = a;
@@ -783,26 +786,26 @@ static void mx4_product(const Mx4Args& a, float* sums, int64_t cols, hipStream_t
     b.ldo = (a.n + 3) / 4 * 4;
     b.wide = 1;                                              // (the workspace is 16-byte aligned)
     b.slices = slices;
-    mx4_launch<float, 2, 2, 2>(b, s);
+    if (const int rc = mx4_launch<float, 2, 2, 2>(b, s)) return rc;
     const int64_t threads = a.m * (b.ldo / 4);
     hipLaunchKernelGGL((mx4_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, sums, slices, a.m, a.n, b.ldo,
                        a.bias, (T*)a.out, a.ldo);
-    return;
+    return 0;
   }
-  if (a.m <= 32) mx4_few_launch<T, true>(a, Mx4X{}, s);
+  if (a.m <= 32) return mx4_few_launch<T, true>(a, Mx4X{}, s);
   // up to six panels: B in registers (1021 x 130000 x 768 in bf16 157 us with 128 x 128 tiles, 124 so; 8192 x 8192 x 768 68 and
   // 46; 4096 x 4096 x 768 17.4 and 16.5; 130000 x 256 x 768 37 and 29); each class of rows loads it anew.
-  else if (a.steps == 1) mx4_stream_launch<T, 1>(a, s);
-  else if (a.steps == 2) mx4_stream_launch<T, 2>(a, s);
-  else if (a.steps == 3) mx4_stream_launch<T, 3>(a, s);
-  else if (a.steps == 4) mx4_stream_launch<T, 4>(a, s);
-  else if (a.steps == 5) mx4_stream_launch<T, 5>(a, s);
-  else if (a.steps == 6) mx4_stream_launch<T, 6>(a, s);
+  if (a.steps == 1) return mx4_stream_launch<T, 1>(a, s);
+  if (a.steps == 2) return mx4_stream_launch<T, 2>(a, s);
+  if (a.steps == 3) return mx4_stream_launch<T, 3>(a, s);
+  if (a.steps == 4) return mx4_stream_launch<T, 4>(a, s);
+  if (a.steps == 5) return mx4_stream_launch<T, 5>(a, s);
+  if (a.steps == 6) return mx4_stream_launch<T, 6>(a, s);
   // More: 256 x 256 tiles, a block with a CU to itself, where they fill the chip and the inner dimension is long (8192 x 8192 x
   // 8192 in bf16: 271 us, 4 PFLOP/s, against 316 with 128 x 128; 4096 x 4096 x 4096 42 and 46; x 2048 31 and 31); else 128 x 128,
   // four blocks on a CU: one stores while others multiply (5000 x 6000 x 1024: 34 us, 256 x 256 44; 2048 x 2048 x 8192 39 and 52).
-  else if ((a.m + 255) / 256 * ((a.n + 255) / 256) >= 192 && a.steps >= 16) mx4_launch<T, 4, 4, 4>(a, s);
-  else mx4_launch<T, 2, 2, 2>(a, s);
+  if ((a.m + 255) / 256 * ((a.n + 255) / 256) >= 192 && a.steps >= 16) return mx4_launch<T, 4, 4, 4>(a, s);
+  return mx4_launch<T, 2, 2, 2>(a, s);
 }
 
 extern "C" int64_t bkg_mx4_matmul_workspace_bytes(int64_t m, int64_t n, int64_t cols) {
@@ -821,7 +824,9 @@ extern "C" int bkg_mx4_matmul(const void* a_codes, const void* a_scales, int64_t
   const Mx4Args a{(const unsigned char*)a_codes, (const uint32_t*)a_scales, m, (const unsigned char*)b_codes,
                   (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0, bias, out, ldo,
                   access_bytes(out, 0, ldo * type_bytes(type)) == 16, 1, 0, 1};
-  BKG_BY_TYPE(type, mx4_product<T>(a, (float*)workspace, cols, (hipStream_t)stream));
+  int rc = 0;
+  BKG_BY_TYPE(type, rc = mx4_product<T>(a, (float*)workspace, cols, (hipStream_t)stream));
+  if (rc) return rc;
   return check_launch("bkg_mx4_matmul");
 }
 
@@ -848,6 +853,8 @@ extern "C" int bkg_mx4_linear(const void* x, int32_t x_type, int64_t ldx, int64_
   }
   const Mx4Args a{nullptr, nullptr, m, (const unsigned char*)b_codes, (const uint32_t*)b_scales, n, (int)mx4_steps(cols), 0, 0, 0,
                   bias, out, ldo, 0, 1, 0, 1};
-  BKG_BY_TYPE(type, (mx4_few_launch<T, false>(a, Mx4X{x, x_type, ldx, (int)cols}, (hipStream_t)stream)));
+  int rc = 0;
+  BKG_BY_TYPE(type, rc = (mx4_few_launch<T, false>(a, Mx4X{x, x_type, ldx, (int)cols}, (hipStream_t)stream)));
+  if (rc) return rc;
   return check_launch("bkg_mx4_linear");
 }

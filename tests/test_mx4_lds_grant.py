@@ -1,0 +1,20 @@
+"""The packed product's kernels ask for their dynamic LDS on the device that they are launched on; a refusal is the call's error."""
+import pytest
+import torch
+
+from biomedkg_amd import _lib as L
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the buffers are the host's: nothing may be launched")
+@pytest.mark.parametrize("m,n,cols", [(100, 100, 100), (100, 100, 800), (1000, 1000, 4000), (4000, 4000, 4000), (100, 3, 8320)])
+@pytest.mark.parametrize("times", [1, 2])
+def test_a_refused_grant_is_the_calls_error(m, n, cols, times):
+    """without a device there is nothing to grant: every call says so, the second one as well"""
+    lib = L.lib()
+    host = torch.zeros(1 << 12, dtype=torch.uint8)
+    p = (host.data_ptr() + 255) // 256 * 256
+    for _ in range(times):
+        assert lib.bkg_mx4_matmul(p, p, m, p, p, n, cols, None, p, 1, n, p, 1 << 40, None) != 0
+        assert b"dynamic LDS" in lib.bkg_last_error()
+    assert lib.bkg_mx4_linear(p, 1, 256, 2, p, p, n, 256, None, p, 1, n, p, 1 << 40, None) != 0
+    assert b"dynamic LDS" in lib.bkg_last_error()
