@@ -82,6 +82,13 @@ __device__ __forceinline__ int km_pick(int v, int src_lane) {   // v of lane `sr
   return __builtin_amdgcn_ds_bpermute(src_lane << 2, v);
 }
 __device__ __forceinline__ int km_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// The lane's number, counted where it is asked for: no register holds it, or what is made of it, until then.  (The walk has none to
+// spare.  A spilled one comes back on the row ring's counter, and hipcc waits for it with vmcnt(0): the ring is drained.)
+__device__ __forceinline__ int km_lane() {
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
 
 // one step of the stream a wave walks: 8 rounds of a node quad (lane group g: entries e0 .. e0 + 7 of ITS node's list)
 struct KmStep {
@@ -94,7 +101,8 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
   constexpr int Q = 2, VQ = 4;
   extern __shared__ __attribute__((aligned(16))) unsigned char km_lds[];
   float* rel_lds = reinterpret_cast<float*>(km_lds);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, grp = lane >> 4, lig = lane & 15;
+  // (uniform for hipcc too: what follows from the wave's number -- its quad, step counts, flags -- stays in scalar registers)
+  const int wave = km_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, grp = lane >> 4, lig = lane & 15;
   unsigned char* stage0 = km_lds + KM_NR * KM_D * 4;                  // [4 waves] staging areas
   // (plain LDS words: a volatile generic pointer compiles to a flat store with system scope and a vmcnt(0) behind it)
   int* flags = reinterpret_cast<int*>(km_lds + KM_NR * KM_D * 4 + 4 * KM_STAGE);
@@ -147,7 +155,7 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
     I.first = i_c == 0;
     I.last = i_c + 1 == i_nst;
     {                                                // (unconditional too: a finished stream re-reads entry 0)
-      const int e = min(max(I.e0 + (lig & (KM_STEP - 1)), 0), last_entry);
+      const int e = min(max(I.e0 + (km_lane() & (KM_STEP - 1)), 0), last_entry);
       i_vo = a.packed[e];
       if (SCORES) i_vp = a.perm[e];
     }
@@ -155,19 +163,13 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
 
   // ---- row ring: slot u holds round u of the step being consumed, then of the step behind it
   Piece<__bf16> val[KM_STEP][2];
-  int rid_s[KM_STEP], pm_s[KM_STEP];
+  int rid_s[KM_STEP];
   KmStep R{0, 0, 0, 0, 0, 0, 0}, C{0, 0, 0, 0, 0, 0, 0};
-  int r_vo = 0, r_vp = 0;
+  int r_vo = 0, r_vp = 0, c_vp = 0;                  // step R's entries; step C's positions
   // the row of round u of step R: its entry is picked (an LDS crossbar round trip) at the TOP of the round that frees the
   // slot, the loads are issued at its end
-  auto pick = [&](int u, int& nv, int& np) {
-    const int src = (lane & 48) | u;
-    nv = km_pick(r_vo, src);
-    if (SCORES) np = km_pick(r_vp, src);
-  };
-  auto issue = [&](int u, int nv, int np) {
+  auto issue = [&](int u, int nv) {
     rid_s[u] = (int)((unsigned)nv >> 24);
-    if (SCORES) pm_s[u] = np;
     // (a slot past the end of this group's list -- padding: the quad's four lists run to the longest, rounded up to 8 --
     // loads row 0, a cache hit, instead of whatever entry the clamped position holds: 0.6 GB less off the fabric per launch)
     const unsigned row = (R.e0 + u < R.end) ? (unsigned)(nv & 0xffffff) : 0u;
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
   // that almost nothing younger is in flight, and it drained the row ring at every step)
   for (int step = 0;; ++step) {
     C = R;
-    R = I; r_vo = i_vo; r_vp = i_vp;
+    R = I; r_vo = i_vo; c_vp = r_vp; r_vp = i_vp;
     advance_I();
     const bool c_on = km_uniform(C.valid) != 0;
     if (!c_on) { C.e0 = C.mid = C.end = 0; }                           // (every round dead: this wave only keeps the others company)
@@ -229,8 +231,8 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
       unsigned char* relk = stage + 16 * KM_ROW;
       const int e = C.e0 + u;
       const bool live = e < C.end, head = e < C.mid;
-      int nv = 0, np = 0;
-      pick(u, nv, np);
+      const int nv = km_pick(r_vo, (lane & 48) | u);
+      const int pm = SCORES ? km_pick(c_vp, (lane & 48) | u) : 0;
       if (__builtin_amdgcn_ballot_w64(live) != 0) {                   // (a round past every group's list costs nothing)
         float4 o[VQ];
         val[u][0].expand(o);
@@ -260,7 +262,7 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
           acc[q].z = fmaf(gi, t4[q].z, acc[q].z); acc[q].w = fmaf(gi, t4[q].w, acc[q].w);
         }
         if (head && live && lig == 0) {
-          if (SCORES) a.score[pm_s[u]] = sc;                            // (head end: its position IS the triplet id)
+          if (SCORES) a.score[pm] = sc;                                 // (head end: its position IS the triplet id)
           loss_acc += fmaxf(sc, 0.f) - sc * a.label + 0.6931471805599453f * __builtin_amdgcn_logf(1.0f + ex);
         }
         if (step_heads) {
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
         *reinterpret_cast<uint4*>(dst + 256) = make_uint4(0u, 0u, 0u, 0u);
         if (lig == 0) relk[k] = 255;
       }
-      issue(u, nv, np);   // this slot's next tenant: round u of the step behind (unconditional: past the stream's end entry 0 again)
+      issue(u, nv);   // this slot's next tenant: round u of the step behind (unconditional: past the stream's end entry 0 again)
       if ((u & 3) == 0 && !step_heads && lane < 16) relk[lane] = 255;   // (no head entry left: a zero one-hot over stale rows)
 #if defined(KM_ABL) && (KM_ABL & 4)
       if (false) {
@@ -330,11 +332,12 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
       }
     }
     if (c_on && km_uniform(C.last)) {
+      const int l16 = km_lane() & 15;
       if (C.node < a.n_nodes) {
 #pragma unroll
         for (int q = 0; q < VQ; ++q) {
           float4 v = acc[q];
-          *reinterpret_cast<float4*>(a.dz + (int64_t)C.node * a.lddz + piece_col<__bf16, 16>(lig, q)) = v;
+          *reinterpret_cast<float4*>(a.dz + (int64_t)C.node * a.lddz + piece_col<__bf16, 16>(l16, q)) = v;
         }
       }
       zero4(acc);
@@ -345,15 +348,16 @@ __global__ __launch_bounds__(256, 2) void kge_onepass_mx_kernel(const KmArgs a) 
   }
 
   // ---- the workgroup's sums leave, this wave its 64 columns: C[b][4 j + i] = row 8 j + 4 (lane / 32) + i, column 32 b + lane % 32
+  const int end_lane = km_lane();
   float* out = a.drel_part + (int64_t)blockIdx.x * KM_NR * KM_D + 64 * wave;
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      out[(8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * KM_D + 32 * b + (lane & 31)] = cacc[b][i];
+      out[(8 * (i >> 2) + 4 * (end_lane >> 5) + (i & 3)) * KM_D + 32 * b + (end_lane & 31)] = cacc[b][i];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) loss_acc += __shfl_xor(loss_acc, o, 64);
-  if (lane == 0) a.loss_part[wave_id] = loss_acc;
+  if (end_lane == 0) a.loss_part[wave_id] = loss_acc;
 }
 
 }  // namespace bkg
