@@ -24,6 +24,8 @@ GROUPED_NEG_TYPES = __import__("os").environ.get("BKG_GROUPED_NEG_TYPES", "0") =
 
 
 class KGEModule(LightningModule):
+    _teacher = None      # (of the class: a module that was pickled before there were teachers has none)
+
     def __init__(self, encoder_name: str, decoder_name: str, in_dim: int, hidden_dim: int, out_dim: int,
                  num_hidden_layers: int, num_relation: int, num_heads: int, scheduler_type: str, learning_rate: float,
                  warm_up_ratio: float, fuse_method: str, neg_ratio: int, node_init_method: str):
@@ -45,7 +47,6 @@ class KGEModule(LightningModule):
         self.valid_metrics = metrics.clone(prefix="val_")
         self.test_metrics = metrics.clone(prefix="test_")
         self._fix_edge_id = None
-        self._teacher = None
 
     def fusion_fn(self, x) -> torch.Tensor:
         """reference kge_module.py:77-84."""

@@ -1,5 +1,6 @@
 """The settings of a distillation run reach ``KGEModule.set_teacher`` as they were given (``train_kge.py teacher_*=``)."""
 import os
+import pickle
 
 import pytest
 import torch
@@ -83,3 +84,12 @@ def test_padded_loop_around_a_teacher():
     assert bool(torch.isfinite(loop.step()))
     torch.cuda.synchronize()
     loop.close()
+
+
+def test_a_module_pickled_before_there_were_teachers_has_none():
+    module = _module()
+    module.__dict__.pop("_teacher", None)                    # (whole-module pickles hold the attributes of their time)
+    module = pickle.loads(pickle.dumps(module))
+    assert not module.has_teacher and module._teacher is None
+    module.set_teacher(_module())
+    assert module.has_teacher
