@@ -44,3 +44,37 @@ def test_a_masked_entry_without_weight_adds_nothing(rows):
     got = ops.topk_distill_loss(x.cuda(), ids.cuda(), t.cuda(), 1.0, reduction="none").double().cpu()
     want = torch.log(torch.tensor(48.0, dtype=torch.float64))
     assert float((got - want).abs().max()) <= 64 * U * float(want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,v", [(1100, 2000003), (3, 800000001)])
+def test_beyond_32_bits_no_column_is_left_out(rows, v):
+    """the loss and the gradient's mass of logits with more than 2^31 values, to the accuracy of the sums as they are cut: a block
+    of 1024 threads for a row, or (few rows) ceil(2048 / rows) blocks of 256"""
+    gen = torch.Generator().manual_seed(4)
+    x = torch.empty(rows, v, dtype=torch.bfloat16, device="cuda").normal_()
+    k = 5
+    ids, tl = torch.randint(0, v, (rows, k), generator=gen).cuda(), torch.randn(rows, k, generator=gen).cuda()
+    ids[-1, 0] = v - 1
+    chain = v / 1024 if rows >= 192 else v / (256 * -(-2048 // rows))
+    losses = ops.topk_distill_loss(x, ids, tl, 1.0, reduction="none")
+    xx = x.requires_grad_()
+    ops.topk_distill_loss(xx, ids, tl, 1.0, reduction="sum").backward()
+    for r in (0, rows - 1):
+        row = x.detach()[r].double()
+        lse = torch.logsumexp(row, 0)
+        lq = torch.log_softmax(tl[r].double(), 0)
+        want = float((lq.exp() * (lq - (row[ids[r]] - lse))).sum())
+        span = float(row.max() - row.min())
+        # An exponential is off by 3 u of its argument's range and 2 u; a thread's chain adds u per term, its rescaling when a
+        # larger logit comes and the joins of threads, waves and blocks a few u each (64 in all), the teacher's sums 2 k u.
+        err = U * (3 * span + chain + 2 * k + 64)
+        assert err < 1e-3
+        assert abs(float(losses[r]) - want) <= err + U * 8 * (span + 8 + abs(want))
+        p = (row - lse).exp()
+        pq = p.clone()
+        p.index_add_(0, ids[r], -lq.exp())
+        pq.index_add_(0, ids[r], lq.exp())
+        over = (xx.grad[r].double() - p).abs() - (p.abs() * (2.0 ** -8 + 4 * U) + 2 * err * pq * (1 + 2.0 ** -8) + 2.0 ** -134)
+        assert float(over.max()) <= 0
+        del row, p, pq, over
