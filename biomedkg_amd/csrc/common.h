@@ -27,6 +27,7 @@ static inline int check_launch(const char* what) {
 // Dynamic LDS beyond the 64 KB that a kernel gets unasked: granted per device, so it is asked for on every device that a launch
 // goes to (`granted`: a bit per device, one word per kernel), and again where asking failed.
 static inline int grant_lds(const void* kernel, int bytes, std::atomic<uint64_t>& granted, const char* who) {
+  if (bytes <= (64 << 10)) return 0;
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);

@@ -56,9 +56,8 @@ def _refuse_devices(what, dev, others):
 
 def _refuse_tangents(what, *tensors):
     """Forward-mode derivatives are not implemented: an input that carries one is refused, whether or not a gradient is recorded
-    (an autograd function refuses it by itself, but a call that records nothing does not go through one)."""
-    if getattr(_forward_ad, "_current_level", 0) < 0:        # (outside every dual_level no tensor carries one)
-        return
+    (an autograd function refuses it by itself, but a call that records nothing does not go through one).  Callers look at the
+    current level first: outside every ``dual_level`` no tensor carries one."""
     for t in tensors:
         if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
@@ -114,7 +113,8 @@ def _check_embedding(weight, ids):
     if weight.dim() != 2:
         raise ValueError(f"embedding: expected a [V, d] table, got {tuple(weight.shape)}")
     _type_of(weight, "embedding")
-    _refuse_tangents("embedding", weight)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("embedding", weight)
     _ids(ids, "embedding ids")
     _on_current_device("embedding", weight.device, ids)
 
@@ -226,7 +226,8 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, redu
     _type_of(logits, "topk_distill_loss logits")
     _type_of(teacher_logits, "topk_distill_loss teacher logits")
     _ids(teacher_ids, "topk_distill_loss teacher ids")
-    _refuse_tangents("topk_distill_loss", logits, teacher_logits)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("topk_distill_loss", logits, teacher_logits)
     _on_current_device("topk_distill_loss", logits.device, teacher_ids, teacher_logits)
     if reduction not in ("batchmean", "sum", "none"):
         raise ValueError(f"topk_distill_loss: reduction {reduction!r} (batchmean, sum or none)")
@@ -258,31 +259,39 @@ class Mx4Table:
     with zeros): ``codes`` uint8 ``[panels, rows, 64]`` (two columns a byte, the lower one in the low nibble) and ``scales``
     uint8 ``[panels, rows, 4]`` (the exponent of each 32 columns + 127; 255: the block held an infinity or NaN).  0.53 bytes a
     value."""
-    __slots__ = ("shape", "_store")
+    __slots__ = ("shape", "device", "codes_ptr", "scales_ptr", "_store")
 
     def __init__(self, codes, scales, shape):
-        self.shape = tuple(shape)
-        rows, cols = self.shape
+        rows, cols = shape
         panels = (cols + 127) // 128
         for t, want, what in ((codes, (panels, rows, 64), "codes"), (scales, (panels, rows, 4), "scales")):
             if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
-                raise ValueError(f"Mx4Table: {what} must be contiguous uint8 {want} for a table of {self.shape}")
+                raise ValueError(f"Mx4Table: {what} must be contiguous uint8 {want} for a table of {tuple(shape)}")
         if codes.device != scales.device:
             raise ValueError(f"Mx4Table: codes on {codes.device}, scales on {scales.device}")
         if codes.data_ptr() % 16 or scales.data_ptr() % 4:
             raise ValueError("Mx4Table: codes must be 16-byte, scales 4-byte aligned")
+        self.shape, self.device = (rows, cols), codes.device
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
         self._store = (codes, scales)
 
     @classmethod
-    def _empty(cls, rows, cols, device):
-        """An unwritten table in one piece of memory: the codes, then the scales."""
+    def _of(cls, store, rows, cols):
+        """A table in one piece of memory: the codes, then the scales."""
         self = cls.__new__(cls)
-        self._store = torch.empty((cols + 127) // 128 * rows * 68, dtype=torch.uint8, device=device)
-        self.shape = (rows, cols)
+        self.shape, self.device = (rows, cols), store.device
+        self.codes_ptr = store.data_ptr()
+        self.scales_ptr = self.codes_ptr + (cols + 127) // 128 * rows * 64
+        self._store = store
         return self
 
+    @classmethod
+    def _empty(cls, rows, cols, device):
+        return cls._of(torch.empty((cols + 127) // 128 * rows * 68, dtype=torch.uint8, device=device), rows, cols)
+
     def __reduce__(self):
-        """Copies and saved tables (``copy``, ``pickle``, ``torch.save``) are made from the memory and the shape."""
+        """Copies and saved tables (``copy``, ``pickle``, ``torch.save``) are made from the memory and the shape: device and
+        addresses are those of the copy's own memory."""
         if self._store.__class__ is tuple:
             return Mx4Table, (*self._store, self.shape)
         return _table_in_one_piece, (self._store, self.shape)
@@ -295,15 +304,6 @@ class Mx4Table:
         cut = panels * rows * 64
         return store[:cut].view(panels, rows, 64), store[cut:].view(panels, rows, 4)
 
-    def _addresses(self):
-        """Where the codes and the scales lie.  (Asked of the memory at every call: a number kept beside it would go along into
-        a copy, whose memory is another.)"""
-        store = self._store
-        if store.__class__ is tuple:
-            return store[0].data_ptr(), store[1].data_ptr()
-        base = store.data_ptr()
-        return base, base + (self.shape[1] + 127) // 128 * self.shape[0] * 64
-
     @property
     def codes(self):
         return self._parts()[0]
@@ -311,18 +311,6 @@ class Mx4Table:
     @property
     def scales(self):
         return self._parts()[1]
-
-    @property
-    def codes_ptr(self):
-        return self._addresses()[0]
-
-    @property
-    def scales_ptr(self):
-        return self._addresses()[1]
-
-    @property
-    def device(self):
-        return (self._store[0] if self._store.__class__ is tuple else self._store).device
 
     @property
     def nbytes(self):
@@ -337,9 +325,7 @@ def _table_in_one_piece(store, shape):
     if store.dtype != torch.uint8 or store.shape != ((cols + 127) // 128 * rows * 68,) or not store.is_contiguous() \
             or store.data_ptr() % 16:
         raise ValueError(f"Mx4Table: no packed table of {tuple(shape)}")
-    self = Mx4Table.__new__(Mx4Table)
-    self.shape, self._store = (rows, cols), store
-    return self
+    return Mx4Table._of(store, rows, cols)
 
 
 def mx4_quantize(x):
@@ -356,8 +342,7 @@ def mx4_quantize(x):
     if not x.is_contiguous():
         x = _rows(x.detach())
     table = Mx4Table._empty(rows, cols, x.device)
-    codes, scales = table._addresses()
-    rc = L.lib().bkg_mx4_quantize(x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, codes, scales, L.stream())
+    rc = L.lib().bkg_mx4_quantize(x.data_ptr(), _TYPE[x.dtype], x.stride(0), rows, cols, table.codes_ptr, table.scales_ptr, L.stream())
     if rc:
         L.failed("bkg_mx4_quantize", rc)
     return table
@@ -372,8 +357,7 @@ def mx4_dequantize(table, dtype=torch.float32):
     _on_current_device("mx4_dequantize", table.device)
     rows, cols = table.shape
     out = torch.empty(rows, cols, dtype=dtype, device=table.device)
-    codes, scales = table._addresses()
-    rc = L.lib().bkg_mx4_dequantize(codes, scales, rows, cols, out.data_ptr(), _TYPE[dtype], cols, L.stream())
+    rc = L.lib().bkg_mx4_dequantize(table.codes_ptr, table.scales_ptr, rows, cols, out.data_ptr(), _TYPE[dtype], cols, L.stream())
     if rc:
         L.failed("bkg_mx4_dequantize", rc)
     return out
@@ -390,28 +374,28 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     n, cols = table.shape
     if bias is not None and (bias.shape != (n,) or bias.dtype != torch.float32 or not bias.is_contiguous()):
         raise ValueError(f"mx4_linear: bias must be contiguous fp32 [{n}]")
-    if torch.is_grad_enabled() and ((bias is not None and bias.requires_grad)
-                                    or (isinstance(x, torch.Tensor) and x.requires_grad)):
-        raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
-    codes, scales = table._addresses()
     packed = isinstance(x, Mx4Table)
+    if ((bias is not None and bias.requires_grad) or (not packed and x.requires_grad)) and torch.is_grad_enabled():
+        raise ValueError("mx4_linear is an inference product without a gradient (call it under torch.no_grad())")
     if (x.shape[-1] if len(x.shape) else -1) != cols:
         raise ValueError(f"mx4_linear: x {tuple(x.shape)} against a table of {cols} columns")
     out_dtype = out_dtype or (torch.float32 if packed else x.dtype)
     if out_dtype not in _TYPE:
         raise TypeError(f"mx4_linear: out_dtype float32, bfloat16 or float16, got {out_dtype}")
     if packed:
-        _refuse_tangents("mx4_linear", bias)
+        if _forward_ad._current_level >= 0:
+            _refuse_tangents("mx4_linear", bias)
         _on_current_device("mx4_linear", table.device, x, bias)
         m = x.shape[0]
         out = torch.empty(m, n, dtype=out_dtype, device=table.device)
         ws_bytes = L.lib().bkg_mx4_matmul_workspace_bytes(m, n, cols)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=table.device) if ws_bytes else None
-        L.call("bkg_mx4_matmul", *x._addresses(), m, codes, scales, n, cols, L.ptr(bias),
+        L.call("bkg_mx4_matmul", x.codes_ptr, x.scales_ptr, m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
                out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
         return out
     xt = _type_of(x, "mx4_linear")
-    _refuse_tangents("mx4_linear", x, bias)
+    if _forward_ad._current_level >= 0:
+        _refuse_tangents("mx4_linear", x, bias)
     _on_current_device("mx4_linear", x.device, table, bias)
     lib = L.lib()
     x2 = x if x.dim() == 2 else x.reshape(-1, cols)
@@ -421,7 +405,7 @@ def mx4_linear(x, table, bias=None, out_dtype=None):
     out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
     ws_bytes = lib.bkg_mx4_linear_workspace_bytes(m, n, cols)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-    rc = lib.bkg_mx4_linear(x2.data_ptr(), xt, x2.stride(0), m, codes, scales, n, cols, L.ptr(bias),
+    rc = lib.bkg_mx4_linear(x2.data_ptr(), xt, x2.stride(0), m, table.codes_ptr, table.scales_ptr, n, cols, L.ptr(bias),
                             out.data_ptr(), _TYPE[out_dtype], n, L.ptr(ws), ws_bytes, L.stream())
     if rc:
         L.failed("bkg_mx4_linear", rc)
