@@ -304,8 +304,8 @@ __device__ __forceinline__ KdDone kd_finish_row(const KdArgs& a, float m, float 
 // threads two blocks share a CU, and the rows in work (133 MB of 260 KB rows) stay in the Infinity Cache; more, smaller blocks
 // push them out (4096 x 130000 in bf16: 1024 threads 547 us, 512 594, 256 699).  Rows up to KD_SHORT bytes take 512 threads
 // (1021 x 32771 in fp16, loss only: 17 us against 21).  Keeping part of a row on the CU -- 272 KB of registers and LDS, one
-// block per CU, each place filled with the next row's access as its gradient leaves -- took 595 us (nothing moves while it
-// adds up), two smaller blocks with half a row kept 537.
+// block per CU, each place filled with the next row's access as its gradient leaves -- took 595 us beside those 547 (nothing moves
+// while it adds up), two smaller blocks with half a row kept 537: two percent, not worth a second kernel.
 constexpr int64_t KD_SHORT = 128 << 10;
 template <typename T, int N>
 __global__ __launch_bounds__(N) void kd_row_kernel(const KdArgs a) {

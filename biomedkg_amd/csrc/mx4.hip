@@ -184,8 +184,8 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(mx_i32x4 a, mx_i32x4 b, mx_f32x16 c
 //
 // The result goes through LDS once (32 rows of a wave at a time) so that rows leave in runs of 16-byte stores.
 //
-// Bound by power at 256 x 256: a product of random values runs at 1.66 GHz with the matrix units 55 % busy, one of zeros takes
-// two thirds of its time; without copies and LDS reads the products alone would take three quarters.
+// At 256 x 256 an 8192^3 product takes 493 k cycles, 262 k of them products on every matrix unit (53 %), whatever the values; the
+// clock is what power leaves: 1.81 GHz for random values (272 us), 2.28 for zeros (214).
 template <typename T, int MT, int NT, int S>
 __global__ __launch_bounds__(256, MT * NT >= 16 ? 1 : 2) void mx4_tile_kernel(const Mx4Args a) {
   constexpr int BM = 64 * MT, BN = 64 * NT;
