@@ -153,6 +153,7 @@ class KGEModule(LightningModule):
             if not hasattr(m.model.decoder, "entity_logits"):
                 raise NotImplementedError(f"distillation over entities is implemented for DistMult decoders (the {who}'s is "
                                           f"{type(m.model.decoder).__name__})")
+        temperature, weight = float(temperature), float(weight)
         if not (1 <= k <= 1024 and 1e-18 <= temperature <= 1e18 and queries >= 1):
             raise ValueError("set_teacher: k between 1 and 1024, the temperature between 1e-18 and 1e18, at least one query")
         if not 0.0 <= weight < float("inf"):
@@ -163,7 +164,7 @@ class KGEModule(LightningModule):
             raise ValueError(f"set_teacher: the teacher knows {teacher.model.decoder.rel_emb.size(0)} relations, the student "
                              f"{self.model.decoder.rel_emb.size(0)}")
         teacher.eval().requires_grad_(False)
-        self._teacher = (teacher, int(k), float(temperature), float(weight), int(queries))     # (a tuple: not a submodule)
+        self._teacher = (teacher, int(k), temperature, weight, int(queries))     # (a tuple: not a submodule)
 
     @property
     def has_teacher(self):

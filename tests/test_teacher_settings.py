@@ -32,6 +32,10 @@ def test_settings_as_given(checkpoint):
     assert built(checkpoint, "teacher_k=5", "teacher_temperature=2.0", "teacher_weight=0.5")[1:4] == (5, 2.0, 0.5)
 
 
+def test_numbers_that_the_command_line_reads_as_text(checkpoint):
+    assert built(checkpoint, "teacher_weight=1e-3", "teacher_temperature=1e1")[2:4] == (10.0, 0.001)     # (YAML wants a point)
+
+
 @pytest.mark.parametrize("zero", ["0", "0.0"])
 def test_a_weight_of_zero_is_zero(checkpoint, zero):
     assert built(checkpoint, f"teacher_weight={zero}")[3] == 0.0
