@@ -296,6 +296,17 @@ class Mx4Table:
             return Mx4Table, (*self._store, self.shape)
         return _table_in_one_piece, (self._store, self.shape)
 
+    def __setstate__(self, state):
+        """A table that was saved with its attributes: only its memory and shape are taken, its addresses are another process's."""
+        _, saved = state
+        store, (rows, cols) = saved["_store"], saved["shape"]
+        if store.__class__ is tuple:
+            table = Mx4Table(*store, (rows, cols))
+        else:
+            table = _table_in_one_piece(store, (rows, cols))
+        for name in self.__slots__:
+            setattr(self, name, getattr(table, name))
+
     def _parts(self):
         store = self._store
         if store.__class__ is tuple:

@@ -1,5 +1,6 @@
 """A packed table that is kept: copied, pickled, saved and loaded (``ops.Mx4Table``)."""
 import copy
+import copyreg
 import io
 import pickle
 
@@ -60,6 +61,25 @@ def test_addresses_before_and_after_the_parts_are_looked_at():
     t = ops.Mx4Table._empty(7, 300, "cpu")
     before = (t.codes_ptr, t.scales_ptr, t.device)
     assert before == (t.codes.data_ptr(), t.scales.data_ptr(), t.codes.device) == (t.codes_ptr, t.scales_ptr, t.device)
+
+
+class WithAttributes(pickle.Pickler):
+    """saves a table as its attributes, addresses among them, as tables were saved once"""
+
+    def reducer_override(self, obj):
+        if not isinstance(obj, ops.Mx4Table):
+            return NotImplemented
+        state = {"shape": obj.shape, "device": obj.device, "codes_ptr": 4096, "scales_ptr": 8192, "_store": obj._store}
+        return copyreg.__newobj__, (ops.Mx4Table,), (None, state)
+
+
+@pytest.mark.parametrize("whole", [True, False])
+def test_addresses_in_a_saved_table_are_not_taken(whole):
+    t, buf = host_table(whole), io.BytesIO()
+    WithAttributes(buf, 4).dump(t)
+    c = pickle.loads(buf.getvalue())
+    assert torch.equal(c.codes, t.codes) and torch.equal(c.scales, t.scales) and c.shape == t.shape and c.device == t.device
+    assert (c.codes_ptr, c.scales_ptr) == (c.codes.data_ptr(), c.scales.data_ptr())
 
 
 def test_a_saved_table_is_written_once():
