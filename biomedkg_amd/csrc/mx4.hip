@@ -709,7 +709,8 @@ static int mx4_check_product(int64_t m, int64_t n, int64_t cols, const void* b_c
 template <typename T, bool PACKED, bool KSPLIT>
 static int mx4_few_launch_as(const Mx4Args& a, const Mx4X& x, unsigned blocks, hipStream_t s) {
   const int lds = PACKED ? 0 : a.steps * (2048 + 128);
-  if (lds > (64 << 10)) {                                    // (up to 64 panels, all granted at once)
+  constexpr int SUMS = KSPLIT ? 3 * 16 * 64 * 4 : 4;         // (the kernel's static LDS)
+  if (lds + SUMS > (64 << 10)) {                             // (up to 64 panels, all granted at once)
     static std::atomic<uint64_t> granted{0};
     if (const int rc = grant_lds((const void*)mx4_few_kernel<T, PACKED, KSPLIT>, 64 * 2176, granted, MX_LDS)) return rc;
   }
