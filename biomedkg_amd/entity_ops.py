@@ -258,7 +258,7 @@ class Mx4Table:
     """A ``[rows, cols]`` table in microscaled 4 bits (:func:`mx4_quantize`), in panels of 128 columns (the last one padded
     with zeros): ``codes`` uint8 ``[panels, rows, 64]`` (two columns a byte, the lower one in the low nibble) and ``scales``
     uint8 ``[panels, rows, 4]`` (the exponent of each 32 columns + 127; 255: the block held an infinity or NaN).  0.53 bytes a
-    value."""
+    value.  May be copied, pickled and saved; made of given parts, their memory has to stay where it is."""
     __slots__ = ("shape", "device", "codes_ptr", "scales_ptr", "_store")
 
     def __init__(self, codes, scales, shape):

@@ -145,7 +145,8 @@ class KGEModule(LightningModule):
         """Distil from ``teacher`` (another :class:`KGEModule` over the same nodes and relations, any width): every training
         step adds ``weight`` times the distillation loss of ``queries`` random edges of its batch, each predicting its tail and its
         head out of ALL entities of the batch, against the teacher's ``k`` best entities (:func:`ops.topk_distill_loss`).
-        ``None`` switches it off.  The teacher is frozen and is no part of this module's parameters or state."""
+        ``None`` switches it off; a ``weight`` of 0 keeps the term and adds nothing.  The teacher is frozen and is no part of this
+        module's parameters or state."""
         if teacher is None:
             self._teacher = None
             return
